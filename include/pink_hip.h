@@ -258,6 +258,132 @@ int pink_hip_fill_random_uniform(float *values_out, size_t length, uint32_t seed
 int pink_hip_make_update_factors(uint32_t layout, const uint32_t *dims, uint32_t ndims, uint32_t functor,
                                  float sigma, float damping, float max_update_distance, float *factors_out);
 
+/* ------------------------------------------------------------------------------------------------
+ * Read-out of a trained map.  No counterpart in the reference, which ends at the heatmap: here the
+ * neurons nearest to an image answer a question about it, each with a two-layer model of its own.
+ * Three operators share one handle: images are routed to neurons by their distances (the heatmap of
+ * pink_hip_map_device, or any), the chosen neurons' models are evaluated on the images' features and
+ * added up by their gates, and AdamW trains both.
+ *
+ * All data pointers are device pointers.  Calls are asynchronous on the handle's stream: its own, or
+ * one given with pink_hip_readout_set_stream; inputs made on another stream have to be complete (or
+ * ordered by events) before.  The handle holds a workspace that grows to what its calls need (a call
+ * that makes it grow waits for the stream, allocates, and cannot be captured into a graph:
+ * pink_hip_readout_reserve grows it beforehand).  A handle must not be used from two threads at once.
+ * Results do not depend on the order in which blocks run: the same call gives the same bits.
+ */
+typedef struct pink_hip_readout pink_hip_readout;
+
+/* Element type of features, weights, answers and their gradients.  Distances, gates and the router's
+ * parameters are float32 always; sums are float32 at least. */
+typedef enum { PINK_HIP_ELEMENT_FLOAT = 0, PINK_HIP_ELEMENT_BFLOAT = 1 } pink_hip_element;
+typedef enum { PINK_HIP_SCORE_SOFTMAX = 0, PINK_HIP_SCORE_SIGMOID = 1 } pink_hip_score;
+/* GELU is the exact one (error function); SILU is a * sigmoid(a). */
+typedef enum { PINK_HIP_IDENTITY = 0, PINK_HIP_RELU = 1, PINK_HIP_GELU = 2, PINK_HIP_SILU = 3 } pink_hip_activation;
+
+typedef struct pink_hip_readout_config {
+    uint32_t neurons;        /* N, at most 32768                                                    */
+    uint32_t chosen;         /* k neurons answer for an image; at most 64 and at most N             */
+    uint32_t score;          /* pink_hip_score                                                      */
+    uint32_t renormalise;    /* 1: the gates of an image's chosen neurons add up to one             */
+    uint32_t groups;         /* equal bands of ceil(N / groups) neurons, the last may be shorter    */
+    uint32_t groups_kept;    /* bands that an image's neurons are chosen from                       */
+    uint32_t features;       /* F, H, O: 0, 0, 0 for a handle without models, else each             */
+    uint32_t hidden;         /* at least 1 and at most 2^20                                         */
+    uint32_t outputs;
+    uint32_t activation;     /* pink_hip_activation                                                 */
+    uint32_t element;        /* pink_hip_element                                                    */
+    int32_t  device;         /* HIP device ordinal                                                  */
+} pink_hip_readout_config;
+
+int pink_hip_readout_create(pink_hip_readout **out, const pink_hip_readout_config *cfg);
+/* The argument checks of pink_hip_readout_create without touching a device; message through
+ * pink_hip_readout_last_error(NULL). */
+int pink_hip_readout_check(const pink_hip_readout_config *cfg);
+void pink_hip_readout_destroy(pink_hip_readout *readout);
+/* As pink_hip_last_error. */
+const char *pink_hip_readout_last_error(const pink_hip_readout *readout);
+/* Calls run on `hip_stream` (a hipStream_t of the HIP runtime that this library runs on; NULL is the
+ * default stream) from here on; PINK_HIP_OWN_STREAM goes back to the handle's own.  Waits for what the
+ * handle has queued before.  The stream has to exist until the handle leaves it. */
+#define PINK_HIP_OWN_STREAM ((void *)-1)
+int pink_hip_readout_set_stream(pink_hip_readout *readout, void *hip_stream);
+int pink_hip_readout_synchronize(pink_hip_readout *readout);
+/* Grows the workspace to what any call on so many images needs. */
+int pink_hip_readout_reserve(pink_hip_readout *readout, uint32_t images);
+
+/* Logits z[t][n] = sharpness[n] * (radius[n] - distance[t][n]) as 32-bit numbers (a subtraction and a
+ * product, each rounded).  An entry takes part if z and z + bias are finite, so neurons are masked with
+ * infinite or NaN distances.  Of the groups the `groups_kept` with the largest score are kept, a
+ * group's score being the sum of its two largest z + bias (of the one if no more take part); of their
+ * neurons the k with the largest z + bias are chosen, in that order.  The lowest index goes first on
+ * ties.  Places that no neuron is left for get neuron -1 and gate 0.  The bias (NULL: zero) takes part
+ * in the choice alone.  Gates are the scores
+ *    softmax: exp(z) / sum over all neurons that take part of exp(z);   sigmoid: 1 / (1 + exp(-z));
+ * renormalised, these over their sum over the chosen neurons (formed without overflow or underflow).
+ * distances: images x N, rows distance_stride floats apart (0: N). */
+int pink_hip_readout_route(pink_hip_readout *readout, const float *dev_distances, uint32_t images, uint64_t distance_stride,
+                           const float *dev_sharpness, const float *dev_radius, const float *dev_bias,
+                           int32_t *dev_neuron_out, float *dev_gates_out);
+/* Gradients of the gates: of the distances (images x N, dense), of sharpness and radius (N each,
+ * summed over the images).  Arguments and results of pink_hip_readout_route on the same inputs;
+ * gate_gradients are of the handle's element type.  Any of the outputs may be NULL. */
+int pink_hip_readout_route_backward(pink_hip_readout *readout, const float *dev_distances, uint32_t images, uint64_t distance_stride,
+                                    const float *dev_sharpness, const float *dev_radius, const float *dev_bias,
+                                    const int32_t *dev_neuron, const float *dev_gates, const void *dev_gate_gradients,
+                                    float *dev_distance_gradients_out, float *dev_sharpness_gradients_out, float *dev_radius_gradients_out);
+/* One step towards an even load: a neuron chosen less often than the mean of these images gets
+ * bias + rate, one chosen more often bias - rate.  load_out (may be NULL) receives how often each was. */
+int pink_hip_readout_balance(pink_hip_readout *readout, const int32_t *dev_neuron, uint32_t images, float rate,
+                             float *dev_bias, int32_t *dev_load_out);
+
+/* Weights of all neurons, neuron by neuron, row-major: first H x F, second O x H; biases may be NULL. */
+typedef struct pink_hip_readout_weights {
+    const void *first, *first_bias, *second, *second_bias;
+} pink_hip_readout_weights;
+/* Where gradients go, same shapes; features images x F, gates images x k.  NULL where one is not wanted. */
+typedef struct pink_hip_readout_gradients {
+    void *features, *gates, *first, *first_bias, *second, *second_bias;
+} pink_hip_readout_gradients;
+
+/* y[t] = residual[t] + sum over slots s of gate[t][s] * (second f(first x[t] + first_bias) + second_bias)
+ * with the weights of neuron[t][s]; slots whose neuron is not in [0, N) do not count.  residual may be
+ * NULL, and may be x or y.  Rows are *_stride elements apart (0: dense).  What a backward pass needs is
+ * left in `saved` (pink_hip_readout_saved_bytes(images) bytes, 256-byte aligned) unless it is NULL. */
+size_t pink_hip_readout_saved_bytes(pink_hip_readout *readout, uint32_t images);
+int pink_hip_readout_experts(pink_hip_readout *readout, const void *dev_x, uint32_t images, uint64_t x_stride,
+                             const int32_t *dev_neuron, const float *dev_gates, const pink_hip_readout_weights *dev_weights,
+                             const void *dev_residual, uint64_t residual_stride, void *dev_y, uint64_t y_stride, void *dev_saved);
+/* Gradients for those of y; x, gates and weights as in the forward call that left `saved`.  Weights of
+ * neurons that no image chose get zeros. */
+int pink_hip_readout_experts_backward(pink_hip_readout *readout, const void *dev_x, uint32_t images, uint64_t x_stride,
+                                      const float *dev_gates, const pink_hip_readout_weights *dev_weights, const void *dev_saved,
+                                      const void *dev_y_gradients, uint64_t y_gradient_stride,
+                                      const pink_hip_readout_gradients *dev_gradients_out, uint64_t x_gradient_stride);
+
+/* One trained tensor of an AdamW step.  Pointers need their element's alignment only. */
+typedef struct pink_hip_readout_tensor {
+    float *value;                        /* updated                                                    */
+    const void *gradient;
+    void *rounded;                       /* bfloat16 copy of the updated value; NULL: none              */
+    void *first, *second;                /* states: float32, or int8 and uint8 codes                    */
+    float *first_scale, *second_scale;   /* 8 bits: one for every 256 codes, ceil(size / 256); else unused */
+    float *first_values, *second_values; /* pink_hip_readout_unpack: where the values of the codes go   */
+    uint64_t size;
+    float decay;                         /* weight decay, decoupled                                     */
+    uint32_t gradient_element;           /* pink_hip_element                                            */
+} pink_hip_readout_tensor;
+/* first  = beta_first  * first  + (1 - beta_first)  * gradient
+ * second = beta_second * second + (1 - beta_second) * gradient^2
+ * value -= learning_rate * (c1 first / (sqrt(c2 second) + epsilon) + decay * value),  ci = 1 / (1 - beta_i^step)
+ * in float32, over all tensors at once.  With state_bits 8 the states are held as codes: q in -127..127
+ * is sign(q) (q/127)^2 and q in 0..255 is (q/255)^4 times the scale, the block's largest magnitude (0
+ * where that is below 2^-126); a second state above zero never becomes zero by packing. */
+int pink_hip_readout_adamw(pink_hip_readout *readout, const pink_hip_readout_tensor *tensors, uint32_t count, uint32_t state_bits,
+                           uint64_t step, float learning_rate, float beta_first, float beta_second, float epsilon);
+/* The values that the tensors' 8-bit states stand for, into first_values and second_values. */
+int pink_hip_readout_unpack(pink_hip_readout *readout, const pink_hip_readout_tensor *tensors, uint32_t count);
+
 int pink_hip_abi_version(void);
 
 #ifdef __cplusplus

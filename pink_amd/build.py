@@ -13,7 +13,8 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SOURCES = [os.path.join(HERE, "csrc", "pink_hip.hip"), os.path.join(HERE, "csrc", "update_factors.cpp")]
+SOURCES = [os.path.join(HERE, "csrc", "pink_hip.hip"), os.path.join(HERE, "csrc", "update_factors.cpp"),
+           os.path.join(HERE, "csrc", "readout.hip")]
 # Compiled on its own with the MFMA accumulators in the architectural vector registers: its
 # distance kernel fills all 256 accumulation registers with resident SOM fragments (which the MFMA
 # reads as operands) and post-processes the accumulators on the vector ALU, which cannot read

@@ -22,6 +22,10 @@ CARTESIAN, HEXAGONAL = 0, 1
 STEP, GAUSSIAN, UNITY_GAUSSIAN, MEXICAN_HAT = 0, 1, 2, 3
 NUM_KERNEL_CLASSES = 5
 KERNEL_CLASS_NAMES = ("rotate", "pack", "distance", "update", "finalize")
+ELEMENT_F32, ELEMENT_BF16 = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+ACT_IDENTITY, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
+OWN_STREAM = C.c_void_p(-1).value
 
 EXPORTS = (
     "pink_hip_abi_version", "pink_hip_create", "pink_hip_destroy", "pink_hip_last_error",
@@ -32,6 +36,10 @@ EXPORTS = (
     "pink_hip_make_update_factors", "pink_hip_layout_distances", "pink_hip_shuffled_order",
     "pink_hip_fill_random_uniform", "pink_hip_update_counts", "pink_hip_check_config",
     "pink_hip_map_device_static",
+    "pink_hip_readout_create", "pink_hip_readout_check", "pink_hip_readout_destroy", "pink_hip_readout_last_error",
+    "pink_hip_readout_set_stream", "pink_hip_readout_synchronize", "pink_hip_readout_reserve", "pink_hip_readout_route",
+    "pink_hip_readout_route_backward", "pink_hip_readout_balance", "pink_hip_readout_saved_bytes", "pink_hip_readout_experts",
+    "pink_hip_readout_experts_backward", "pink_hip_readout_adamw", "pink_hip_readout_unpack",
 )
 
 
@@ -49,6 +57,25 @@ class Config(C.Structure):
         ("ed_type", C.c_uint32), ("update_factors", C.POINTER(C.c_float)), ("device", C.c_int32),
         ("max_batch", C.c_uint32), ("kernel_choice", C.c_uint32),
     ]
+
+
+class ReadoutConfig(C.Structure):
+    _fields_ = [(name, C.c_uint32) for name in ("neurons", "chosen", "score", "renormalise", "groups", "groups_kept", "features", "hidden",
+                                                "outputs", "activation", "element")] + [("device", C.c_int32)]
+
+
+class _Weights(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("first", "first_bias", "second", "second_bias")]
+
+
+class _Gradients(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("features", "gates", "first", "first_bias", "second", "second_bias")]
+
+
+class ReadoutTensor(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("value", "gradient", "rounded", "first", "second", "first_scale", "second_scale",
+                                                "first_values", "second_values")] + [
+        ("size", C.c_uint64), ("decay", C.c_float), ("gradient_element", C.c_uint32)]
 
 
 _lib = None
@@ -104,6 +131,25 @@ def lib():
         L.pink_hip_layout_distances.argtypes = [u32, u32p, u32, f32p]
         L.pink_hip_shuffled_order.argtypes = [C.c_uint64, u32, u32p]
         L.pink_hip_fill_random_uniform.argtypes = [f32p, C.c_size_t, u32]
+        u64, f32 = C.c_uint64, C.c_float
+        L.pink_hip_readout_create.argtypes = [C.POINTER(vp), C.POINTER(ReadoutConfig)]
+        L.pink_hip_readout_check.argtypes = [C.POINTER(ReadoutConfig)]
+        L.pink_hip_readout_destroy.argtypes = [vp]
+        L.pink_hip_readout_destroy.restype = None
+        L.pink_hip_readout_last_error.argtypes = [vp]
+        L.pink_hip_readout_last_error.restype = C.c_char_p
+        L.pink_hip_readout_set_stream.argtypes = [vp, vp]
+        L.pink_hip_readout_synchronize.argtypes = [vp]
+        L.pink_hip_readout_reserve.argtypes = [vp, u32]
+        L.pink_hip_readout_route.argtypes = [vp, vp, u32, u64, vp, vp, vp, vp, vp]
+        L.pink_hip_readout_route_backward.argtypes = [vp, vp, u32, u64] + [vp] * 9
+        L.pink_hip_readout_balance.argtypes = [vp, vp, u32, f32, vp, vp]
+        L.pink_hip_readout_saved_bytes.argtypes = [vp, u32]
+        L.pink_hip_readout_saved_bytes.restype = C.c_size_t
+        L.pink_hip_readout_experts.argtypes = [vp, vp, u32, u64, vp, vp, C.POINTER(_Weights), vp, u64, vp, u64, vp]
+        L.pink_hip_readout_experts_backward.argtypes = [vp, vp, u32, u64, vp, C.POINTER(_Weights), vp, vp, u64, C.POINTER(_Gradients), u64]
+        L.pink_hip_readout_adamw.argtypes = [vp, C.POINTER(ReadoutTensor), u32, u32, u64, f32, f32, f32, f32]
+        L.pink_hip_readout_unpack.argtypes = [vp, C.POINTER(ReadoutTensor), u32]
         _lib = L
     return _lib
 
@@ -344,3 +390,116 @@ class Context:
         ms = (C.c_double * NUM_KERNEL_CLASSES)()
         self._check(self._L.pink_hip_kernel_times(self._h, n, ms))
         return {KERNEL_CLASS_NAMES[i]: (int(n[i]), float(ms[i])) for i in range(NUM_KERNEL_CLASSES)}
+
+
+class Readout:
+    """The read-out of a trained map: images routed to neurons by their distances, the chosen neurons' two-layer models, and the
+    optimiser that trains both (the pink_hip_readout_* functions of include/pink_hip.h, which say what each computes).
+
+    All data arguments are device pointers (integers, None for NULL).  Calls are asynchronous: on the handle's own stream, or on the
+    one given to set_stream, e.g. torch.cuda.current_stream().cuda_stream where PyTorch was imported before this library was
+    loaded (they then run on one HIP runtime).  Fence the handle's own stream with synchronize()."""
+
+    def __init__(self, neurons, chosen=1, features=0, hidden=0, outputs=0, score=SCORE_SOFTMAX, renormalise=True, groups=1, groups_kept=1,
+                 activation=ACT_GELU, element=ELEMENT_F32, device=0):
+        self._h = C.c_void_p()
+        self._L = lib()
+        cfg = ReadoutConfig(neurons, chosen, score, int(bool(renormalise)), groups, groups_kept, features, hidden, outputs, activation, element, device)
+        rc = self._L.pink_hip_readout_create(C.byref(self._h), C.byref(cfg))
+        if rc != 0:
+            self._h = C.c_void_p()
+            raise PinkError(rc, self._L.pink_hip_readout_last_error(None).decode())
+        self.neurons, self.chosen, self.features, self.hidden, self.outputs = neurons, chosen, features, hidden, outputs
+
+    @staticmethod
+    def check(neurons, chosen=1, features=0, hidden=0, outputs=0, score=SCORE_SOFTMAX, renormalise=True, groups=1, groups_kept=1,
+              activation=ACT_GELU, element=ELEMENT_F32):
+        """The constructor's argument checks without touching a device."""
+        cfg = ReadoutConfig(neurons, chosen, score, int(bool(renormalise)), groups, groups_kept, features, hidden, outputs, activation, element, 0)
+        rc = lib().pink_hip_readout_check(C.byref(cfg))
+        if rc != 0:
+            raise PinkError(rc, lib().pink_hip_readout_last_error(None).decode())
+
+    def _check(self, rc):
+        if rc != 0:
+            raise PinkError(rc, self._L.pink_hip_readout_last_error(self._h).decode())
+
+    def close(self):
+        if self._h:
+            self._L.pink_hip_readout_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        self.close()
+
+    def set_stream(self, stream):
+        """Calls run on this hipStream_t (an integer; 0 is the default stream) from here on; OWN_STREAM goes back to the handle's own."""
+        self._check(self._L.pink_hip_readout_set_stream(self._h, stream))
+
+    def synchronize(self):
+        self._check(self._L.pink_hip_readout_synchronize(self._h))
+
+    def reserve(self, images):
+        """Grows the workspace to what any call on so many images needs, so that none of them allocates."""
+        self._check(self._L.pink_hip_readout_reserve(self._h, images))
+
+    def route(self, dev_distances, images, dev_sharpness, dev_radius, dev_bias, dev_neuron, dev_gates, distance_stride=0):
+        self._check(self._L.pink_hip_readout_route(self._h, dev_distances, images, distance_stride, dev_sharpness, dev_radius, dev_bias,
+                                                   dev_neuron, dev_gates))
+
+    def route_backward(self, dev_distances, images, dev_sharpness, dev_radius, dev_bias, dev_neuron, dev_gates, dev_gate_gradients,
+                       dev_distance_gradients=None, dev_sharpness_gradients=None, dev_radius_gradients=None, distance_stride=0):
+        self._check(self._L.pink_hip_readout_route_backward(
+            self._h, dev_distances, images, distance_stride, dev_sharpness, dev_radius, dev_bias, dev_neuron, dev_gates, dev_gate_gradients,
+            dev_distance_gradients, dev_sharpness_gradients, dev_radius_gradients))
+
+    def balance(self, dev_neuron, images, rate, dev_bias, dev_load=None):
+        self._check(self._L.pink_hip_readout_balance(self._h, dev_neuron, images, rate, dev_bias, dev_load))
+
+    def saved_bytes(self, images):
+        """Size of the buffer in which experts() leaves what experts_backward() needs."""
+        return int(self._L.pink_hip_readout_saved_bytes(self._h, images))
+
+    def experts(self, dev_x, images, dev_neuron, dev_gates, weights, dev_y, dev_residual=None, dev_saved=None, x_stride=0, residual_stride=0,
+                y_stride=0):
+        """`weights`: pointers to first, first_bias, second, second_bias."""
+        w = _Weights(*weights)
+        self._check(self._L.pink_hip_readout_experts(self._h, dev_x, images, x_stride, dev_neuron, dev_gates, C.byref(w), dev_residual,
+                                                     residual_stride, dev_y, y_stride, dev_saved))
+
+    def experts_backward(self, dev_x, images, dev_gates, weights, dev_saved, dev_y_gradients, gradients, x_stride=0, y_gradient_stride=0,
+                         x_gradient_stride=0):
+        """`gradients`: pointers to where those of features, gates, first, first_bias, second and second_bias go; None where one is not wanted."""
+        w, g = _Weights(*weights), _Gradients(*gradients)
+        self._check(self._L.pink_hip_readout_experts_backward(self._h, dev_x, images, x_stride, dev_gates, C.byref(w), dev_saved, dev_y_gradients,
+                                                              y_gradient_stride, C.byref(g), x_gradient_stride))
+
+    @staticmethod
+    def tensors(described):
+        """The argument of adamw() and adamw_unpack(): one dict for each tensor, with ReadoutTensor's fields as keys (gradient_bf16 in
+        place of gradient_element)."""
+        out = (ReadoutTensor * len(described))()
+        for to, d in zip(out, described):
+            for key, value in d.items():
+                if key == "gradient_bf16":
+                    to.gradient_element = ELEMENT_BF16 if value else ELEMENT_F32
+                else:
+                    setattr(to, key, value)
+        return out
+
+    def adamw(self, tensors, step, learning_rate=1e-3, beta_first=0.9, beta_second=0.999, epsilon=1e-8, bits=32):
+        """One step, the step'th (from 1), over the tensors that tensors() described."""
+        self._check(self._L.pink_hip_readout_adamw(self._h, tensors, len(tensors), bits, step, learning_rate, beta_first, beta_second, epsilon))
+
+    def adamw_unpack(self, tensors):
+        """The values of 8-bit states, into first_values and second_values."""
+        self._check(self._L.pink_hip_readout_unpack(self._h, tensors, len(tensors)))

@@ -1,0 +1,1328 @@
+// readout.hip -- the read-out of a trained map (pink_hip_readout_* of include/pink_hip.h): images routed to neurons by
+// their distances, the neurons' two-layer models, and the optimiser that trains both.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+#include <new>
+
+#include "pink_hip.h"
+
+#include "readout_product.inc"
+
+struct pink_hip_readout {
+    pink_hip_readout_config cfg;
+    hipStream_t own, stream;
+    void *work;
+    size_t work_bytes;
+    char err[320];
+};
+
+namespace {
+
+constexpr uint32_t kMaxNeurons = 32768, kMaxChosen = 64, kMaxGroups = 1024, kMaxSize = 1u << 20;
+constexpr uint32_t kBlock8 = 256;                          // codes that share a scale
+
+thread_local char g_readout_error[320];
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
+{
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, 64));
+    return v;
+}
+
+__device__ __forceinline__ float wave_sum(float v)
+{
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+
+__device__ __forceinline__ float wave_max(float v)
+{
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+    return v;
+}
+
+// ---------------------------------------------------------------------------------
+// Routing
+// ---------------------------------------------------------------------------------
+
+struct RouteArgs {
+    const float *distances;
+    uint64_t stride;
+    const float *sharpness, *radius, *bias;
+    uint32_t images, neurons, chosen, groups, groups_kept, group_size;
+    uint32_t sigmoid, renormalise;
+    int32_t *neuron;
+    float *gates;
+};
+
+// An entry's key in the choice: a number that grows with z + bias, 0 where the entry takes no part.
+__device__ __forceinline__ uint32_t order_key(float z, float biased)
+{
+    if (!isfinite(z) || !isfinite(biased)) return 0;
+    const uint32_t bits = __float_as_uint(biased + 0.0f);  // (-0 and 0 tie)
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+
+__device__ __forceinline__ float key_value(uint32_t key)
+{
+    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+__device__ __forceinline__ float logit(const RouteArgs &g, const float *row, uint32_t n)
+{
+    return g.sharpness[n] * (g.radius[n] - row[n]);
+}
+
+// Gates of an image's chosen neurons, a lane each (at most 64); `z` of a lane without a neuron does not count.
+__device__ __forceinline__ float gate_of(const RouteArgs &g, float z, bool valid, float top, float total)
+{
+    if (g.renormalise) {
+        const float level = g.sigmoid ? fminf(z, 0.0f) - log1pf(expf(-fabsf(z))) : z;
+        const float highest = wave_max(valid ? level : -INFINITY);
+        const float e = valid ? expf(level - highest) : 0.0f;
+        const float sum = wave_sum(e);
+        return valid ? e / sum : 0.0f;
+    }
+    if (!valid) return 0.0f;
+    return g.sigmoid ? 1.0f / (1.0f + expf(-z)) : expf(z - top) / total;
+}
+
+// The general form, a block per image: keys in LDS, the groups kept by counting how many go before each, then the largest key
+// `chosen` times.
+__global__ __launch_bounds__(256) void k_route_block(const RouteArgs g)
+{
+    extern __shared__ __align__(16) uint32_t lds[];
+    uint32_t *const keys = lds, *const group_keys = lds + g.neurons;     // neurons, groups
+    __shared__ uint32_t best_key[4], best_at[4];
+    __shared__ float wave_top[4], wave_total[4];
+    __shared__ int32_t picked[kMaxChosen];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float *const row = g.distances + (uint64_t)blockIdx.x * g.stride;
+
+    float top = -INFINITY;
+    for (uint32_t n = tid; n < g.neurons; n += 256) {
+        const float z = logit(g, row, n), biased = g.bias ? z + g.bias[n] : z;
+        const uint32_t key = order_key(z, biased);
+        keys[n] = key;
+        if (key) top = fmaxf(top, z);
+    }
+    top = wave_max(top);
+    if (lane == 0) wave_top[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+    float total = 0.0f;
+    if (!g.renormalise && !g.sigmoid) {
+        for (uint32_t n = tid; n < g.neurons; n += 256)
+            if (keys[n]) total += expf(logit(g, row, n) - top);
+        total = wave_sum(total);
+        if (lane == 0) wave_total[wave] = total;
+        __syncthreads();
+        total = (wave_total[0] + wave_total[1]) + (wave_total[2] + wave_total[3]);
+    }
+
+    if (g.groups > 1) {
+        for (uint32_t k = wave; k < g.groups; k += 4) {
+            uint32_t first = 0, second = 0;
+            const uint32_t end = min((k + 1) * g.group_size, g.neurons);
+            for (uint32_t n = k * g.group_size + lane; n < end; n += 64) {
+                const uint32_t key = keys[n];
+                second = max(second, min(first, key));
+                first = max(first, key);
+            }
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) {
+                const uint32_t a = __shfl_xor((int)first, off, 64), b = __shfl_xor((int)second, off, 64);
+                second = max(max(second, b), min(first, a));
+                first = max(first, a);
+            }
+            if (lane == 0) {
+                uint32_t key = first;
+                if (second) {
+                    const float both = key_value(first) + key_value(second);
+                    key = order_key(0.0f, fminf(fmaxf(both, -3.402823466e38f), 3.402823466e38f));
+                }
+                group_keys[k] = key;
+            }
+        }
+        __syncthreads();
+        for (uint32_t n = tid; n < g.neurons; n += 256) {
+            const uint32_t mine = n / g.group_size, key = group_keys[mine];
+            uint32_t before = 0;
+            for (uint32_t k = 0; k < g.groups; ++k) before += group_keys[k] > key || (group_keys[k] == key && k < mine);
+            if (before >= g.groups_kept) keys[n] = 0;
+        }
+        __syncthreads();
+    }
+
+    for (uint32_t s = 0; s < g.chosen; ++s) {
+        uint32_t key = 0, at = 0xffffffffu;
+        for (uint32_t n = tid; n < g.neurons; n += 256)
+            if (keys[n] > key) {
+                key = keys[n];
+                at = n;
+            }
+        const uint32_t highest = wave_max_u32(key);
+        const uint32_t lowest = ~wave_max_u32(key == highest && key ? ~at : 0u);
+        if (lane == 0) {
+            best_key[wave] = highest;
+            best_at[wave] = lowest;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            uint32_t k = 0, a = 0xffffffffu;
+            for (int w = 0; w < 4; ++w)
+                if (best_key[w] > k || (best_key[w] == k && best_at[w] < a)) {
+                    k = best_key[w];
+                    a = best_at[w];
+                }
+            picked[s] = k ? (int32_t)a : -1;
+            if (k) keys[a] = 0;
+        }
+        __syncthreads();
+    }
+    if (wave == 0) {
+        const int32_t n = lane < g.chosen ? picked[lane] : -1;
+        const float gate = gate_of(g, n >= 0 ? logit(g, row, n) : 0.0f, n >= 0, top, total);
+        if (lane < g.chosen) {
+            g.neuron[(uint64_t)blockIdx.x * g.chosen + lane] = n;
+            g.gates[(uint64_t)blockIdx.x * g.chosen + lane] = gate;
+        }
+    }
+}
+
+struct RouteBackwardArgs {
+    RouteArgs r;                   // neuron and gates are inputs here
+    const void *gate_gradients;
+    float *distance_gradients;
+    float *sharpness_part, *radius_part;       // chunks x N each
+    uint32_t chunk;                // images of a block
+    uint32_t want_sums;
+};
+
+constexpr uint32_t kChunkMost = 64;
+
+// Gradients of a chunk of images over a strip of 256 neurons.  Waves first form each image's own numbers: dz of its chosen
+// neurons and, for the full softmax, its normaliser and what every neuron's share is multiplied with.  Then a thread goes
+// down its neuron's column, in the images' order.
+//   renormalised: dz_c = g_c (G_c - sum_s g_s G_s) [sigmoid: times 1 - sigmoid(z_c)];  sigmoid: dz_c = G_c s (1 - s);
+//   softmax: dz_n = [n chosen] g_n G_n - share_n sum_s g_s G_s
+template <typename E> __global__ __launch_bounds__(256) void k_route_backward(const RouteBackwardArgs a)
+{
+    const RouteArgs &g = a.r;
+    extern __shared__ __align__(16) char lds_raw[];
+    float *const dz = (float *)lds_raw;                                  // chunk x chosen
+    int32_t *const at = (int32_t *)(dz + a.chunk * g.chosen);            // chunk x chosen
+    __shared__ float top_of[kChunkMost], over_of[kChunkMost], pull_of[kChunkMost];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t t0 = blockIdx.y * a.chunk, count = min(a.chunk, g.images - t0);
+    const bool full = !g.sigmoid && !g.renormalise;
+
+    for (uint32_t i = wave; i < count; i += 4) {
+        const uint64_t slot = (uint64_t)(t0 + i) * g.chosen + lane;
+        const float *const row = g.distances + (uint64_t)(t0 + i) * g.stride;
+        const int32_t n = lane < g.chosen ? g.neuron[slot] : -1;
+        const bool valid = n >= 0 && (uint32_t)n < g.neurons;
+        const float gate = valid ? g.gates[slot] : 0.0f, grad = valid ? to_float(((const E *)a.gate_gradients)[slot]) : 0.0f;
+        const float z = valid ? logit(g, row, n) : 0.0f;
+        const float pull = wave_sum(gate * grad);
+        float d;
+        if (g.renormalise) {
+            d = gate * (grad - pull);
+            if (g.sigmoid) d /= 1.0f + expf(z);
+        } else {
+            d = gate * grad;
+            if (g.sigmoid) d /= 1.0f + expf(z);
+        }
+        if (lane < g.chosen) {
+            dz[i * g.chosen + lane] = valid ? d : 0.0f;
+            at[i * g.chosen + lane] = valid ? n : -1;
+        }
+        if (full) {
+            float top = -INFINITY, total = 0.0f;
+            for (uint32_t m = lane; m < g.neurons; m += 64) {
+                const float v = logit(g, row, m);
+                if (order_key(v, g.bias ? v + g.bias[m] : v)) top = fmaxf(top, v);
+            }
+            top = wave_max(top);
+            for (uint32_t m = lane; m < g.neurons; m += 64) {
+                const float v = logit(g, row, m);
+                if (order_key(v, g.bias ? v + g.bias[m] : v)) total += expf(v - top);
+            }
+            total = wave_sum(total);
+            if (lane == 0) {
+                top_of[i] = top;
+                over_of[i] = total > 0.0f ? 1.0f / total : 0.0f;
+                pull_of[i] = pull;
+            }
+        }
+    }
+    __syncthreads();
+
+    const uint32_t n = blockIdx.x * 256 + tid;
+    if (n >= g.neurons) return;
+    const float sharpness = g.sharpness[n], radius = g.radius[n], bias = g.bias ? g.bias[n] : 0.0f;
+    float of_sharpness = 0.0f, of_radius = 0.0f;
+    for (uint32_t i = 0; i < count; ++i) {
+        const uint64_t place = (uint64_t)(t0 + i) * g.stride + n;
+        float d = 0.0f;
+        if (full) {
+            const float v = sharpness * (radius - g.distances[place]);
+            if (order_key(v, v + bias)) d = -pull_of[i] * (expf(v - top_of[i]) * over_of[i]);
+        }
+        for (uint32_t s = 0; s < g.chosen; ++s)
+            if (at[i * g.chosen + s] == (int32_t)n) d += dz[i * g.chosen + s];
+        if (a.distance_gradients) a.distance_gradients[(uint64_t)(t0 + i) * g.neurons + n] = -sharpness * d;
+        if (d != 0.0f) {
+            of_sharpness += d * (radius - g.distances[place]);
+            of_radius += sharpness * d;
+        }
+    }
+    if (a.want_sums) {
+        a.sharpness_part[(uint64_t)blockIdx.y * g.neurons + n] = of_sharpness;
+        a.radius_part[(uint64_t)blockIdx.y * g.neurons + n] = of_radius;
+    }
+}
+
+// Column sums of the chunks' parts: 64 columns by 4 waves, each a quarter of the chunks in order.
+__global__ __launch_bounds__(256) void k_route_sums(const float *sharpness_part, const float *radius_part, uint32_t chunks, uint32_t neurons,
+                                                    float *sharpness_out, float *radius_out)
+{
+    __shared__ float held[2][4][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
+    const uint32_t each = (chunks + 3) / 4, first = wave * each, end = min(first + each, chunks);
+    float s = 0.0f, r = 0.0f;
+    if (n < neurons)
+        for (uint32_t c = first; c < end; ++c) {
+            s += sharpness_part[(uint64_t)c * neurons + n];
+            r += radius_part[(uint64_t)c * neurons + n];
+        }
+    held[0][wave][lane] = s;
+    held[1][wave][lane] = r;
+    __syncthreads();
+    if (wave || n >= neurons) return;
+    if (sharpness_out) sharpness_out[n] = (held[0][0][lane] + held[0][1][lane]) + (held[0][2][lane] + held[0][3][lane]);
+    if (radius_out) radius_out[n] = (held[1][0][lane] + held[1][1][lane]) + (held[1][2][lane] + held[1][3][lane]);
+}
+
+// One block: how often each neuron was chosen, then a step of the bias against the mean.
+__global__ __launch_bounds__(1024) void k_balance(const int32_t *neuron, uint64_t slots, uint32_t neurons, float rate, float *bias, int32_t *load)
+{
+    extern __shared__ __align__(16) uint32_t counts[];
+    __shared__ uint32_t used;
+    for (uint32_t n = threadIdx.x; n < neurons; n += 1024) counts[n] = 0;
+    if (threadIdx.x == 0) used = 0;
+    __syncthreads();
+    uint32_t mine = 0;
+    for (uint64_t i = threadIdx.x; i < slots; i += 1024) {
+        const uint32_t n = (uint32_t)neuron[i];
+        if (n < neurons) {
+            atomicAdd(&counts[n], 1u);
+            ++mine;
+        }
+    }
+    if (mine) atomicAdd(&used, mine);
+    __syncthreads();
+    for (uint32_t n = threadIdx.x; n < neurons; n += 1024) {
+        const uint64_t mean = used, now = (uint64_t)counts[n] * neurons;            // both times N: exact
+        bias[n] += now < mean ? rate : now > mean ? -rate : 0.0f;
+        if (load) load[n] = (int32_t)counts[n];
+    }
+}
+
+// ---------------------------------------------------------------------------------
+// Rows sorted by neuron
+// ---------------------------------------------------------------------------------
+
+// A stable counting sort of the slots by neuron.  A block takes waves * 64 * kPerWave slots in order; a wave goes through its
+// own in order with a histogram of its own, so that ranks need no atomics and the order is that of the images always.
+constexpr uint32_t kPerWave = 4;
+
+struct PlanArgs {
+    const int32_t *neuron;
+    uint32_t slots, neurons, tile_rows;
+    uint32_t *counts;              // blocks x N
+    uint32_t *order, *offsets, *tile_count;
+    int32_t *place;                // slot -> row, -1 where it has none
+    uint2 *tiles;
+};
+
+// Exclusive prefix sums over the block of one 64-bit value a thread.
+__device__ __forceinline__ unsigned long long block_prefix(unsigned long long v, unsigned long long *shared, unsigned long long *total)
+{
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    unsigned long long sum = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const unsigned long long o = __shfl_up(sum, off, 64);
+        if ((int)lane >= off) sum += o;
+    }
+    if (lane == 63) shared[wave] = sum;
+    __syncthreads();
+    unsigned long long before = 0, all = 0;
+    for (uint32_t w = 0; w < waves; ++w) {
+        if (w < wave) before += shared[w];
+        all += shared[w];
+    }
+    __syncthreads();
+    *total = all;
+    return before + sum - v;
+}
+
+// First rows and tiles of all neurons from their numbers of rows: rows in the low half, tiles in the high half of one sum.
+template <typename Count> __device__ __forceinline__ void plan_offsets(const PlanArgs &g, const Count &count, unsigned long long *shared)
+{
+    const uint32_t each = (g.neurons + blockDim.x - 1) / blockDim.x;
+    const uint32_t first = min(threadIdx.x * each, g.neurons), end = min(first + each, g.neurons);
+    unsigned long long mine = 0, total;
+    for (uint32_t n = first; n < end; ++n) {
+        const uint32_t c = count(n);
+        mine += c | (unsigned long long)((c + g.tile_rows - 1) / g.tile_rows) << 32;
+    }
+    unsigned long long at = block_prefix(mine, shared, &total);
+    for (uint32_t n = first; n < end; ++n) {
+        const uint32_t c = count(n);
+        g.offsets[n] = (uint32_t)at;
+        uint32_t tile = (uint32_t)(at >> 32);
+        for (uint32_t r = 0; r < c; r += g.tile_rows) g.tiles[tile++] = make_uint2(n, (uint32_t)at + r);
+        at += c | (unsigned long long)((c + g.tile_rows - 1) / g.tile_rows) << 32;
+    }
+    if (threadIdx.x == 0) {
+        g.offsets[g.neurons] = (uint32_t)total;
+        *g.tile_count = (uint32_t)(total >> 32);
+    }
+}
+
+// STAGE 0: count only; 1: place rows, from counts' prefixes; 2: all in one block.
+template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanArgs g)
+{
+    extern __shared__ __align__(16) uint32_t hist[];       // waves x N
+    __shared__ unsigned long long shared[16];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    for (uint32_t i = threadIdx.x; i < waves * g.neurons; i += blockDim.x) hist[i] = 0;
+    __syncthreads();
+    volatile uint32_t *const mine = hist + wave * g.neurons;
+    const uint64_t first = ((uint64_t)blockIdx.x * waves + wave) * 64 * kPerWave;
+    uint32_t rank[kPerWave], id[kPerWave];
+#pragma unroll
+    for (uint32_t i = 0; i < kPerWave; ++i) {
+        const uint64_t slot = first + i * 64 + lane;
+        id[i] = slot < g.slots ? (uint32_t)g.neuron[slot] : 0xffffffffu;
+        const bool valid = id[i] < g.neurons;
+        unsigned long long same = __ballot(valid);
+        for (uint32_t b = 0; (g.neurons - 1) >> b; ++b) {
+            const unsigned long long set = __ballot(id[i] >> b & 1);
+            same &= id[i] >> b & 1 ? set : ~set;
+        }
+        const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+        rank[i] = valid ? mine[id[i]] + below : 0;
+        __builtin_amdgcn_wave_barrier();
+        if (valid && below == 0) mine[id[i]] = rank[i] + __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    for (uint32_t n = threadIdx.x; n < g.neurons; n += blockDim.x) {
+        uint32_t before = 0;
+        for (uint32_t w = 0; w < waves; ++w) {
+            const uint32_t c = hist[w * g.neurons + n];
+            hist[w * g.neurons + n] = before;
+            before += c;
+        }
+        if (STAGE != 1) g.counts[(uint64_t)blockIdx.x * g.neurons + n] = before;
+    }
+    if (STAGE == 0) return;
+    __syncthreads();                                       // (counts and offsets go through memory, within the block)
+    if (STAGE == 2) {
+        plan_offsets(g, [&](uint32_t n) { return g.counts[n]; }, shared);
+        __syncthreads();
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kPerWave; ++i) {
+        const uint64_t slot = first + i * 64 + lane;
+        if (slot >= g.slots) continue;
+        int32_t row = -1;
+        if (id[i] < g.neurons) {
+            row = (int32_t)(g.offsets[id[i]] + hist[wave * g.neurons + id[i]] + rank[i]);
+            if (STAGE == 1) row += (int32_t)g.counts[(uint64_t)blockIdx.x * g.neurons + id[i]];
+            g.order[row] = (uint32_t)slot;
+        }
+        g.place[slot] = row;
+    }
+}
+
+// One block: every block's counts become the rows of its neuron that lie in blocks before; first rows and tiles.
+__global__ __launch_bounds__(1024) void k_plan_offsets(const PlanArgs g, uint32_t blocks, uint32_t *totals)
+{
+    __shared__ unsigned long long shared[16];
+    for (uint32_t n = threadIdx.x; n < g.neurons; n += blockDim.x) {
+        uint32_t before = 0;
+        for (uint32_t b = 0; b < blocks; ++b) {
+            const uint32_t c = g.counts[(uint64_t)b * g.neurons + n];
+            g.counts[(uint64_t)b * g.neurons + n] = before;
+            before += c;
+        }
+        totals[n] = before;
+    }
+    __syncthreads();
+    plan_offsets(g, [&](uint32_t n) { return totals[n]; }, shared);
+}
+
+// ---------------------------------------------------------------------------------
+// Rows back to images, gradients of gates and biases
+// ---------------------------------------------------------------------------------
+
+// out[t] = residual[t] + the sum of the image's rows, in the order of its slots.
+template <typename E>
+__global__ __launch_bounds__(256) void k_combine(const float *rows, const int32_t *place, uint32_t images, uint32_t chosen, uint32_t cols,
+                                                 const E *residual, uint64_t residual_stride, E *out, uint64_t out_stride)
+{
+    const uint64_t n = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t t = n / cols;
+    const uint32_t c = (uint32_t)(n - t * cols);
+    if (t >= images) return;
+    float v = residual ? to_float(residual[t * residual_stride + c]) : 0.0f;
+    for (uint32_t s = 0; s < chosen; ++s)
+        if (place[t * chosen + s] >= 0) v += rows[(t * chosen + s) * cols + c];
+    out[t * out_stride + c] = from_float<E>(v);
+}
+
+// d gate of a slot = dy . (W2 f(a) + b2) = sum of its row's parts + dy . b2; a wave per slot.
+template <typename E>
+__global__ __launch_bounds__(256) void k_gate_gradients(const float *partial, uint32_t parts, const int32_t *place, const uint32_t *offsets,
+                                                        uint32_t neurons, uint64_t slots, uint32_t chosen, const E *dy, uint64_t dy_stride,
+                                                        uint32_t cols, const E *bias, E *out)
+{
+    const uint64_t slot = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63;
+    if (slot >= slots) return;
+    const int32_t row = place[slot];
+    float v = 0.0f;
+    if (row >= 0) {
+        for (uint32_t i = lane; i < parts; i += 64) v += partial[(uint64_t)row * parts + i];
+        if (bias) {
+            uint32_t lo = 0, hi = neurons;                 // the last neuron that starts at or before the row
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (offsets[mid] <= (uint32_t)row) lo = mid;
+                else hi = mid;
+            }
+            const E *const d = dy + slot / chosen * dy_stride;
+            for (uint32_t c = lane; c < cols; c += 64) v += to_float(d[c]) * to_float(bias[(uint64_t)lo * cols + c]);
+        }
+    }
+    v = wave_sum(v);
+    if (lane == 0) out[slot] = from_float<E>(v);
+}
+
+// Gradients of a layer's biases: the sum of a neuron's rows, gated and by image for the second layer.
+template <typename E, bool SECOND>
+__global__ __launch_bounds__(256) void k_bias_gradients(const E *rows, uint64_t stride, const uint32_t *order, const uint32_t *offsets, uint32_t chosen,
+                                                        const float *gates, uint32_t cols, E *out)
+{
+    const uint32_t neuron = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    float v = 0.0f;
+    for (uint32_t r = offsets[neuron]; r < offsets[neuron + 1]; ++r) {
+        if (SECOND) v += gates[order[r]] * to_float(rows[order[r] / chosen * stride + c]);
+        else v += to_float(rows[(uint64_t)r * stride + c]);
+    }
+    out[(uint64_t)neuron * cols + c] = from_float<E>(v);
+}
+
+// Zeros, by a kernel: a recorded memset has not always been replayed right in graphs.
+__global__ __launch_bounds__(256) void k_clear(uint8_t *at, uint64_t bytes)
+{
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < bytes; i += (uint64_t)gridDim.x * 256) at[i] = 0;
+}
+
+// ---------------------------------------------------------------------------------
+// AdamW
+// ---------------------------------------------------------------------------------
+
+constexpr uint32_t kAdamTensors = 32, kAdamChunk = 2048;   // tensors of a launch (their table is a kernel argument), values of a block
+
+struct AdamArgs {
+    pink_hip_readout_tensor tensor[kAdamTensors];
+    uint32_t first_block[kAdamTensors + 1];
+    uint32_t count;
+    float rate, beta1, rest1, beta2, rest2, c1, c2, epsilon;
+};
+
+__device__ __forceinline__ uint32_t adam_tensor(const AdamArgs &g)
+{
+    uint32_t i = 0;
+    while (i + 1 < g.count && blockIdx.x >= g.first_block[i + 1]) ++i;
+    return i;
+}
+
+template <typename V, int N> struct Run {                  // N values at their own alignment
+    V v[N];
+};
+
+template <typename V> __device__ __forceinline__ void load_run(V (&v)[8], const V *at, uint32_t valid)
+{
+    if (valid >= 8) {
+        __builtin_memcpy(v, at, sizeof v);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) v[i] = i < valid ? at[i] : V{};
+    }
+}
+
+template <typename V> __device__ __forceinline__ void store_run(V *at, const V (&v)[8], uint32_t valid)
+{
+    if (valid >= 8) {
+        __builtin_memcpy(at, v, sizeof v);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+            if (i < valid) at[i] = v[i];
+    }
+}
+
+__device__ __forceinline__ float first_value(int8_t code, float scale)
+{
+    const float u = (float)code * (1.0f / 127);
+    return (u * fabsf(u)) * scale;
+}
+
+__device__ __forceinline__ float second_value(uint8_t code, float scale)
+{
+    float u = (float)code * (1.0f / 255);
+    u = u * u;
+    return (u * u) * scale;
+}
+
+// The largest of the 32 lanes that hold one block of codes.
+__device__ __forceinline__ float half_wave_max(float v)
+{
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+    return v;
+}
+
+// A thread has eight neighbouring values, so a block of 256 codes belongs to half a wave.
+template <bool CODES> __global__ __launch_bounds__(256) void k_adamw(const AdamArgs g)
+{
+    const uint32_t which = adam_tensor(g);
+    const pink_hip_readout_tensor &t = g.tensor[which];
+    const uint64_t at = (uint64_t)(blockIdx.x - g.first_block[which]) * kAdamChunk + threadIdx.x * 8;
+    const uint32_t valid = at >= t.size ? 0 : (uint32_t)min((uint64_t)8, t.size - at);
+    if (__ballot(valid != 0) == 0) return;
+
+    float p[8], d[8], m[8], v[8];
+    load_run(p, t.value + at, valid);
+    if (t.gradient_element == PINK_HIP_ELEMENT_BFLOAT) {
+        Bfloat b[8];
+        load_run(b, (const Bfloat *)t.gradient + at, valid);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = to_float(b[i]);
+    } else {
+        load_run(d, (const float *)t.gradient + at, valid);
+    }
+    const uint64_t block = at / kBlock8;
+    if constexpr (CODES) {
+        int8_t mc[8];
+        uint8_t vc[8];
+        load_run(mc, (const int8_t *)t.first + at, valid);
+        load_run(vc, (const uint8_t *)t.second + at, valid);
+        const float ms = valid ? t.first_scale[block] : 0.0f, vs = valid ? t.second_scale[block] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            m[i] = first_value(mc[i], ms);
+            v[i] = second_value(vc[i], vs);
+        }
+    } else {
+        load_run(m, (const float *)t.first + at, valid);
+        load_run(v, (const float *)t.second + at, valid);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        m[i] = m[i] * g.beta1 + d[i] * g.rest1;
+        v[i] = v[i] * g.beta2 + (d[i] * d[i]) * g.rest2;
+        const float step = (m[i] * g.c1) / (sqrtf(v[i] * g.c2) + g.epsilon);
+        p[i] = p[i] - (step + p[i] * t.decay) * g.rate;
+    }
+    store_run(t.value + at, p, valid);
+    if (t.rounded) {
+        Bfloat b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = from_float<Bfloat>(p[i]);
+        store_run((Bfloat *)t.rounded + at, b, valid);
+    }
+    if constexpr (CODES) {
+        float ms = 0.0f, vs = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            ms = fmaxf(ms, fabsf(m[i]));                   // (values past the end are zero)
+            vs = fmaxf(vs, fabsf(v[i]));
+        }
+        ms = half_wave_max(ms);
+        vs = half_wave_max(vs);
+        ms = ms < 1.175494351e-38f ? 0.0f : ms;
+        vs = vs < 1.175494351e-38f ? 0.0f : vs;
+        const float mi = ms > 0.0f ? 1.0f / ms : 0.0f, vi = vs > 0.0f ? 1.0f / vs : 0.0f;
+        int8_t mc[8];
+        uint8_t vc[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float code = rintf(sqrtf(fabsf(m[i]) * mi) * 127.0f);
+            mc[i] = (int8_t)(int)(m[i] < 0.0f ? -code : code);
+            const float ratio = fabsf(v[i]) * vi, root = rintf(sqrtf(sqrtf(ratio)) * 255.0f);
+            vc[i] = (uint8_t)(int)(ratio > 0.0f ? fmaxf(root, 1.0f) : root);
+        }
+        store_run((int8_t *)t.first + at, mc, valid);
+        store_run((uint8_t *)t.second + at, vc, valid);
+        if (valid && at % kBlock8 == 0) {
+            t.first_scale[block] = ms;
+            t.second_scale[block] = vs;
+        }
+    } else {
+        store_run((float *)t.first + at, m, valid);
+        store_run((float *)t.second + at, v, valid);
+    }
+}
+
+__global__ __launch_bounds__(256) void k_unpack(const AdamArgs g)
+{
+    const uint32_t which = adam_tensor(g);
+    const pink_hip_readout_tensor &t = g.tensor[which];
+    const uint64_t at = (uint64_t)(blockIdx.x - g.first_block[which]) * kAdamChunk + threadIdx.x * 8;
+    if (at >= t.size) return;
+    const uint32_t valid = (uint32_t)min((uint64_t)8, t.size - at);
+    int8_t mc[8];
+    uint8_t vc[8];
+    load_run(mc, (const int8_t *)t.first + at, valid);
+    load_run(vc, (const uint8_t *)t.second + at, valid);
+    const float ms = t.first_scale[at / kBlock8], vs = t.second_scale[at / kBlock8];
+    float m[8], v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        m[i] = first_value(mc[i], ms);
+        v[i] = second_value(vc[i], vs);
+    }
+    store_run(t.first_values + at, m, valid);
+    store_run(t.second_values + at, v, valid);
+}
+
+// ---------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------
+
+int fail(pink_hip_readout *r, int code, const char *what, const char *why = nullptr)
+{
+    char *const to = r ? r->err : g_readout_error;
+    std::snprintf(to, 320, why ? "%s: %s" : "%s", what, why);
+    return code;
+}
+
+#define HIP_TRY(r, call)                                                                                              \
+    do {                                                                                                              \
+        const hipError_t e_ = (call);                                                                                 \
+        if (e_ != hipSuccess)                                                                                         \
+            return fail(r, e_ == hipErrorOutOfMemory ? PINK_HIP_ENOMEM : PINK_HIP_EDEVICE, #call, hipGetErrorString(e_)); \
+    } while (0)
+
+#define TRY(expr)                            \
+    do {                                     \
+        const int rc_ = (expr);              \
+        if (rc_ != PINK_HIP_OK) return rc_;  \
+    } while (0)
+
+#define REFUSE(r, condition, what)                                   \
+    do {                                                             \
+        if (condition) return fail(r, PINK_HIP_EINVAL, what);        \
+    } while (0)
+
+int launched(pink_hip_readout *r, const char *what)
+{
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? PINK_HIP_OK : fail(r, PINK_HIP_EDEVICE, what, hipGetErrorString(e));
+}
+
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+size_t element_bytes(const pink_hip_readout *r) { return r->cfg.element == PINK_HIP_ELEMENT_BFLOAT ? 2 : 4; }
+
+uint32_t group_size(const pink_hip_readout_config &c) { return (c.neurons + c.groups - 1) / c.groups; }
+
+int grow(pink_hip_readout *r, size_t bytes)
+{
+    if (bytes <= r->work_bytes) return PINK_HIP_OK;
+    HIP_TRY(r, hipStreamSynchronize(r->stream));
+    if (r->work) HIP_TRY(r, hipFree(r->work));
+    r->work = nullptr;
+    r->work_bytes = 0;
+    HIP_TRY(r, hipMalloc(&r->work, bytes));
+    r->work_bytes = bytes;
+    return PINK_HIP_OK;
+}
+
+// What a forward call leaves for the backward one, and where.
+struct Saved {
+    size_t order, place, offsets, tile_count, tiles, before, after, bytes;
+    uint64_t stride;               // of before's and after's rows: whole 16-byte chunks
+};
+
+constexpr uint32_t kLeastTileRows = 128;
+
+Saved saved_layout(const pink_hip_readout *r, uint64_t images)
+{
+    const pink_hip_readout_config &c = r->cfg;
+    const size_t e = element_bytes(r), slots = images * c.chosen;
+    Saved s;
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += align256(bytes);
+        return here;
+    };
+    s.stride = (c.hidden + 16 / e - 1) / (16 / e) * (16 / e);
+    s.order = take(slots * 4);
+    s.place = take(slots * 4);
+    s.offsets = take(((size_t)c.neurons + 1) * 4);
+    s.tile_count = take(4);
+    s.tiles = take((slots / kLeastTileRows + std::min<size_t>(c.neurons, slots)) * sizeof(uint2));
+    s.after = take(slots * s.stride * e);
+    s.before = take(slots * s.stride * e);
+    s.bytes = at;
+    return s;
+}
+
+uint32_t plan_waves(uint32_t neurons) { return std::max(1u, std::min(16u, 32768u / neurons)); }
+
+struct Work {
+    size_t counts, totals, rows, partial, saved, bytes;
+};
+
+Work work_layout(const pink_hip_readout *r, uint64_t images)
+{
+    const pink_hip_readout_config &c = r->cfg;
+    const size_t slots = images * c.chosen, plan_blocks = (slots + plan_waves(c.neurons) * 64 * kPerWave - 1) / (plan_waves(c.neurons) * 64 * kPerWave);
+    Work w;
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += align256(bytes);
+        return here;
+    };
+    w.counts = take(plan_blocks * c.neurons * 4);
+    w.totals = take((size_t)c.neurons * 4);
+    w.rows = take(slots * std::max(c.features, c.outputs) * 4);
+    w.partial = take(slots * ((c.hidden + 31) / 32) * 4);
+    w.saved = take(saved_layout(r, images).bytes);         // forward calls that keep nothing; gradients of `before`
+    w.bytes = at;
+    return w;
+}
+
+int check(const pink_hip_readout_config *c, pink_hip_readout *r)
+{
+    REFUSE(r, !c, "pink_hip_readout: null argument");
+    REFUSE(r, c->neurons == 0 || c->neurons > kMaxNeurons, "Number of neurons must be between 1 and 32768");
+    REFUSE(r, c->chosen == 0 || c->chosen > kMaxChosen || c->chosen > c->neurons, "Number of chosen neurons must be between 1 and 64 and not larger than the number of neurons");
+    REFUSE(r, c->score > PINK_HIP_SCORE_SIGMOID, "unknown score");
+    REFUSE(r, c->renormalise > 1, "renormalise must be 0 or 1");
+    REFUSE(r, c->groups == 0 || c->groups > kMaxGroups || c->groups > c->neurons, "Number of groups must be between 1 and 1024 and not larger than the number of neurons");
+    REFUSE(r, (uint64_t)(c->groups - 1) * group_size(*c) >= c->neurons, "Number of groups leaves a group without neurons");
+    REFUSE(r, c->groups_kept == 0 || c->groups_kept > c->groups, "Number of kept groups must be between 1 and the number of groups");
+    REFUSE(r, c->activation > PINK_HIP_SILU, "unknown activation");
+    REFUSE(r, c->element > PINK_HIP_ELEMENT_BFLOAT, "unknown element type");
+    const bool models = c->features || c->hidden || c->outputs;
+    REFUSE(r, models && (!c->features || !c->hidden || !c->outputs), "features, hidden and outputs must be all zero or none");
+    REFUSE(r, c->features > kMaxSize || c->hidden > kMaxSize || c->outputs > kMaxSize, "features, hidden and outputs must be at most 1048576");
+    return PINK_HIP_OK;
+}
+
+RouteArgs route_args(const pink_hip_readout *r, const float *distances, uint32_t images, uint64_t stride, const float *sharpness,
+                     const float *radius, const float *bias)
+{
+    const pink_hip_readout_config &c = r->cfg;
+    RouteArgs g = {};
+    g.distances = distances;
+    g.stride = stride ? stride : c.neurons;
+    g.sharpness = sharpness;
+    g.radius = radius;
+    g.bias = bias;
+    g.images = images;
+    g.neurons = c.neurons;
+    g.chosen = c.chosen;
+    g.groups = c.groups;
+    g.groups_kept = c.groups_kept;
+    g.group_size = group_size(c);
+    g.sigmoid = c.score == PINK_HIP_SCORE_SIGMOID;
+    g.renormalise = c.renormalise;
+    return g;
+}
+
+template <typename E, int OP> int product(pink_hip_readout *r, ProductArgs g, uint64_t slots)
+{
+    constexpr int PR = 128, QC = 128, PW = 2, QW = 2;
+    const bool grad = OP == kGradFirst || OP == kGradSecond;
+    g.col_tiles = (g.cols + QC - 1) / QC;
+    g.row_tiles = grad ? (g.rows + PR - 1) / PR : 0;
+    const uint64_t tiles = grad ? (uint64_t)r->cfg.neurons * g.row_tiles : slots / PR + std::min<uint64_t>(r->cfg.neurons, slots);
+    const uint64_t blocks = tiles * g.col_tiles;
+    REFUSE(r, blocks > 0x7fffffffu, "too many images for one call");
+    k_product<E, OP, PR, QC, PW, QW><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
+    return launched(r, "k_product");
+}
+
+int plan(pink_hip_readout *r, const int32_t *neuron, uint32_t slots, char *saved, const Saved &s, const Work &w)
+{
+    const pink_hip_readout_config &c = r->cfg;
+    char *const work = (char *)r->work;
+    PlanArgs g = {};
+    g.neuron = neuron;
+    g.slots = slots;
+    g.neurons = c.neurons;
+    g.tile_rows = kLeastTileRows;
+    g.counts = (uint32_t *)(work + w.counts);
+    g.order = (uint32_t *)(saved + s.order);
+    g.place = (int32_t *)(saved + s.place);
+    g.offsets = (uint32_t *)(saved + s.offsets);
+    g.tile_count = (uint32_t *)(saved + s.tile_count);
+    g.tiles = (uint2 *)(saved + s.tiles);
+    const uint32_t waves = plan_waves(c.neurons), per_block = waves * 64 * kPerWave, blocks = (slots + per_block - 1) / per_block;
+    const size_t lds = (size_t)waves * c.neurons * 4;
+    if (blocks == 1) {
+        k_plan<2><<<1, waves * 64, lds, r->stream>>>(g);
+        return launched(r, "k_plan");
+    }
+    k_plan<0><<<blocks, waves * 64, lds, r->stream>>>(g);
+    TRY(launched(r, "k_plan"));
+    k_plan_offsets<<<1, 1024, 0, r->stream>>>(g, blocks, (uint32_t *)(work + w.totals));
+    TRY(launched(r, "k_plan_offsets"));
+    k_plan<1><<<blocks, waves * 64, lds, r->stream>>>(g);
+    return launched(r, "k_plan");
+}
+
+template <typename E>
+int combine(pink_hip_readout *r, const float *rows, const int32_t *place, uint32_t images, uint32_t cols, const void *residual,
+            uint64_t residual_stride, void *out, uint64_t out_stride)
+{
+    const uint64_t blocks = ((uint64_t)images * cols + 255) / 256;
+    REFUSE(r, blocks > 0x7fffffffu, "too many images for one call");
+    k_combine<E><<<(uint32_t)blocks, 256, 0, r->stream>>>(rows, place, images, r->cfg.chosen, cols, (const E *)residual, residual_stride, (E *)out, out_stride);
+    return launched(r, "k_combine");
+}
+
+template <typename E>
+int experts(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stride, const int32_t *neuron, const float *gates,
+            const pink_hip_readout_weights &weights, const void *residual, uint64_t residual_stride, void *y, uint64_t y_stride, void *keep)
+{
+    const pink_hip_readout_config &c = r->cfg;
+    const Saved s = saved_layout(r, images);
+    const Work w = work_layout(r, images);
+    TRY(grow(r, w.bytes));
+    char *const work = (char *)r->work, *const saved = keep ? (char *)keep : work + w.saved;
+    const uint32_t slots = images * c.chosen;
+    TRY(plan(r, neuron, slots, saved, s, w));
+
+    ProductArgs g = {};
+    g.order = (const uint32_t *)(saved + s.order);
+    g.offsets = (const uint32_t *)(saved + s.offsets);
+    g.tiles = (const uint2 *)(saved + s.tiles);
+    g.tile_count = (const uint32_t *)(saved + s.tile_count);
+    g.chosen = c.chosen;
+    g.activation = c.activation;
+    g.gates = gates;
+    g.p = x;
+    g.p_stride = x_stride;
+    g.q = weights.first;
+    g.q_stride = c.features;
+    g.q_matrix = (uint64_t)c.hidden * c.features;
+    g.depth = c.features;
+    g.cols = c.hidden;
+    g.bias = weights.first_bias;
+    g.out = keep ? saved + s.before : nullptr;
+    g.out_after = saved + s.after;
+    g.out_stride = s.stride;
+    TRY((product<E, kHidden>(r, g, slots)));
+    g.p = saved + s.after;
+    g.p_stride = s.stride;
+    g.q = weights.second;
+    g.q_stride = c.hidden;
+    g.q_matrix = (uint64_t)c.outputs * c.hidden;
+    g.depth = c.hidden;
+    g.cols = c.outputs;
+    g.bias = weights.second_bias;
+    g.out = work + w.rows;
+    g.out_stride = c.outputs;
+    TRY((product<E, kAnswer>(r, g, slots)));
+    return combine<E>(r, (const float *)(work + w.rows), (const int32_t *)(saved + s.place), images, c.outputs, residual, residual_stride, y, y_stride);
+}
+
+template <typename E>
+int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stride, const float *gates,
+                     const pink_hip_readout_weights &weights, const void *keep, const void *dy, uint64_t dy_stride,
+                     const pink_hip_readout_gradients &out, uint64_t dx_stride)
+{
+    const pink_hip_readout_config &c = r->cfg;
+    const Saved s = saved_layout(r, images);
+    const Work w = work_layout(r, images);
+    TRY(grow(r, w.bytes));
+    char *const work = (char *)r->work;
+    const char *const saved = (const char *)keep;
+    const uint32_t slots = images * c.chosen;
+    const uint32_t *const order = (const uint32_t *)(saved + s.order), *const offsets = (const uint32_t *)(saved + s.offsets);
+    const int32_t *const place = (const int32_t *)(saved + s.place);
+    void *const dbefore = work + w.saved;                  // (slots x stride: `saved` is larger)
+
+    ProductArgs g = {};
+    g.order = order;
+    g.offsets = offsets;
+    g.tiles = (const uint2 *)(saved + s.tiles);
+    g.tile_count = (const uint32_t *)(saved + s.tile_count);
+    g.chosen = c.chosen;
+    g.activation = c.activation;
+    g.gates = gates;
+    if (out.gates || out.features || out.first || out.first_bias) {
+        g.p = dy;
+        g.p_stride = dy_stride;
+        g.q = weights.second;
+        g.q_stride = c.hidden;
+        g.q_matrix = (uint64_t)c.outputs * c.hidden;
+        g.depth = c.outputs;
+        g.cols = c.hidden;
+        g.before = saved + s.before;
+        g.out = dbefore;
+        g.out_stride = s.stride;
+        g.partial = (float *)(work + w.partial);
+        TRY((product<E, kBackHidden>(r, g, slots)));
+    }
+    if (out.gates) {
+        k_gate_gradients<E><<<(uint32_t)(((uint64_t)slots + 3) / 4), 256, 0, r->stream>>>(
+            g.partial, (c.hidden + 127) / 128, place, offsets, c.neurons, slots, c.chosen, (const E *)dy, dy_stride, c.outputs,
+            (const E *)weights.second_bias, (E *)out.gates);
+        TRY(launched(r, "k_gate_gradients"));
+    }
+    if (out.features) {
+        g.p = dbefore;
+        g.p_stride = s.stride;
+        g.q = weights.first;
+        g.q_stride = c.features;
+        g.q_matrix = (uint64_t)c.hidden * c.features;
+        g.depth = c.hidden;
+        g.cols = c.features;
+        g.out = work + w.rows;
+        g.out_stride = c.features;
+        TRY((product<E, kBackInput>(r, g, slots)));
+        TRY(combine<E>(r, (const float *)(work + w.rows), place, images, c.features, nullptr, 0, out.features, dx_stride));
+    }
+    if (out.first) {
+        g.p = dbefore;
+        g.p_stride = s.stride;
+        g.q = x;
+        g.q_stride = x_stride;
+        g.rows = c.hidden;
+        g.cols = c.features;
+        g.out = out.first;
+        g.out_stride = c.features;
+        TRY((product<E, kGradFirst>(r, g, slots)));
+    }
+    if (out.second) {
+        g.p = dy;
+        g.p_stride = dy_stride;
+        g.q = saved + s.after;
+        g.q_stride = s.stride;
+        g.rows = c.outputs;
+        g.cols = c.hidden;
+        g.out = out.second;
+        g.out_stride = c.hidden;
+        TRY((product<E, kGradSecond>(r, g, slots)));
+    }
+    if (out.first_bias) {
+        k_bias_gradients<E, false><<<dim3((c.hidden + 255) / 256, c.neurons), 256, 0, r->stream>>>(
+            (const E *)dbefore, s.stride, order, offsets, c.chosen, gates, c.hidden, (E *)out.first_bias);
+        TRY(launched(r, "k_bias_gradients"));
+    }
+    if (out.second_bias) {
+        k_bias_gradients<E, true><<<dim3((c.outputs + 255) / 256, c.neurons), 256, 0, r->stream>>>(
+            (const E *)dy, dy_stride, order, offsets, c.chosen, gates, c.outputs, (E *)out.second_bias);
+        TRY(launched(r, "k_bias_gradients"));
+    }
+    return PINK_HIP_OK;
+}
+
+// Slots of a call are counted in 31 bits.
+int check_images(pink_hip_readout *r, uint32_t images)
+{
+    REFUSE(r, (uint64_t)images * r->cfg.chosen > 0x7fffffffu, "too many images for one call");
+    return PINK_HIP_OK;
+}
+
+// Tensors in launches of at most kAdamTensors.
+template <typename Check, typename Launch>
+int over_tensors(pink_hip_readout *r, const pink_hip_readout_tensor *tensors, uint32_t count, AdamArgs &g, const Check &ok, const Launch &launch)
+{
+    for (uint32_t i = 0; i < count; ++i)
+        if (tensors[i].size) TRY(ok(tensors[i]));
+    uint64_t blocks = 0;
+    g.count = 0;
+    for (uint32_t i = 0; i <= count; ++i) {
+        const uint64_t more = i < count ? (tensors[i].size + kAdamChunk - 1) / kAdamChunk : 0;
+        if (g.count && (i == count || g.count == kAdamTensors || blocks + more > 0x7fffffffu)) {
+            g.first_block[g.count] = (uint32_t)blocks;
+            launch((uint32_t)blocks);
+            TRY(launched(r, "k_adamw"));
+            g.count = 0;
+            blocks = 0;
+        }
+        if (!more) continue;
+        g.tensor[g.count] = tensors[i];
+        g.first_block[g.count++] = (uint32_t)blocks;
+        blocks += more;
+    }
+    return PINK_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+const char *pink_hip_readout_last_error(const pink_hip_readout *r) { return r ? r->err : g_readout_error; }
+
+int pink_hip_readout_check(const pink_hip_readout_config *cfg) { return check(cfg, nullptr); }
+
+int pink_hip_readout_create(pink_hip_readout **out, const pink_hip_readout_config *cfg)
+{
+    if (!out) return fail(nullptr, PINK_HIP_EINVAL, "pink_hip_readout_create: null argument");
+    *out = nullptr;
+    TRY(check(cfg, nullptr));
+    HIP_TRY(nullptr, hipSetDevice(cfg->device));
+    // the forms whose LDS goes by the number of neurons
+    const int lds = (int)(kMaxNeurons * 4 + kMaxGroups * 4);
+    HIP_TRY(nullptr, hipFuncSetAttribute((const void *)k_route_block, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    HIP_TRY(nullptr, hipFuncSetAttribute((const void *)k_balance, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    HIP_TRY(nullptr, hipFuncSetAttribute((const void *)k_plan<0>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    HIP_TRY(nullptr, hipFuncSetAttribute((const void *)k_plan<1>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    HIP_TRY(nullptr, hipFuncSetAttribute((const void *)k_plan<2>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    pink_hip_readout *r = new (std::nothrow) pink_hip_readout();
+    if (!r) return fail(nullptr, PINK_HIP_ENOMEM, "pink_hip_readout_create: out of memory");
+    r->cfg = *cfg;
+    const hipError_t e = hipStreamCreateWithFlags(&r->own, hipStreamNonBlocking);
+    if (e != hipSuccess) {
+        delete r;
+        return fail(nullptr, PINK_HIP_EDEVICE, "hipStreamCreateWithFlags", hipGetErrorString(e));
+    }
+    r->stream = r->own;
+    *out = r;
+    return PINK_HIP_OK;
+}
+
+void pink_hip_readout_destroy(pink_hip_readout *r)
+{
+    if (!r) return;
+    (void)hipSetDevice(r->cfg.device);
+    if (r->stream != r->own) (void)hipStreamSynchronize(r->stream);
+    (void)hipStreamSynchronize(r->own);
+    if (r->work) (void)hipFree(r->work);
+    (void)hipStreamDestroy(r->own);
+    delete r;
+}
+
+int pink_hip_readout_set_stream(pink_hip_readout *r, void *hip_stream)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    const hipStream_t next = hip_stream == PINK_HIP_OWN_STREAM ? r->own : (hipStream_t)hip_stream;
+    if (next == r->stream) return PINK_HIP_OK;
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    HIP_TRY(r, hipStreamSynchronize(r->stream));           // the workspace is one stream's at a time
+    r->stream = next;
+    return PINK_HIP_OK;
+}
+
+int pink_hip_readout_synchronize(pink_hip_readout *r)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    HIP_TRY(r, hipStreamSynchronize(r->stream));
+    return PINK_HIP_OK;
+}
+
+int pink_hip_readout_route(pink_hip_readout *r, const float *distances, uint32_t images, uint64_t stride, const float *sharpness,
+                           const float *radius, const float *bias, int32_t *neuron, float *gates)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    if (images == 0) return PINK_HIP_OK;
+    REFUSE(r, !distances || !sharpness || !radius || !neuron || !gates, "pink_hip_readout_route: null argument");
+    REFUSE(r, stride && stride < r->cfg.neurons, "pink_hip_readout_route: rows of distances overlap");
+    TRY(check_images(r, images));
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    RouteArgs g = route_args(r, distances, images, stride, sharpness, radius, bias);
+    g.neuron = neuron;
+    g.gates = gates;
+    k_route_block<<<images, 256, (g.neurons + (g.groups > 1 ? g.groups : 0)) * 4, r->stream>>>(g);
+    return launched(r, "k_route_block");
+}
+
+int pink_hip_readout_route_backward(pink_hip_readout *r, const float *distances, uint32_t images, uint64_t stride, const float *sharpness,
+                                    const float *radius, const float *bias, const int32_t *neuron, const float *gates,
+                                    const void *gate_gradients, float *ddistances, float *dsharpness, float *dradius)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    const uint32_t neurons = r->cfg.neurons;
+    REFUSE(r, images && (!distances || !sharpness || !radius || !neuron || !gates || !gate_gradients), "pink_hip_readout_route_backward: null argument");
+    REFUSE(r, stride && stride < neurons, "pink_hip_readout_route_backward: rows of distances overlap");
+    TRY(check_images(r, images));
+    if (!ddistances && !dsharpness && !dradius) return PINK_HIP_OK;
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    RouteBackwardArgs a = {};
+    a.r = route_args(r, distances, images, stride, sharpness, radius, bias);
+    a.r.neuron = const_cast<int32_t *>(neuron);
+    a.r.gates = const_cast<float *>(gates);
+    a.gate_gradients = gate_gradients;
+    a.distance_gradients = ddistances;
+    a.want_sums = dsharpness || dradius;
+    a.chunk = std::max(4u, std::min(kChunkMost, images / 512));
+    a.chunk = std::max(a.chunk, (images + 65534) / 65535);               // (the grid's second dimension)
+    REFUSE(r, a.chunk > kChunkMost, "too many images for one call");
+    const uint32_t chunks = (images + a.chunk - 1) / a.chunk;
+    TRY(grow(r, std::max<size_t>(1, (size_t)chunks * neurons * 8)));
+    a.sharpness_part = (float *)r->work;
+    a.radius_part = a.sharpness_part + (size_t)chunks * neurons;
+    if (images) {
+        const dim3 grid((neurons + 255) / 256, chunks);
+        const size_t lds = (size_t)a.chunk * a.r.chosen * 8;
+        if (r->cfg.element == PINK_HIP_ELEMENT_BFLOAT) k_route_backward<Bfloat><<<grid, 256, lds, r->stream>>>(a);
+        else k_route_backward<float><<<grid, 256, lds, r->stream>>>(a);
+        TRY(launched(r, "k_route_backward"));
+    }
+    if (!a.want_sums) return PINK_HIP_OK;
+    k_route_sums<<<(neurons + 63) / 64, 256, 0, r->stream>>>(a.sharpness_part, a.radius_part, chunks, neurons, dsharpness, dradius);
+    return launched(r, "k_route_sums");
+}
+
+int pink_hip_readout_balance(pink_hip_readout *r, const int32_t *neuron, uint32_t images, float rate, float *bias, int32_t *load)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    REFUSE(r, (images && !neuron) || !bias, "pink_hip_readout_balance: null argument");
+    TRY(check_images(r, images));
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    k_balance<<<1, 1024, r->cfg.neurons * 4, r->stream>>>(neuron, (uint64_t)images * r->cfg.chosen, r->cfg.neurons, rate, bias, load);
+    return launched(r, "k_balance");
+}
+
+int pink_hip_readout_reserve(pink_hip_readout *r, uint32_t images)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    TRY(check_images(r, images));
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    const size_t parts = ((size_t)images / 4 + 1) * r->cfg.neurons * 8;
+    return grow(r, std::max(parts, r->cfg.features ? work_layout(r, images).bytes : 0));
+}
+
+size_t pink_hip_readout_saved_bytes(pink_hip_readout *r, uint32_t images)
+{
+    return !r || !r->cfg.features || (uint64_t)images * r->cfg.chosen > 0x7fffffffu ? 0 : saved_layout(r, images).bytes;
+}
+
+int pink_hip_readout_experts(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stride, const int32_t *neuron, const float *gates,
+                             const pink_hip_readout_weights *weights, const void *residual, uint64_t residual_stride, void *y,
+                             uint64_t y_stride, void *saved)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    const pink_hip_readout_config &c = r->cfg;
+    if (!c.features) return fail(r, PINK_HIP_ESTATE, "pink_hip_readout_experts: the handle was made without models");
+    if (images == 0) return PINK_HIP_OK;
+    REFUSE(r, !x || !neuron || !gates || !weights || !weights->first || !weights->second || !y, "pink_hip_readout_experts: null argument");
+    x_stride = x_stride ? x_stride : c.features;
+    y_stride = y_stride ? y_stride : c.outputs;
+    residual_stride = residual_stride ? residual_stride : c.outputs;
+    REFUSE(r, x_stride < c.features || y_stride < c.outputs || residual_stride < c.outputs, "pink_hip_readout_experts: rows overlap");
+    REFUSE(r, (uintptr_t)saved & 255, "pink_hip_readout_experts: saved must be aligned to 256 bytes");
+    TRY(check_images(r, images));
+    HIP_TRY(r, hipSetDevice(c.device));
+    if (c.element == PINK_HIP_ELEMENT_BFLOAT)
+        return experts<Bfloat>(r, x, images, x_stride, neuron, gates, *weights, residual, residual_stride, y, y_stride, saved);
+    return experts<float>(r, x, images, x_stride, neuron, gates, *weights, residual, residual_stride, y, y_stride, saved);
+}
+
+int pink_hip_readout_experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stride, const float *gates,
+                                      const pink_hip_readout_weights *weights, const void *saved, const void *dy, uint64_t dy_stride,
+                                      const pink_hip_readout_gradients *out, uint64_t dx_stride)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    const pink_hip_readout_config &c = r->cfg;
+    if (!c.features) return fail(r, PINK_HIP_ESTATE, "pink_hip_readout_experts_backward: the handle was made without models");
+    REFUSE(r, !out, "pink_hip_readout_experts_backward: null argument");
+    const size_t e = element_bytes(r);
+    HIP_TRY(r, hipSetDevice(c.device));
+    if (images == 0) {                                     // nothing was chosen: the weights' gradients are zero
+        const auto clear = [&](void *at, uint64_t n) {
+            if (at) k_clear<<<1024, 256, 0, r->stream>>>((uint8_t *)at, n * e);
+        };
+        clear(out->first, (uint64_t)c.neurons * c.hidden * c.features);
+        clear(out->first_bias, (uint64_t)c.neurons * c.hidden);
+        clear(out->second, (uint64_t)c.neurons * c.outputs * c.hidden);
+        clear(out->second_bias, (uint64_t)c.neurons * c.outputs);
+        return launched(r, "k_clear");
+    }
+    REFUSE(r, !x || !gates || !weights || !weights->first || !weights->second || !saved || !dy, "pink_hip_readout_experts_backward: null argument");
+    x_stride = x_stride ? x_stride : c.features;
+    dx_stride = dx_stride ? dx_stride : c.features;
+    dy_stride = dy_stride ? dy_stride : c.outputs;
+    REFUSE(r, x_stride < c.features || dx_stride < c.features || dy_stride < c.outputs, "pink_hip_readout_experts_backward: rows overlap");
+    REFUSE(r, (uintptr_t)saved & 255, "pink_hip_readout_experts_backward: saved must be aligned to 256 bytes");
+    TRY(check_images(r, images));
+    if (c.element == PINK_HIP_ELEMENT_BFLOAT)
+        return experts_backward<Bfloat>(r, x, images, x_stride, gates, *weights, saved, dy, dy_stride, *out, dx_stride);
+    return experts_backward<float>(r, x, images, x_stride, gates, *weights, saved, dy, dy_stride, *out, dx_stride);
+}
+
+int pink_hip_readout_adamw(pink_hip_readout *r, const pink_hip_readout_tensor *tensors, uint32_t count, uint32_t state_bits, uint64_t step,
+                           float learning_rate, float beta_first, float beta_second, float epsilon)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    REFUSE(r, count && !tensors, "pink_hip_readout_adamw: null argument");
+    REFUSE(r, state_bits != 8 && state_bits != 32, "pink_hip_readout_adamw: states have 8 or 32 bits");
+    REFUSE(r, step == 0, "pink_hip_readout_adamw: steps count from 1");
+    REFUSE(r, !(beta_first >= 0.0f && beta_first < 1.0f && beta_second >= 0.0f && beta_second < 1.0f), "pink_hip_readout_adamw: betas must be in [0, 1)");
+    REFUSE(r, !(epsilon > 0.0f), "pink_hip_readout_adamw: epsilon must be larger than 0");
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    AdamArgs g = {};
+    g.rate = learning_rate;
+    g.beta1 = beta_first;
+    g.beta2 = beta_second;
+    g.rest1 = 1.0f - beta_first;
+    g.rest2 = 1.0f - beta_second;
+    g.c1 = (float)(1.0 / (1.0 - std::pow((double)beta_first, (double)step)));
+    g.c2 = (float)(1.0 / (1.0 - std::pow((double)beta_second, (double)step)));
+    g.epsilon = epsilon;
+    return over_tensors(
+        r, tensors, count, g,
+        [&](const pink_hip_readout_tensor &t) -> int {
+            REFUSE(r, !t.value || !t.gradient || !t.first || !t.second, "pink_hip_readout_adamw: null argument");
+            REFUSE(r, state_bits == 8 && (!t.first_scale || !t.second_scale), "pink_hip_readout_adamw: 8-bit states need scales");
+            REFUSE(r, t.gradient_element > PINK_HIP_ELEMENT_BFLOAT, "unknown element type");
+            return PINK_HIP_OK;
+        },
+        [&](uint32_t blocks) {
+            if (state_bits == 8) k_adamw<true><<<blocks, 256, 0, r->stream>>>(g);
+            else k_adamw<false><<<blocks, 256, 0, r->stream>>>(g);
+        });
+}
+
+int pink_hip_readout_unpack(pink_hip_readout *r, const pink_hip_readout_tensor *tensors, uint32_t count)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    REFUSE(r, count && !tensors, "pink_hip_readout_unpack: null argument");
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    AdamArgs g = {};
+    return over_tensors(
+        r, tensors, count, g,
+        [&](const pink_hip_readout_tensor &t) -> int {
+            REFUSE(r, !t.first || !t.second || !t.first_scale || !t.second_scale || !t.first_values || !t.second_values, "pink_hip_readout_unpack: null argument");
+            return PINK_HIP_OK;
+        },
+        [&](uint32_t blocks) { k_unpack<<<blocks, 256, 0, r->stream>>>(g); });
+}
+
+}  // extern "C"
