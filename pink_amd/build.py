@@ -13,14 +13,16 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SOURCES = [os.path.join(HERE, "csrc", "pink_hip.hip"), os.path.join(HERE, "csrc", "update_factors.cpp"),
-           os.path.join(HERE, "csrc", "readout.hip")]
+SOURCES = [os.path.join(HERE, "csrc", "pink_hip.hip"), os.path.join(HERE, "csrc", "update_factors.cpp")]
 # Compiled on its own with the MFMA accumulators in the architectural vector registers: its
 # distance kernel fills all 256 accumulation registers with resident SOM fragments (which the MFMA
 # reads as operands) and post-processes the accumulators on the vector ALU, which cannot read
 # accumulation registers.  The other MFMA kernels want the default (accumulators there).
 SYM_SOURCE = os.path.join(HERE, "csrc", "mfma_u8_sym.hip")
 SYM_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+# The read-out's products keep their sums in the architectural registers too: 64 to 128 a lane, which fit there, and the default
+# moves them between the two kinds in every step.
+READOUT_SOURCE = os.path.join(HERE, "csrc", "readout.hip")
 OUT = os.path.join(HERE, "lib", "libpink_hip.so")
 
 HIPCC_FLAGS = [
@@ -37,9 +39,9 @@ def build(verbose=False, extra=()):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     obj_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
     objects, cmds = [], []
-    for src in SOURCES + [SYM_SOURCE]:
+    for src in SOURCES + [SYM_SOURCE, READOUT_SOURCE]:
         obj = os.path.join(HERE, "lib", os.path.splitext(os.path.basename(src))[0] + ".o")
-        flags = obj_flags + (SYM_FLAGS if src == SYM_SOURCE else [])
+        flags = obj_flags + (SYM_FLAGS if src in (SYM_SOURCE, READOUT_SOURCE) else [])
         cmds.append([hipcc] + flags + list(extra) + ["-c", src, "-o", obj])
         objects.append(obj)
     cmds.append([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC"] + objects + ["-o", OUT])

@@ -349,7 +349,8 @@ struct PlanArgs {
     const int32_t *neuron;
     uint32_t slots, neurons, tile_rows;
     uint32_t *counts;              // blocks x N
-    uint32_t *order, *offsets, *tile_count;
+    uint32_t *order, *images, *owner, *offsets, *tile_count;      // row -> slot, image, neuron; neuron -> first row
+    uint32_t chosen;
     int32_t *place;                // slot -> row, -1 where it has none
     uint2 *tiles;
 };
@@ -452,6 +453,8 @@ template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanAr
             row = (int32_t)(g.offsets[id[i]] + hist[wave * g.neurons + id[i]] + rank[i]);
             if (STAGE == 1) row += (int32_t)g.counts[(uint64_t)blockIdx.x * g.neurons + id[i]];
             g.order[row] = (uint32_t)slot;
+            g.images[row] = (uint32_t)slot / g.chosen;
+            g.owner[row] = id[i];
         }
         g.place[slot] = row;
     }
@@ -483,20 +486,32 @@ template <typename E>
 __global__ __launch_bounds__(256) void k_combine(const float *rows, const int32_t *place, uint32_t images, uint32_t chosen, uint32_t cols,
                                                  const E *residual, uint64_t residual_stride, E *out, uint64_t out_stride)
 {
-    const uint64_t n = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint64_t t = n / cols;
-    const uint32_t c = (uint32_t)(n - t * cols);
+    const uint64_t n = (uint64_t)blockIdx.x * 256 + threadIdx.x, stride = ((uint64_t)cols + 3) / 4 * 4;
+    const uint64_t t = n / (stride / 4);
+    const uint32_t c = (uint32_t)(n - t * (stride / 4)) * 4;
     if (t >= images) return;
-    float v = residual ? to_float(residual[t * residual_stride + c]) : 0.0f;
+    float v[4] = {0, 0, 0, 0};
+    if (residual)
+        for (uint32_t e = 0; e < 4; ++e)
+            if (c + e < cols) v[e] = to_float(residual[t * residual_stride + c + e]);
     for (uint32_t s = 0; s < chosen; ++s)
-        if (place[t * chosen + s] >= 0) v += rows[(t * chosen + s) * cols + c];
-    out[t * out_stride + c] = from_float<E>(v);
+        if (place[t * chosen + s] >= 0) {
+            const v4f r = *(const v4f *)(rows + (t * chosen + s) * stride + c);
+            for (int e = 0; e < 4; ++e) v[e] += r[e];
+        }
+    E *const to = out + t * out_stride + c;
+    if (c + 4 <= cols) {
+        store_four(to, v);
+    } else {
+        for (uint32_t e = 0; e < 4; ++e)
+            if (c + e < cols) to[e] = from_float<E>(v[e]);
+    }
 }
 
 // d gate of a slot = dy . (W2 f(a) + b2) = sum of its row's parts + dy . b2; a wave per slot.
 template <typename E>
-__global__ __launch_bounds__(256) void k_gate_gradients(const float *partial, uint32_t parts, const int32_t *place, const uint32_t *offsets,
-                                                        uint32_t neurons, uint64_t slots, uint32_t chosen, const E *dy, uint64_t dy_stride,
+__global__ __launch_bounds__(256) void k_gate_gradients(const float *partial, uint32_t parts, const int32_t *place, const uint32_t *owner,
+                                                        uint64_t slots, uint32_t chosen, const E *dy, uint64_t dy_stride,
                                                         uint32_t cols, const E *bias, E *out)
 {
     const uint64_t slot = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -507,33 +522,13 @@ __global__ __launch_bounds__(256) void k_gate_gradients(const float *partial, ui
     if (row >= 0) {
         for (uint32_t i = lane; i < parts; i += 64) v += partial[(uint64_t)row * parts + i];
         if (bias) {
-            uint32_t lo = 0, hi = neurons;                 // the last neuron that starts at or before the row
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (offsets[mid] <= (uint32_t)row) lo = mid;
-                else hi = mid;
-            }
+            const uint64_t neuron = owner[row];
             const E *const d = dy + slot / chosen * dy_stride;
-            for (uint32_t c = lane; c < cols; c += 64) v += to_float(d[c]) * to_float(bias[(uint64_t)lo * cols + c]);
+            for (uint32_t c = lane; c < cols; c += 64) v += to_float(d[c]) * to_float(bias[neuron * cols + c]);
         }
     }
     v = wave_sum(v);
     if (lane == 0) out[slot] = from_float<E>(v);
-}
-
-// Gradients of a layer's biases: the sum of a neuron's rows, gated and by image for the second layer.
-template <typename E, bool SECOND>
-__global__ __launch_bounds__(256) void k_bias_gradients(const E *rows, uint64_t stride, const uint32_t *order, const uint32_t *offsets, uint32_t chosen,
-                                                        const float *gates, uint32_t cols, E *out)
-{
-    const uint32_t neuron = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
-    float v = 0.0f;
-    for (uint32_t r = offsets[neuron]; r < offsets[neuron + 1]; ++r) {
-        if (SECOND) v += gates[order[r]] * to_float(rows[order[r] / chosen * stride + c]);
-        else v += to_float(rows[(uint64_t)r * stride + c]);
-    }
-    out[(uint64_t)neuron * cols + c] = from_float<E>(v);
 }
 
 // Zeros, by a kernel: a recorded memset has not always been replayed right in graphs.
@@ -767,11 +762,16 @@ int grow(pink_hip_readout *r, size_t bytes)
 
 // What a forward call leaves for the backward one, and where.
 struct Saved {
-    size_t order, place, offsets, tile_count, tiles, before, after, bytes;
+    size_t order, images, owner, place, offsets, tile_count, tiles, before, after, bytes;
     uint64_t stride;               // of before's and after's rows: whole 16-byte chunks
 };
 
+#ifdef ROWS_CFG
+constexpr int kRowsCfg[5] = {ROWS_CFG};
+constexpr uint32_t kLeastTileRows = kRowsCfg[0];
+#else
 constexpr uint32_t kLeastTileRows = 128;
+#endif
 
 Saved saved_layout(const pink_hip_readout *r, uint64_t images)
 {
@@ -786,6 +786,8 @@ Saved saved_layout(const pink_hip_readout *r, uint64_t images)
     };
     s.stride = (c.hidden + 16 / e - 1) / (16 / e) * (16 / e);
     s.order = take(slots * 4);
+    s.images = take(slots * 4);
+    s.owner = take(slots * 4);
     s.place = take(slots * 4);
     s.offsets = take(((size_t)c.neurons + 1) * 4);
     s.tile_count = take(4);
@@ -797,6 +799,9 @@ Saved saved_layout(const pink_hip_readout *r, uint64_t images)
 }
 
 uint32_t plan_waves(uint32_t neurons) { return std::max(1u, std::min(16u, 32768u / neurons)); }
+
+// Floats between rows of products that images are summed up from: whole chunks.
+uint64_t whole_rows(uint32_t cols) { return ((uint64_t)cols + 3) / 4 * 4; }
 
 struct Work {
     size_t counts, totals, rows, partial, saved, bytes;
@@ -815,7 +820,7 @@ Work work_layout(const pink_hip_readout *r, uint64_t images)
     };
     w.counts = take(plan_blocks * c.neurons * 4);
     w.totals = take((size_t)c.neurons * 4);
-    w.rows = take(slots * std::max(c.features, c.outputs) * 4);
+    w.rows = take(slots * whole_rows(std::max(c.features, c.outputs)) * 4);
     w.partial = take(slots * ((c.hidden + 31) / 32) * 4);
     w.saved = take(saved_layout(r, images).bytes);         // forward calls that keep nothing; gradients of `before`
     w.bytes = at;
@@ -861,16 +866,32 @@ RouteArgs route_args(const pink_hip_readout *r, const float *distances, uint32_t
     return g;
 }
 
-template <typename E, int OP> int product(pink_hip_readout *r, ProductArgs g, uint64_t slots)
+template <typename E, int OP> int product(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
 {
-    constexpr int PR = 128, QC = 128, PW = 2, QW = 2;
-    const bool grad = OP == kGradFirst || OP == kGradSecond;
-    g.col_tiles = (g.cols + QC - 1) / QC;
+    constexpr bool grad = OP == kGradFirst || OP == kGradSecond;
+#ifdef ROWS_CFG
+    constexpr int cfg[2][5] = {{ROWS_CFG}, {GRAD_CFG}};
+    constexpr int PR = cfg[grad][0], QC = cfg[grad][1], PW = cfg[grad][2], QW = cfg[grad][3], M = cfg[grad][4];
+#else
+    constexpr int PR = 128, QC = 128, PW = 2, QW = 2, M = 32;
+#endif
+    g.col_tiles = grad && !g.out ? 1 : (g.cols + QC - 1) / QC;
     g.row_tiles = grad ? (g.rows + PR - 1) / PR : 0;
     const uint64_t tiles = grad ? (uint64_t)r->cfg.neurons * g.row_tiles : slots / PR + std::min<uint64_t>(r->cfg.neurons, slots);
     const uint64_t blocks = tiles * g.col_tiles;
     REFUSE(r, blocks > 0x7fffffffu, "too many images for one call");
-    k_product<E, OP, PR, QC, PW, QW><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
+    // Whole chunks at their alignment?  (`saved` and the workspace have both; what lies past a row's end there is readable.)
+    constexpr uint32_t per = 16 / sizeof(E);
+    const auto whole = [](const void *at, uint64_t stride) { return ((uintptr_t)at & 15) == 0 && stride % per == 0; };
+    bool direct = whole(g.p, g.p_stride) && whole(g.q, g.q_stride);
+    if (OP == kHidden || OP == kAnswer || OP == kBackHidden || OP == kBackInput) direct = direct && g.q_matrix % per == 0;
+    if (OP == kHidden || OP == kAnswer) direct = direct && g.depth % per == 0;
+    if (OP == kBackHidden) direct = direct && g.depth % per == 0 && g.cols % per == 0;
+    if (OP == kBackInput) direct = direct && g.cols % per == 0;
+    if (OP == kGradFirst) direct = direct && g.cols % per == 0;
+    if (OP == kGradSecond) direct = direct && g.rows % per == 0;
+    if (direct) k_product<E, OP, PR, QC, PW, QW, M, true><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
+    else k_product<E, OP, PR, QC, PW, QW, M, false><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
     return launched(r, "k_product");
 }
 
@@ -884,7 +905,10 @@ int plan(pink_hip_readout *r, const int32_t *neuron, uint32_t slots, char *saved
     g.neurons = c.neurons;
     g.tile_rows = kLeastTileRows;
     g.counts = (uint32_t *)(work + w.counts);
+    g.chosen = c.chosen;
     g.order = (uint32_t *)(saved + s.order);
+    g.images = (uint32_t *)(saved + s.images);
+    g.owner = (uint32_t *)(saved + s.owner);
     g.place = (int32_t *)(saved + s.place);
     g.offsets = (uint32_t *)(saved + s.offsets);
     g.tile_count = (uint32_t *)(saved + s.tile_count);
@@ -907,7 +931,7 @@ template <typename E>
 int combine(pink_hip_readout *r, const float *rows, const int32_t *place, uint32_t images, uint32_t cols, const void *residual,
             uint64_t residual_stride, void *out, uint64_t out_stride)
 {
-    const uint64_t blocks = ((uint64_t)images * cols + 255) / 256;
+    const uint64_t blocks = (images * (whole_rows(cols) / 4) + 255) / 256;
     REFUSE(r, blocks > 0x7fffffffu, "too many images for one call");
     k_combine<E><<<(uint32_t)blocks, 256, 0, r->stream>>>(rows, place, images, r->cfg.chosen, cols, (const E *)residual, residual_stride, (E *)out, out_stride);
     return launched(r, "k_combine");
@@ -927,6 +951,7 @@ int experts(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stri
 
     ProductArgs g = {};
     g.order = (const uint32_t *)(saved + s.order);
+    g.images = (const uint32_t *)(saved + s.images);
     g.offsets = (const uint32_t *)(saved + s.offsets);
     g.tiles = (const uint2 *)(saved + s.tiles);
     g.tile_count = (const uint32_t *)(saved + s.tile_count);
@@ -954,7 +979,7 @@ int experts(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stri
     g.cols = c.outputs;
     g.bias = weights.second_bias;
     g.out = work + w.rows;
-    g.out_stride = c.outputs;
+    g.out_stride = whole_rows(c.outputs);
     TRY((product<E, kAnswer>(r, g, slots)));
     return combine<E>(r, (const float *)(work + w.rows), (const int32_t *)(saved + s.place), images, c.outputs, residual, residual_stride, y, y_stride);
 }
@@ -971,13 +996,13 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
     char *const work = (char *)r->work;
     const char *const saved = (const char *)keep;
     const uint32_t slots = images * c.chosen;
-    const uint32_t *const order = (const uint32_t *)(saved + s.order), *const offsets = (const uint32_t *)(saved + s.offsets);
     const int32_t *const place = (const int32_t *)(saved + s.place);
     void *const dbefore = work + w.saved;                  // (slots x stride: `saved` is larger)
 
     ProductArgs g = {};
-    g.order = order;
-    g.offsets = offsets;
+    g.order = (const uint32_t *)(saved + s.order);
+    g.images = (const uint32_t *)(saved + s.images);
+    g.offsets = (const uint32_t *)(saved + s.offsets);
     g.tiles = (const uint2 *)(saved + s.tiles);
     g.tile_count = (const uint32_t *)(saved + s.tile_count);
     g.chosen = c.chosen;
@@ -999,7 +1024,7 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
     }
     if (out.gates) {
         k_gate_gradients<E><<<(uint32_t)(((uint64_t)slots + 3) / 4), 256, 0, r->stream>>>(
-            g.partial, (c.hidden + 127) / 128, place, offsets, c.neurons, slots, c.chosen, (const E *)dy, dy_stride, c.outputs,
+            g.partial, g.col_tiles, place, (const uint32_t *)(saved + s.owner), slots, c.chosen, (const E *)dy, dy_stride, c.outputs,
             (const E *)weights.second_bias, (E *)out.gates);
         TRY(launched(r, "k_gate_gradients"));
     }
@@ -1012,11 +1037,11 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
         g.depth = c.hidden;
         g.cols = c.features;
         g.out = work + w.rows;
-        g.out_stride = c.features;
+        g.out_stride = whole_rows(c.features);
         TRY((product<E, kBackInput>(r, g, slots)));
         TRY(combine<E>(r, (const float *)(work + w.rows), place, images, c.features, nullptr, 0, out.features, dx_stride));
     }
-    if (out.first) {
+    if (out.first || out.first_bias) {
         g.p = dbefore;
         g.p_stride = s.stride;
         g.q = x;
@@ -1024,10 +1049,11 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
         g.rows = c.hidden;
         g.cols = c.features;
         g.out = out.first;
+        g.out_bias = out.first_bias;
         g.out_stride = c.features;
         TRY((product<E, kGradFirst>(r, g, slots)));
     }
-    if (out.second) {
+    if (out.second || out.second_bias) {
         g.p = dy;
         g.p_stride = dy_stride;
         g.q = saved + s.after;
@@ -1035,18 +1061,9 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
         g.rows = c.outputs;
         g.cols = c.hidden;
         g.out = out.second;
+        g.out_bias = out.second_bias;
         g.out_stride = c.hidden;
         TRY((product<E, kGradSecond>(r, g, slots)));
-    }
-    if (out.first_bias) {
-        k_bias_gradients<E, false><<<dim3((c.hidden + 255) / 256, c.neurons), 256, 0, r->stream>>>(
-            (const E *)dbefore, s.stride, order, offsets, c.chosen, gates, c.hidden, (E *)out.first_bias);
-        TRY(launched(r, "k_bias_gradients"));
-    }
-    if (out.second_bias) {
-        k_bias_gradients<E, true><<<dim3((c.outputs + 255) / 256, c.neurons), 256, 0, r->stream>>>(
-            (const E *)dy, dy_stride, order, offsets, c.chosen, gates, c.outputs, (E *)out.second_bias);
-        TRY(launched(r, "k_bias_gradients"));
     }
     return PINK_HIP_OK;
 }
