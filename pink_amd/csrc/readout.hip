@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstring>
 #include <new>
+#include <type_traits>
 
 #include "pink_hip.h"
 
@@ -64,9 +65,10 @@ struct RouteArgs {
 };
 
 // An entry's key in the choice: a number that grows with z + bias, 0 where the entry takes no part.
-__device__ __forceinline__ uint32_t order_key(float z, float biased)
+// (An infinite or NaN z does not become finite by a bias.)
+__device__ __forceinline__ uint32_t order_key(float biased)
 {
-    if (!isfinite(z) || !isfinite(biased)) return 0;
+    if (!isfinite(biased)) return 0;
     const uint32_t bits = __float_as_uint(biased + 0.0f);  // (-0 and 0 tie)
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
@@ -74,6 +76,14 @@ __device__ __forceinline__ uint32_t order_key(float z, float biased)
 __device__ __forceinline__ float key_value(uint32_t key)
 {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+// A group's key from the two largest of its neurons.
+__device__ __forceinline__ uint32_t group_score(uint32_t first, uint32_t second)
+{
+    if (!second) return first;
+    const float both = key_value(first) + key_value(second);
+    return order_key(fminf(fmaxf(both, -3.402823466e38f), 3.402823466e38f));
 }
 
 __device__ __forceinline__ float logit(const RouteArgs &g, const float *row, uint32_t n)
@@ -110,7 +120,7 @@ __global__ __launch_bounds__(256) void k_route_block(const RouteArgs g)
     float top = -INFINITY;
     for (uint32_t n = tid; n < g.neurons; n += 256) {
         const float z = logit(g, row, n), biased = g.bias ? z + g.bias[n] : z;
-        const uint32_t key = order_key(z, biased);
+        const uint32_t key = order_key(biased);
         keys[n] = key;
         if (key) top = fmaxf(top, z);
     }
@@ -144,12 +154,7 @@ __global__ __launch_bounds__(256) void k_route_block(const RouteArgs g)
                 first = max(first, a);
             }
             if (lane == 0) {
-                uint32_t key = first;
-                if (second) {
-                    const float both = key_value(first) + key_value(second);
-                    key = order_key(0.0f, fminf(fmaxf(both, -3.402823466e38f), 3.402823466e38f));
-                }
-                group_keys[k] = key;
+                group_keys[k] = group_score(first, second);
             }
         }
         __syncthreads();
@@ -195,6 +200,194 @@ __global__ __launch_bounds__(256) void k_route_block(const RouteArgs g)
             g.neuron[(uint64_t)blockIdx.x * g.chosen + lane] = n;
             g.gates[(uint64_t)blockIdx.x * g.chosen + lane] = gate;
         }
+    }
+}
+
+// The largest of the wave, by DPP within rows of sixteen and across them into lane 63.
+__device__ __forceinline__ uint32_t wave_max_u32_dpp(uint32_t v)
+{
+#define PINK_DPP_MAX(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false))
+    PINK_DPP_MAX(0xb1, 0xf);      // quad_perm [1, 0, 3, 2]
+    PINK_DPP_MAX(0x4e, 0xf);      // quad_perm [2, 3, 0, 1]
+    PINK_DPP_MAX(0x141, 0xf);     // row_half_mirror
+    PINK_DPP_MAX(0x140, 0xf);     // row_mirror
+    PINK_DPP_MAX(0x142, 0xa);     // row_bcast:15 into rows 1 and 3
+    PINK_DPP_MAX(0x143, 0xc);     // row_bcast:31 into rows 2 and 3
+#undef PINK_DPP_MAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// Sums of 64 neurons' keys per register: what a wave holds of an image, candidate 64 j + lane in key[j].
+template <int J> struct Candidates {
+    static constexpr int kSet = J <= 8 ? J : J % 8 ? 4 : 8, kSets = J / kSet;
+    static_assert(J % kSet == 0, "whole sets");
+    uint32_t key[J], best[kSets], where[kSets];            // of each set of registers: the largest key and its register
+
+    template <int B> __device__ __forceinline__ void find()
+    {
+        best[B] = key[B * kSet];
+        where[B] = B * kSet;
+#pragma unroll
+        for (int i = 1; i < kSet; ++i)
+            if (key[B * kSet + i] > best[B]) {
+                best[B] = key[B * kSet + i];
+                where[B] = B * kSet + i;
+            }
+    }
+    template <int B> __device__ __forceinline__ void find_all()
+    {
+        find<B>();
+        if constexpr (B + 1 < kSets) find_all<B + 1>();
+    }
+    // Takes one candidate, of register j in lane l, out; only its set of registers is gone through again.
+    template <int B> __device__ __forceinline__ void remove(uint32_t j, uint32_t l, uint32_t lane)
+    {
+        if (j / kSet == B) {
+#pragma unroll
+            for (int i = 0; i < kSet; ++i)
+                if (j == B * kSet + i && lane == l) key[B * kSet + i] = 0;
+            find<B>();
+        }
+        if constexpr (B + 1 < kSets) remove<B + 1>(j, l, lane);
+    }
+    // The next candidate in order (the largest key, the lowest number on ties), or none: -1.
+    __device__ __forceinline__ int take(uint32_t lane)
+    {
+        uint32_t k = best[0], w = where[0];
+#pragma unroll
+        for (int b = 1; b < kSets; ++b)
+            if (best[b] > k) {
+                k = best[b];
+                w = where[b];
+            }
+        const uint32_t most = wave_max_u32_dpp(k);
+        if (most == 0) return -1;
+        const unsigned long long holders = __ballot(k == most);
+        uint32_t c = w * 64 + lane;
+        if (__popcll(holders) == 1) c = (uint32_t)__builtin_amdgcn_readlane((int)c, __ffsll(holders) - 1);
+        else c = ~wave_max_u32_dpp(k == most ? ~c : 0);
+        remove<0>(c / 64, c % 64, lane);
+        return (int)c;
+    }
+};
+
+// A wave per image, for up to 2048 neurons in at most 64 groups: keys in registers, the k largest taken one by one (a maximum over
+// the wave each).  With groups, keys go through LDS: lane g finds group g's two largest, groups are kept by counting how many go
+// before each, and only the kept groups' neurons are candidates, in the order of their numbers.
+// J: registers for all neurons, C: for the candidates; FULL: gates over the sum of all neurons that take part.
+template <int J, int C, bool FULL> __global__ __launch_bounds__(256) void k_route_wave(const RouteArgs g, uint32_t over_size)
+{
+    extern __shared__ __align__(16) uint32_t lds[];        // with groups: waves x (groups x line + 64)
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t t = blockIdx.x * 4 + wave;
+    if (t >= g.images) return;                             // (no barriers below)
+    const float *const row = g.distances + (uint64_t)t * g.stride;
+    uint32_t keys_of[J];
+    Candidates<C> c;
+    float top = -INFINITY, total = 0.0f;
+    {
+        float z[FULL ? J : 1];
+        constexpr int kAtOnce = J < 8 ? J : J % 8 ? 4 : 8;               // loads of so many registers are under way together
+#pragma unroll
+        for (int j0 = 0; j0 < J; j0 += kAtOnce) {
+            float d[kAtOnce], of[kAtOnce], to[kAtOnce], bias[kAtOnce];
+            uint32_t n[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+                n[j] = min((uint32_t)(j0 + j) * 64 + lane, g.neurons - 1);
+                d[j] = row[n[j]];
+                of[j] = g.sharpness[n[j]];
+                to[j] = g.radius[n[j]];
+                bias[j] = 0.0f;
+            }
+            if (g.bias) {
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) bias[j] = g.bias[n[j]];
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+                const float at = of[j] * (to[j] - d[j]);
+                const uint32_t key = order_key(at + bias[j]);
+                if (FULL) z[j0 + j] = at;
+                keys_of[j0 + j] = (uint32_t)(j0 + j) * 64 + lane < g.neurons ? key : 0;
+                asm volatile("" : "+v"(keys_of[j0 + j]));  // formed here: what it is formed from would take four registers, and waves with them
+            }
+        }
+        if constexpr (FULL) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) top = fmaxf(top, keys_of[j] ? z[j] : -INFINITY);
+            top = wave_max(top);
+#pragma unroll
+            for (int j = 0; j < J; ++j) total += keys_of[j] ? expf(z[j] - top) : 0.0f;
+            total = wave_sum(total);
+        }
+    }
+    const uint32_t line = g.group_size | 1;                // a group's keys in LDS: an odd step, so that lanes reading one each meet no banks
+    uint32_t *const keys = lds + wave * (g.groups * line + 64), *const kept_groups = keys + g.groups * line;
+    if (g.groups > 1) {
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            if (j * 64 + lane < g.neurons) {
+                const uint32_t n = j * 64 + lane, group = g.group_size == 1 ? n : __umulhi(n, over_size);
+                keys[n + group * (line - g.group_size)] = keys_of[j];
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        uint32_t score = 0;
+        if (lane < g.groups) {
+            const uint32_t size = min(g.group_size, g.neurons - lane * g.group_size);
+            const uint32_t *const mine = keys + lane * line;
+            uint32_t first = 0, second = 0;
+#pragma unroll 8
+            for (uint32_t i = 0; i < size; ++i) {
+                const uint32_t key = mine[i];
+                second = max(second, min(first, key));
+                first = max(first, key);
+            }
+            score = group_score(first, second);
+        }
+        unsigned long long all = 0;                        // the kept groups, taken one by one
+        for (uint32_t k = 0; k < g.groups_kept; ++k) {
+            const uint32_t most = wave_max_u32_dpp(score);
+            if (most == 0) break;
+            const unsigned long long one = __ballot(score == most) & -__ballot(score == most);
+            all |= one;
+            if (one >> lane & 1) score = 0;
+        }
+        const bool kept = all >> lane & 1;
+        if (kept) kept_groups[__popcll(all & ((1ull << lane) - 1))] = lane;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const uint32_t count = __popcll(all) * g.group_size;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            c.key[j] = 0;
+            if (j * 64 < count) {
+                const uint32_t i = j * 64 + lane, slot = g.group_size == 1 ? i : __umulhi(i, over_size);
+                if (i < count) {
+                    const uint32_t group = kept_groups[slot], in_group = i - slot * g.group_size;
+                    if (group * g.group_size + in_group < g.neurons) c.key[j] = keys[group * line + in_group];
+                }
+            }
+        }
+    }
+    if (g.groups == 1) {
+#pragma unroll
+        for (int j = 0; j < C; ++j) c.key[j] = j < J ? keys_of[j] : 0;
+    }
+    c.template find_all<0>();
+    int mine = -1;
+    for (uint32_t s = 0; s < g.chosen; ++s) {
+        const int next = c.take(lane);
+        if (next < 0) break;
+        if (lane == s) mine = next;
+    }
+    if (mine >= 0 && g.groups > 1) {
+        const uint32_t slot = g.group_size == 1 ? (uint32_t)mine : __umulhi((uint32_t)mine, over_size);
+        mine = (int)(kept_groups[slot] * g.group_size + ((uint32_t)mine - slot * g.group_size));
+    }
+    const float gate = gate_of(g, mine >= 0 ? logit(g, row, mine) : 0.0f, mine >= 0, top, total);
+    if (lane < g.chosen) {
+        g.neuron[(uint64_t)t * g.chosen + lane] = mine;
+        g.gates[(uint64_t)t * g.chosen + lane] = gate;
     }
 }
 
@@ -249,12 +442,12 @@ template <typename E> __global__ __launch_bounds__(256) void k_route_backward(co
             float top = -INFINITY, total = 0.0f;
             for (uint32_t m = lane; m < g.neurons; m += 64) {
                 const float v = logit(g, row, m);
-                if (order_key(v, g.bias ? v + g.bias[m] : v)) top = fmaxf(top, v);
+                if (order_key(g.bias ? v + g.bias[m] : v)) top = fmaxf(top, v);
             }
             top = wave_max(top);
             for (uint32_t m = lane; m < g.neurons; m += 64) {
                 const float v = logit(g, row, m);
-                if (order_key(v, g.bias ? v + g.bias[m] : v)) total += expf(v - top);
+                if (order_key(g.bias ? v + g.bias[m] : v)) total += expf(v - top);
             }
             total = wave_sum(total);
             if (lane == 0) {
@@ -275,7 +468,7 @@ template <typename E> __global__ __launch_bounds__(256) void k_route_backward(co
         float d = 0.0f;
         if (full) {
             const float v = sharpness * (radius - g.distances[place]);
-            if (order_key(v, v + bias)) d = -pull_of[i] * (expf(v - top_of[i]) * over_of[i]);
+            if (order_key(v + bias)) d = -pull_of[i] * (expf(v - top_of[i]) * over_of[i]);
         }
         for (uint32_t s = 0; s < g.chosen; ++s)
             if (at[i * g.chosen + s] == (int32_t)n) d += dz[i * g.chosen + s];
@@ -291,25 +484,30 @@ template <typename E> __global__ __launch_bounds__(256) void k_route_backward(co
     }
 }
 
-// Column sums of the chunks' parts: 64 columns by 4 waves, each a quarter of the chunks in order.
-__global__ __launch_bounds__(256) void k_route_sums(const float *sharpness_part, const float *radius_part, uint32_t chunks, uint32_t neurons,
-                                                    float *sharpness_out, float *radius_out)
+// Column sums of the chunks' parts: 64 columns by 16 waves, each a sixteenth of the chunks in order.
+__global__ __launch_bounds__(1024) void k_route_sums(const float *sharpness_part, const float *radius_part, uint32_t chunks, uint32_t neurons,
+                                                     float *sharpness_out, float *radius_out)
 {
-    __shared__ float held[2][4][64];
+    __shared__ float held[2][16][64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
-    const uint32_t each = (chunks + 3) / 4, first = wave * each, end = min(first + each, chunks);
+    const uint32_t each = (chunks + 15) / 16, first = min(wave * each, chunks), end = min(first + each, chunks);
     float s = 0.0f, r = 0.0f;
-    if (n < neurons)
+    if (n < neurons) {
+#pragma unroll 8
         for (uint32_t c = first; c < end; ++c) {
             s += sharpness_part[(uint64_t)c * neurons + n];
             r += radius_part[(uint64_t)c * neurons + n];
         }
+    }
     held[0][wave][lane] = s;
     held[1][wave][lane] = r;
     __syncthreads();
-    if (wave || n >= neurons) return;
-    if (sharpness_out) sharpness_out[n] = (held[0][0][lane] + held[0][1][lane]) + (held[0][2][lane] + held[0][3][lane]);
-    if (radius_out) radius_out[n] = (held[1][0][lane] + held[1][1][lane]) + (held[1][2][lane] + held[1][3][lane]);
+    if (wave > 1 || n >= neurons) return;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) sum += held[wave][w][lane];
+    float *const out = wave ? radius_out : sharpness_out;
+    if (out) out[n] = sum;
 }
 
 // One block: how often each neuron was chosen, then a step of the bias against the mean.
@@ -1176,8 +1374,37 @@ int pink_hip_readout_route(pink_hip_readout *r, const float *distances, uint32_t
     RouteArgs g = route_args(r, distances, images, stride, sharpness, radius, bias);
     g.neuron = neuron;
     g.gates = gates;
-    k_route_block<<<images, 256, (g.neurons + (g.groups > 1 ? g.groups : 0)) * 4, r->stream>>>(g);
-    return launched(r, "k_route_block");
+    const uint32_t candidates = std::max(g.neurons, g.groups_kept * g.group_size);
+    if (candidates > 2048 || (g.groups > 1 && g.groups > 64)) {
+        k_route_block<<<images, 256, (g.neurons + (g.groups > 1 ? g.groups : 0)) * 4, r->stream>>>(g);
+        return launched(r, "k_route_block");
+    }
+    const uint32_t lds = g.groups > 1 ? 4 * (g.groups * (g.group_size | 1) + 64) * 4 : 0, blocks = (images + 3) / 4;
+    const uint32_t over_size = g.groups > 1 ? (uint32_t)((1ull << 32) / g.group_size + 1) : 0;
+    // Registers for every 64 neurons; with groups the candidates are fewer, and where 8 registers hold them that is
+    // what taking them out of 16000 x 1600 distances in 8 of 40 groups goes through.
+    const bool few = g.groups > 1 && g.groups_kept * g.group_size <= 512;
+    const auto run = [&](auto j) {
+        constexpr int J = decltype(j)::value;
+        constexpr int C = J < 8 ? J : 8;
+        const bool full = !g.renormalise && !g.sigmoid;
+        if (few && full) k_route_wave<J, C, true><<<blocks, 256, lds, r->stream>>>(g, over_size);
+        else if (few) k_route_wave<J, C, false><<<blocks, 256, lds, r->stream>>>(g, over_size);
+        else if (full) k_route_wave<J, J, true><<<blocks, 256, lds, r->stream>>>(g, over_size);
+        else k_route_wave<J, J, false><<<blocks, 256, lds, r->stream>>>(g, over_size);
+    };
+    const uint32_t registers = (candidates + 63) / 64;
+    if (registers <= 2) run(std::integral_constant<int, 2>());
+    else if (registers <= 4) run(std::integral_constant<int, 4>());
+    else if (registers <= 6) run(std::integral_constant<int, 6>());
+    else if (registers <= 8) run(std::integral_constant<int, 8>());
+    else if (registers <= 12) run(std::integral_constant<int, 12>());
+    else if (registers <= 16) run(std::integral_constant<int, 16>());
+    else if (registers <= 20) run(std::integral_constant<int, 20>());
+    else if (registers <= 24) run(std::integral_constant<int, 24>());
+    else if (registers <= 28) run(std::integral_constant<int, 28>());
+    else run(std::integral_constant<int, 32>());
+    return launched(r, "k_route_wave");
 }
 
 int pink_hip_readout_route_backward(pink_hip_readout *r, const float *distances, uint32_t images, uint64_t stride, const float *sharpness,
@@ -1198,7 +1425,7 @@ int pink_hip_readout_route_backward(pink_hip_readout *r, const float *distances,
     a.gate_gradients = gate_gradients;
     a.distance_gradients = ddistances;
     a.want_sums = dsharpness || dradius;
-    a.chunk = std::max(4u, std::min(kChunkMost, images / 512));
+    a.chunk = std::max(4u, std::min(kChunkMost, images / 256));
     a.chunk = std::max(a.chunk, (images + 65534) / 65535);               // (the grid's second dimension)
     REFUSE(r, a.chunk > kChunkMost, "too many images for one call");
     const uint32_t chunks = (images + a.chunk - 1) / a.chunk;
@@ -1213,7 +1440,7 @@ int pink_hip_readout_route_backward(pink_hip_readout *r, const float *distances,
         TRY(launched(r, "k_route_backward"));
     }
     if (!a.want_sums) return PINK_HIP_OK;
-    k_route_sums<<<(neurons + 63) / 64, 256, 0, r->stream>>>(a.sharpness_part, a.radius_part, chunks, neurons, dsharpness, dradius);
+    k_route_sums<<<(neurons + 63) / 64, 1024, 0, r->stream>>>(a.sharpness_part, a.radius_part, chunks, neurons, dsharpness, dradius);
     return launched(r, "k_route_sums");
 }
 
