@@ -575,8 +575,10 @@ __device__ __forceinline__ unsigned long long block_prefix(unsigned long long v,
     return before + sum - v;
 }
 
-// First rows and tiles of all neurons from their numbers of rows: rows in the low half, tiles in the high half of one sum.
-template <typename Count> __device__ __forceinline__ void plan_offsets(const PlanArgs &g, const Count &count, unsigned long long *shared)
+// First rows and tiles of all neurons from their numbers of rows: rows in the low half, tiles in the high half of one sum.  A thread
+// has a run of neurons; `count` gives a neuron's number of rows and `starts` is told its first row.
+template <typename Count, typename Starts>
+__device__ __forceinline__ void plan_offsets(const PlanArgs &g, const Count &count, const Starts &starts, unsigned long long *shared)
 {
     const uint32_t each = (g.neurons + blockDim.x - 1) / blockDim.x;
     const uint32_t first = min(threadIdx.x * each, g.neurons), end = min(first + each, g.neurons);
@@ -586,9 +588,11 @@ template <typename Count> __device__ __forceinline__ void plan_offsets(const Pla
         mine += c | (unsigned long long)((c + g.tile_rows - 1) / g.tile_rows) << 32;
     }
     unsigned long long at = block_prefix(mine, shared, &total);
+    uint32_t last = (uint32_t)mine;                        // (of a run of one: its count)
     for (uint32_t n = first; n < end; ++n) {
-        const uint32_t c = count(n);
+        const uint32_t c = each == 1 ? last : count(n);
         g.offsets[n] = (uint32_t)at;
+        starts(n, (uint32_t)at);
         uint32_t tile = (uint32_t)(at >> 32);
         for (uint32_t r = 0; r < c; r += g.tile_rows) g.tiles[tile++] = make_uint2(n, (uint32_t)at + r);
         at += c | (unsigned long long)((c + g.tile_rows - 1) / g.tile_rows) << 32;
@@ -605,15 +609,18 @@ template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanAr
     extern __shared__ __align__(16) uint32_t hist[];       // waves x N
     __shared__ unsigned long long shared[16];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    for (uint32_t i = threadIdx.x; i < waves * g.neurons; i += blockDim.x) hist[i] = 0;
-    __syncthreads();
-    volatile uint32_t *const mine = hist + wave * g.neurons;
     const uint64_t first = ((uint64_t)blockIdx.x * waves + wave) * 64 * kPerWave;
     uint32_t rank[kPerWave], id[kPerWave];
 #pragma unroll
     for (uint32_t i = 0; i < kPerWave; ++i) {
         const uint64_t slot = first + i * 64 + lane;
         id[i] = slot < g.slots ? (uint32_t)g.neuron[slot] : 0xffffffffu;
+    }
+    for (uint32_t i = threadIdx.x; i < waves * g.neurons; i += blockDim.x) hist[i] = 0;
+    __syncthreads();
+    volatile uint32_t *const mine = hist + wave * g.neurons;
+#pragma unroll
+    for (uint32_t i = 0; i < kPerWave; ++i) {
         const bool valid = id[i] < g.neurons;
         unsigned long long same = __ballot(valid);
         for (uint32_t b = 0; (g.neurons - 1) >> b; ++b) {
@@ -627,29 +634,47 @@ template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanAr
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    for (uint32_t n = threadIdx.x; n < g.neurons; n += blockDim.x) {
+    // Of a neuron's rows those of the waves before; returns all of the block's.
+    const auto over_waves = [&](uint32_t n) {
         uint32_t before = 0;
         for (uint32_t w = 0; w < waves; ++w) {
             const uint32_t c = hist[w * g.neurons + n];
             hist[w * g.neurons + n] = before;
             before += c;
         }
-        if (STAGE != 1) g.counts[(uint64_t)blockIdx.x * g.neurons + n] = before;
+        return before;
+    };
+    if constexpr (STAGE == 2) {
+        bool again = false;                                // (of a run of several neurons, counts are looked at twice: kept in memory)
+        plan_offsets(
+            g,
+            [&](uint32_t n) {
+                if (g.neurons <= blockDim.x) return over_waves(n);
+                const uint32_t each = (g.neurons + blockDim.x - 1) / blockDim.x;
+                if (!again) g.counts[n] = over_waves(n);
+                again = again || n + 1 == min((threadIdx.x + 1) * each, g.neurons);
+                return g.counts[n];
+            },
+            [&](uint32_t n, uint32_t start) {
+                for (uint32_t w = 0; w < waves; ++w) hist[w * g.neurons + n] += start;
+            },
+            shared);
+    } else {
+        for (uint32_t n = threadIdx.x; n < g.neurons; n += blockDim.x) {
+            const uint32_t all = over_waves(n);
+            if (STAGE == 0) g.counts[(uint64_t)blockIdx.x * g.neurons + n] = all;
+        }
     }
     if (STAGE == 0) return;
-    __syncthreads();                                       // (counts and offsets go through memory, within the block)
-    if (STAGE == 2) {
-        plan_offsets(g, [&](uint32_t n) { return g.counts[n]; }, shared);
-        __syncthreads();
-    }
+    __syncthreads();
 #pragma unroll
     for (uint32_t i = 0; i < kPerWave; ++i) {
         const uint64_t slot = first + i * 64 + lane;
         if (slot >= g.slots) continue;
         int32_t row = -1;
         if (id[i] < g.neurons) {
-            row = (int32_t)(g.offsets[id[i]] + hist[wave * g.neurons + id[i]] + rank[i]);
-            if (STAGE == 1) row += (int32_t)g.counts[(uint64_t)blockIdx.x * g.neurons + id[i]];
+            row = (int32_t)(hist[wave * g.neurons + id[i]] + rank[i]);
+            if (STAGE == 1) row += (int32_t)(g.offsets[id[i]] + g.counts[(uint64_t)blockIdx.x * g.neurons + id[i]]);
             g.order[row] = (uint32_t)slot;
             g.images[row] = (uint32_t)slot / g.chosen;
             g.owner[row] = id[i];
@@ -672,7 +697,117 @@ __global__ __launch_bounds__(1024) void k_plan_offsets(const PlanArgs g, uint32_
         totals[n] = before;
     }
     __syncthreads();
-    plan_offsets(g, [&](uint32_t n) { return totals[n]; }, shared);
+    plan_offsets(g, [&](uint32_t n) { return totals[n]; }, [](uint32_t, uint32_t) {}, shared);
+}
+
+// ---------------------------------------------------------------------------------
+// Few images: a slot by itself
+// ---------------------------------------------------------------------------------
+
+struct FewArgs {
+    const void *x;
+    uint64_t x_stride;
+    const int32_t *neuron;
+    const float *gates;
+    const void *first, *first_bias, *second, *second_bias, *residual;
+    uint64_t residual_stride, y_stride;
+    uint32_t neurons, chosen, features, hidden, outputs, activation;
+    float *after;                  // slots x hidden
+    void *y;
+};
+
+template <typename E> __device__ __forceinline__ void to_floats(const uint4 &chunk, float (&v)[16 / sizeof(E)])
+{
+    E e[16 / sizeof(E)];
+    __builtin_memcpy(e, &chunk, sizeof e);
+#pragma unroll
+    for (uint32_t i = 0; i < 16 / sizeof(E); ++i) v[i] = to_float(e[i]);
+}
+
+// With a handful of slots nothing is shared and what there is to do is to read each slot's weights once: a wave takes four rows of
+// a matrix, its lanes 16 bytes each along them, and sums up over the lanes.  No sorting, no tiles, two launches; sums and what
+// lies between the layers stay in float32.
+constexpr uint32_t kFewRows = 4;
+
+template <typename E> __global__ __launch_bounds__(256) void k_few_hidden(const FewArgs g)
+{
+    constexpr uint32_t per = 16 / sizeof(E);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t slot = blockIdx.y, neuron = (uint32_t)g.neuron[slot], h0 = (blockIdx.x * 4 + wave) * kFewRows;
+    if (neuron >= g.neurons || h0 >= g.hidden) return;
+    const E *const x = (const E *)g.x + (uint64_t)(slot / g.chosen) * g.x_stride;
+    const E *w[kFewRows];
+#pragma unroll
+    for (uint32_t i = 0; i < kFewRows; ++i) w[i] = (const E *)g.first + ((uint64_t)neuron * g.hidden + min(h0 + i, g.hidden - 1)) * g.features;
+    float sum[kFewRows] = {};
+    for (uint32_t k = lane * per; k < g.features; k += 64 * per) {
+        const int valid = (int)(g.features - k);
+        float a[per];
+        uint4 b[kFewRows];
+        to_floats<E>(load_chunk(x + k, valid), a);
+#pragma unroll
+        for (uint32_t i = 0; i < kFewRows; ++i) b[i] = load_chunk(w[i] + k, valid);
+#pragma unroll
+        for (uint32_t i = 0; i < kFewRows; ++i) {
+            float v[per];
+            to_floats<E>(b[i], v);
+#pragma unroll
+            for (uint32_t e = 0; e < per; ++e) sum[i] = fmaf(a[e], v[e], sum[i]);
+        }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kFewRows; ++i) {
+        float v = wave_sum(sum[i]);
+        if (lane == 0 && h0 + i < g.hidden) {
+            if (g.first_bias) v += to_float(((const E *)g.first_bias)[(uint64_t)neuron * g.hidden + h0 + i]);
+            g.after[(uint64_t)slot * g.hidden + h0 + i] = g.gates[slot] * activation<E, false>(g.activation, v).value;
+        }
+    }
+}
+
+template <typename E> __global__ __launch_bounds__(256) void k_few_answer(const FewArgs g)
+{
+    constexpr uint32_t per = 16 / sizeof(E);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t t = blockIdx.y, o0 = (blockIdx.x * 4 + wave) * kFewRows;
+    if (o0 >= g.outputs) return;
+    float sum[kFewRows] = {}, bias[kFewRows] = {};
+    for (uint32_t s = 0; s < g.chosen; ++s) {
+        const uint32_t slot = t * g.chosen + s, neuron = (uint32_t)g.neuron[slot];
+        if (neuron >= g.neurons) continue;
+        const float *const after = g.after + (uint64_t)slot * g.hidden;
+        const E *w[kFewRows];
+#pragma unroll
+        for (uint32_t i = 0; i < kFewRows; ++i) {
+            const uint64_t row = (uint64_t)neuron * g.outputs + min(o0 + i, g.outputs - 1);
+            w[i] = (const E *)g.second + row * g.hidden;
+            if (g.second_bias) bias[i] += g.gates[slot] * to_float(((const E *)g.second_bias)[row]);
+        }
+        for (uint32_t k = lane * per; k < g.hidden; k += 64 * per) {
+            const int valid = (int)(g.hidden - k);
+            float a[per];
+            uint4 b[kFewRows];
+#pragma unroll
+            for (uint32_t e = 0; e < per; ++e) a[e] = (int)e < valid ? after[k + e] : 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < kFewRows; ++i) b[i] = load_chunk(w[i] + k, valid);
+#pragma unroll
+            for (uint32_t i = 0; i < kFewRows; ++i) {
+                float v[per];
+                to_floats<E>(b[i], v);
+#pragma unroll
+                for (uint32_t e = 0; e < per; ++e) sum[i] = fmaf(a[e], v[e], sum[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kFewRows; ++i) {
+        float v = wave_sum(sum[i]) + bias[i];
+        if (lane == 0 && o0 + i < g.outputs) {
+            if (g.residual) v += to_float(((const E *)g.residual)[t * g.residual_stride + o0 + i]);
+            ((E *)g.y)[t * g.y_stride + o0 + i] = from_float<E>(v);
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------
@@ -964,12 +1099,7 @@ struct Saved {
     uint64_t stride;               // of before's and after's rows: whole 16-byte chunks
 };
 
-#ifdef ROWS_CFG
-constexpr int kRowsCfg[5] = {ROWS_CFG};
-constexpr uint32_t kLeastTileRows = kRowsCfg[0];
-#else
-constexpr uint32_t kLeastTileRows = 128;
-#endif
+constexpr uint32_t kLeastTileRows = 16, kFewSlots = 512;
 
 Saved saved_layout(const pink_hip_readout *r, uint64_t images)
 {
@@ -1002,7 +1132,7 @@ uint32_t plan_waves(uint32_t neurons) { return std::max(1u, std::min(16u, 32768u
 uint64_t whole_rows(uint32_t cols) { return ((uint64_t)cols + 3) / 4 * 4; }
 
 struct Work {
-    size_t counts, totals, rows, partial, saved, bytes;
+    size_t counts, totals, rows, partial, few, saved, bytes;
 };
 
 Work work_layout(const pink_hip_readout *r, uint64_t images)
@@ -1020,6 +1150,7 @@ Work work_layout(const pink_hip_readout *r, uint64_t images)
     w.totals = take((size_t)c.neurons * 4);
     w.rows = take(slots * whole_rows(std::max(c.features, c.outputs)) * 4);
     w.partial = take(slots * ((c.hidden + 31) / 32) * 4);
+    w.few = take(std::min<size_t>(slots, kFewSlots) * c.hidden * 4);
     w.saved = take(saved_layout(r, images).bytes);         // forward calls that keep nothing; gradients of `before`
     w.bytes = at;
     return w;
@@ -1064,15 +1195,18 @@ RouteArgs route_args(const pink_hip_readout *r, const float *distances, uint32_t
     return g;
 }
 
-template <typename E, int OP> int product(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
+// Rows of a product's tiles, by how many rows a neuron has on average: the weights are read once for each tile of rows, and a tile
+// that is mostly empty multiplies for nothing.
+uint32_t tile_rows(const pink_hip_readout *r, uint64_t slots)
+{
+    const uint64_t neurons = std::min<uint64_t>(r->cfg.neurons, slots);
+    return slots <= 24 * neurons ? 16 : slots <= 64 * neurons ? 64 : 128;
+}
+
+template <typename E, int OP, int PR, int QC, int PW, int QW, int M, int DEEP>
+int product_of_tile(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
 {
     constexpr bool grad = OP == kGradFirst || OP == kGradSecond;
-#ifdef ROWS_CFG
-    constexpr int cfg[2][5] = {{ROWS_CFG}, {GRAD_CFG}};
-    constexpr int PR = cfg[grad][0], QC = cfg[grad][1], PW = cfg[grad][2], QW = cfg[grad][3], M = cfg[grad][4];
-#else
-    constexpr int PR = 128, QC = 128, PW = 2, QW = 2, M = 32;
-#endif
     g.col_tiles = grad && !g.out ? 1 : (g.cols + QC - 1) / QC;
     g.row_tiles = grad ? (g.rows + PR - 1) / PR : 0;
     const uint64_t tiles = grad ? (uint64_t)r->cfg.neurons * g.row_tiles : slots / PR + std::min<uint64_t>(r->cfg.neurons, slots);
@@ -1088,9 +1222,26 @@ template <typename E, int OP> int product(pink_hip_readout *r, ProductArgs &g, u
     if (OP == kBackInput) direct = direct && g.cols % per == 0;
     if (OP == kGradFirst) direct = direct && g.cols % per == 0;
     if (OP == kGradSecond) direct = direct && g.rows % per == 0;
-    if (direct) k_product<E, OP, PR, QC, PW, QW, M, true><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
-    else k_product<E, OP, PR, QC, PW, QW, M, false><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
+    if (direct) k_product<E, OP, PR, QC, PW, QW, M, DEEP, true><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
+    else k_product<E, OP, PR, QC, PW, QW, M, DEEP, false><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
     return launched(r, "k_product");
+}
+
+template <typename E, int OP> int product(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
+{
+    if constexpr (OP == kGradFirst || OP == kGradSecond) {
+        // Few rows a neuron: writing the gradients is what there is to do, and small tiles spread it.
+        if (slots <= 64 * (uint64_t)r->cfg.neurons) return product_of_tile<E, OP, 64, 64, 2, 2, 16, 1>(r, g, slots);
+        return product_of_tile<E, OP, 128, 128, 2, 2, 32, 1>(r, g, slots);
+    } else {
+        // Few rows a neuron: reading the weights is what there is to do; a stage takes 512 bytes of a row so that enough of it is
+        // under way.
+        switch (tile_rows(r, slots)) {
+        case 16: return product_of_tile<E, OP, 16, 32, 1, 2, 16, 4>(r, g, slots);
+        case 64: return product_of_tile<E, OP, 64, 64, 2, 2, 32, 2>(r, g, slots);
+        default: return product_of_tile<E, OP, 128, 128, 2, 2, 32, 1>(r, g, slots);
+        }
+    }
 }
 
 int plan(pink_hip_readout *r, const int32_t *neuron, uint32_t slots, char *saved, const Saved &s, const Work &w)
@@ -1101,7 +1252,7 @@ int plan(pink_hip_readout *r, const int32_t *neuron, uint32_t slots, char *saved
     g.neuron = neuron;
     g.slots = slots;
     g.neurons = c.neurons;
-    g.tile_rows = kLeastTileRows;
+    g.tile_rows = tile_rows(r, slots);
     g.counts = (uint32_t *)(work + w.counts);
     g.chosen = c.chosen;
     g.order = (uint32_t *)(saved + s.order);
@@ -1135,6 +1286,16 @@ int combine(pink_hip_readout *r, const float *rows, const int32_t *place, uint32
     return launched(r, "k_combine");
 }
 
+// Slots by themselves read their neuron's weights each, tiles once for a neuron; sorting and tiles cost some 10 us.  Measured (us, slots by
+// themselves / tiles): 100 neurons of 1.1 MB, bfloat16, 64 slots 13.5 / 21, 512 slots 34 / 28; of 4.5 MB, 64 slots 51 / 54, 128 slots
+// 87 / 72; 331 neurons of 1.7 MB, float32, 64 slots 26 / 51, 256 slots 73 / 90, 512 slots 130 / 119.
+bool is_few(const pink_hip_readout *r, uint64_t slots)
+{
+    const pink_hip_readout_config &c = r->cfg;
+    const uint64_t bytes = ((uint64_t)c.features + c.outputs) * c.hidden * element_bytes(r);
+    return slots <= 64 || (slots <= kFewSlots && (4 * slots <= 3 * (uint64_t)c.neurons || slots * bytes <= 64u << 20));
+}
+
 template <typename E>
 int experts(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stride, const int32_t *neuron, const float *gates,
             const pink_hip_readout_weights &weights, const void *residual, uint64_t residual_stride, void *y, uint64_t y_stride, void *keep)
@@ -1145,6 +1306,16 @@ int experts(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stri
     TRY(grow(r, w.bytes));
     char *const work = (char *)r->work, *const saved = keep ? (char *)keep : work + w.saved;
     const uint32_t slots = images * c.chosen;
+    if (!keep && is_few(r, slots)) {
+        const FewArgs f = {x, x_stride, neuron, gates, weights.first, weights.first_bias, weights.second, weights.second_bias, residual,
+                           residual_stride, y_stride, c.neurons, c.chosen, c.features, c.hidden, c.outputs, c.activation,
+                           (float *)(work + w.few), y};
+        constexpr uint32_t rows = 4 * kFewRows;
+        k_few_hidden<E><<<dim3((c.hidden + rows - 1) / rows, slots), 256, 0, r->stream>>>(f);
+        TRY(launched(r, "k_few_hidden"));
+        k_few_answer<E><<<dim3((c.outputs + rows - 1) / rows, images), 256, 0, r->stream>>>(f);
+        return launched(r, "k_few_answer");
+    }
     TRY(plan(r, neuron, slots, saved, s, w));
 
     ProductArgs g = {};

@@ -496,13 +496,14 @@ def test_experts(gpu, t, n, k, f, h, o, act, bias, residual, spread, pad, bf16):
     with capi.Readout(n, k, f, h, o, activation=ACT[act], element=element.id) as ro:
         saved = gpu.new(ro.saved_bytes(t), np.int8)
         answers = []
-        for keep in (None, saved):
+        for keep in (None, None, saved, saved):
             y = gpu.new((t, o + pad), element.dtype)
             ro.experts(p["x"], t, *where, weights, y, dev_residual=p["residual"], dev_saved=keep, x_stride=f + pad, residual_stride=o + pad, y_stride=o + pad)
             ro.synchronize()
             answers.append(gpu.down(y, (t, o + pad), element.dtype)[:, :o])
             assert_within(element.values(answers[-1]), *want["y"], "y")
-        assert np.array_equal(answers[0], answers[1])
+        # the same call gives the same bits (few images are summed in another order when nothing is kept for a backward pass)
+        assert np.array_equal(answers[0], answers[1]) and np.array_equal(answers[2], answers[3])
         grads = {i: gpu.new(s if i != "dx" else (t, f + pad), element.dtype) for i, s in names.items()}
         dy_dev = gpu.up(padded(dy_stored, pad, nan))
         for _ in range(2):                                 # twice: the same bits
