@@ -7,6 +7,7 @@ if it is missing: there is no CPU fallback.  Errors returned by the library beco
 """
 import ctypes as C
 import os
+import struct
 import sys
 
 import numpy as np
@@ -76,6 +77,10 @@ class ReadoutTensor(C.Structure):
     _fields_ = [(name, C.c_void_p) for name in ("value", "gradient", "rounded", "first", "second", "first_scale", "second_scale",
                                                 "first_values", "second_values")] + [
         ("size", C.c_uint64), ("decay", C.c_float), ("gradient_element", C.c_uint32)]
+
+
+_PACK_TENSOR, _TENSOR_BYTES = struct.Struct("@10QfI").pack_into, struct.calcsize("@10QfI")      # ReadoutTensor's fields
+assert _TENSOR_BYTES == C.sizeof(ReadoutTensor)
 
 
 _lib = None
@@ -487,14 +492,15 @@ class Readout:
     def tensors(described):
         """The argument of adamw() and adamw_unpack(): one dict for each tensor, with ReadoutTensor's fields as keys (gradient_bf16 in
         place of gradient_element)."""
-        out = (ReadoutTensor * len(described))()
-        for to, d in zip(out, described):
-            for key, value in d.items():
-                if key == "gradient_bf16":
-                    to.gradient_element = ELEMENT_BF16 if value else ELEMENT_F32
-                else:
-                    setattr(to, key, value)
-        return out
+        held = bytearray(len(described) * C.sizeof(ReadoutTensor))
+        at = 0
+        for d in described:
+            get = d.get
+            _PACK_TENSOR(held, at, get("value") or 0, get("gradient") or 0, get("rounded") or 0, get("first") or 0, get("second") or 0,
+                         get("first_scale") or 0, get("second_scale") or 0, get("first_values") or 0, get("second_values") or 0, d["size"],
+                         get("decay", 0.0), ELEMENT_BF16 if get("gradient_bf16") else ELEMENT_F32)
+            at += _TENSOR_BYTES
+        return (ReadoutTensor * len(described)).from_buffer(held)
 
     def adamw(self, tensors, step, learning_rate=1e-3, beta_first=0.9, beta_second=0.999, epsilon=1e-8, bits=32):
         """One step, the step'th (from 1), over the tensors that tensors() described."""

@@ -539,16 +539,15 @@ __global__ __launch_bounds__(1024) void k_balance(const int32_t *neuron, uint64_
 // Rows sorted by neuron
 // ---------------------------------------------------------------------------------
 
-// A stable counting sort of the slots by neuron.  A block takes waves * 64 * kPerWave slots in order; a wave goes through its
-// own in order with a histogram of its own, so that ranks need no atomics and the order is that of the images always.
-constexpr uint32_t kPerWave = 4;
+// A stable counting sort of the slots by neuron.  A block takes waves * 64 * PER slots in order (four where one block does all,
+// one where blocks share the work); a wave goes through its own in order with a histogram of its own, so that ranks need no atomics and the order is that of the images always.
 
 struct PlanArgs {
     const int32_t *neuron;
     uint32_t slots, neurons, tile_rows;
     uint32_t *counts;              // blocks x N
-    uint32_t *order, *images, *owner, *offsets, *tile_count;      // row -> slot, image, neuron; neuron -> first row
-    uint32_t chosen;
+    uint32_t *order, *offsets, *tile_count;                // row -> slot; neuron -> first row
+    int32_t *owner;                // slot -> neuron
     int32_t *place;                // slot -> row, -1 where it has none
     uint2 *tiles;
 };
@@ -604,15 +603,18 @@ __device__ __forceinline__ void plan_offsets(const PlanArgs &g, const Count &cou
 }
 
 // STAGE 0: count only; 1: place rows, from counts' prefixes; 2: all in one block.
+template <int STAGE> constexpr uint32_t kPerWave = STAGE == 2 ? 4 : 1;
+
 template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanArgs g)
 {
+    constexpr uint32_t PER = kPerWave<STAGE>;
     extern __shared__ __align__(16) uint32_t hist[];       // waves x N
     __shared__ unsigned long long shared[16];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const uint64_t first = ((uint64_t)blockIdx.x * waves + wave) * 64 * kPerWave;
-    uint32_t rank[kPerWave], id[kPerWave];
+    const uint64_t first = ((uint64_t)blockIdx.x * waves + wave) * 64 * PER;
+    uint32_t rank[PER], id[PER];
 #pragma unroll
-    for (uint32_t i = 0; i < kPerWave; ++i) {
+    for (uint32_t i = 0; i < PER; ++i) {
         const uint64_t slot = first + i * 64 + lane;
         id[i] = slot < g.slots ? (uint32_t)g.neuron[slot] : 0xffffffffu;
     }
@@ -620,7 +622,7 @@ template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanAr
     __syncthreads();
     volatile uint32_t *const mine = hist + wave * g.neurons;
 #pragma unroll
-    for (uint32_t i = 0; i < kPerWave; ++i) {
+    for (uint32_t i = 0; i < PER; ++i) {
         const bool valid = id[i] < g.neurons;
         unsigned long long same = __ballot(valid);
         for (uint32_t b = 0; (g.neurons - 1) >> b; ++b) {
@@ -668,7 +670,7 @@ template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanAr
     if (STAGE == 0) return;
     __syncthreads();
 #pragma unroll
-    for (uint32_t i = 0; i < kPerWave; ++i) {
+    for (uint32_t i = 0; i < PER; ++i) {
         const uint64_t slot = first + i * 64 + lane;
         if (slot >= g.slots) continue;
         int32_t row = -1;
@@ -676,10 +678,9 @@ template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanAr
             row = (int32_t)(hist[wave * g.neurons + id[i]] + rank[i]);
             if (STAGE == 1) row += (int32_t)(g.offsets[id[i]] + g.counts[(uint64_t)blockIdx.x * g.neurons + id[i]]);
             g.order[row] = (uint32_t)slot;
-            g.images[row] = (uint32_t)slot / g.chosen;
-            g.owner[row] = id[i];
         }
         g.place[slot] = row;
+        g.owner[slot] = (int32_t)id[i];
     }
 }
 
@@ -843,7 +844,7 @@ __global__ __launch_bounds__(256) void k_combine(const float *rows, const int32_
 
 // d gate of a slot = dy . (W2 f(a) + b2) = sum of its row's parts + dy . b2; a wave per slot.
 template <typename E>
-__global__ __launch_bounds__(256) void k_gate_gradients(const float *partial, uint32_t parts, const int32_t *place, const uint32_t *owner,
+__global__ __launch_bounds__(256) void k_gate_gradients(const float *partial, uint32_t parts, const int32_t *place, const int32_t *owner,
                                                         uint64_t slots, uint32_t chosen, const E *dy, uint64_t dy_stride,
                                                         uint32_t cols, const E *bias, E *out)
 {
@@ -855,7 +856,7 @@ __global__ __launch_bounds__(256) void k_gate_gradients(const float *partial, ui
     if (row >= 0) {
         for (uint32_t i = lane; i < parts; i += 64) v += partial[(uint64_t)row * parts + i];
         if (bias) {
-            const uint64_t neuron = owner[row];
+            const uint64_t neuron = (uint32_t)owner[slot];
             const E *const d = dy + slot / chosen * dy_stride;
             for (uint32_t c = lane; c < cols; c += 64) v += to_float(d[c]) * to_float(bias[neuron * cols + c]);
         }
@@ -874,7 +875,7 @@ __global__ __launch_bounds__(256) void k_clear(uint8_t *at, uint64_t bytes)
 // AdamW
 // ---------------------------------------------------------------------------------
 
-constexpr uint32_t kAdamTensors = 32, kAdamChunk = 2048;   // tensors of a launch (their table is a kernel argument), values of a block
+constexpr uint32_t kAdamTensors = 32, kAdamRuns = 2, kAdamChunk = 1024 * kAdamRuns;      // tensors of a launch (their table is a kernel argument), values of a block
 
 struct AdamArgs {
     pink_hip_readout_tensor tensor[kAdamTensors];
@@ -890,27 +891,24 @@ __device__ __forceinline__ uint32_t adam_tensor(const AdamArgs &g)
     return i;
 }
 
-template <typename V, int N> struct Run {                  // N values at their own alignment
-    V v[N];
-};
-
-template <typename V> __device__ __forceinline__ void load_run(V (&v)[8], const V *at, uint32_t valid)
+// Four neighbours at their own alignment, those from `valid` on zero and not touched.
+template <typename V> __device__ __forceinline__ void load_run(V (&v)[4], const V *at, uint32_t valid)
 {
-    if (valid >= 8) {
+    if (valid >= 4) {
         __builtin_memcpy(v, at, sizeof v);
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) v[i] = i < valid ? at[i] : V{};
+        for (uint32_t i = 0; i < 4; ++i) v[i] = i < valid ? at[i] : V{};
     }
 }
 
-template <typename V> __device__ __forceinline__ void store_run(V *at, const V (&v)[8], uint32_t valid)
+template <typename V> __device__ __forceinline__ void store_run(V *at, const V (&v)[4], uint32_t valid)
 {
-    if (valid >= 8) {
+    if (valid >= 4) {
         __builtin_memcpy(at, v, sizeof v);
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i)
+        for (uint32_t i = 0; i < 4; ++i)
             if (i < valid) at[i] = v[i];
     }
 }
@@ -928,93 +926,114 @@ __device__ __forceinline__ float second_value(uint8_t code, float scale)
     return (u * u) * scale;
 }
 
-// The largest of the 32 lanes that hold one block of codes.
-__device__ __forceinline__ float half_wave_max(float v)
-{
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    return v;
-}
-
-// A thread has eight neighbouring values, so a block of 256 codes belongs to half a wave.
+// A thread has kAdamRuns times four neighbouring values, 1024 apart, so that a wave's access is a run of memory and a block of 256
+// codes belongs to a wave.  All that is read is asked for before anything is done with it.  The states follow by sums, products,
+// roots and reciprocals that are each rounded (the codes are whole numbers and must not go by how they were computed); the
+// value's own step takes the hardware's root and reciprocal, one unit off at most, which is 2^-23 of a step.
 template <bool CODES> __global__ __launch_bounds__(256) void k_adamw(const AdamArgs g)
 {
     const uint32_t which = adam_tensor(g);
     const pink_hip_readout_tensor &t = g.tensor[which];
-    const uint64_t at = (uint64_t)(blockIdx.x - g.first_block[which]) * kAdamChunk + threadIdx.x * 8;
-    const uint32_t valid = at >= t.size ? 0 : (uint32_t)min((uint64_t)8, t.size - at);
-    if (__ballot(valid != 0) == 0) return;
+    const uint64_t base = (uint64_t)(blockIdx.x - g.first_block[which]) * kAdamChunk + threadIdx.x * 4;
 
-    float p[8], d[8], m[8], v[8];
-    load_run(p, t.value + at, valid);
-    if (t.gradient_element == PINK_HIP_ELEMENT_BFLOAT) {
-        Bfloat b[8];
-        load_run(b, (const Bfloat *)t.gradient + at, valid);
+    float p[kAdamRuns][4], d[kAdamRuns][4], m[kAdamRuns][4], v[kAdamRuns][4];
+    Bfloat half[kAdamRuns][4];
+    int8_t mc[kAdamRuns][4];
+    uint8_t vc[kAdamRuns][4];
+    float ms[kAdamRuns], vs[kAdamRuns];
+    uint32_t valid[kAdamRuns];
+    const bool halves = t.gradient_element == PINK_HIP_ELEMENT_BFLOAT;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = to_float(b[i]);
-    } else {
-        load_run(d, (const float *)t.gradient + at, valid);
-    }
-    const uint64_t block = at / kBlock8;
-    if constexpr (CODES) {
-        int8_t mc[8];
-        uint8_t vc[8];
-        load_run(mc, (const int8_t *)t.first + at, valid);
-        load_run(vc, (const uint8_t *)t.second + at, valid);
-        const float ms = valid ? t.first_scale[block] : 0.0f, vs = valid ? t.second_scale[block] : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            m[i] = first_value(mc[i], ms);
-            v[i] = second_value(vc[i], vs);
+    for (uint32_t n = 0; n < kAdamRuns; ++n) {
+        const uint64_t at = base + n * 1024;
+        valid[n] = at >= t.size ? 0 : (uint32_t)min((uint64_t)4, t.size - at);
+        load_run(p[n], t.value + at, valid[n]);
+        if (halves) load_run(half[n], (const Bfloat *)t.gradient + at, valid[n]);
+        else load_run(d[n], (const float *)t.gradient + at, valid[n]);
+        if constexpr (CODES) {
+            load_run(mc[n], (const int8_t *)t.first + at, valid[n]);
+            load_run(vc[n], (const uint8_t *)t.second + at, valid[n]);
+            ms[n] = valid[n] ? t.first_scale[at / kBlock8] : 0.0f;
+            vs[n] = valid[n] ? t.second_scale[at / kBlock8] : 0.0f;
+        } else {
+            load_run(m[n], (const float *)t.first + at, valid[n]);
+            load_run(v[n], (const float *)t.second + at, valid[n]);
         }
-    } else {
-        load_run(m, (const float *)t.first + at, valid);
-        load_run(v, (const float *)t.second + at, valid);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        m[i] = m[i] * g.beta1 + d[i] * g.rest1;
-        v[i] = v[i] * g.beta2 + (d[i] * d[i]) * g.rest2;
-        const float step = (m[i] * g.c1) / (sqrtf(v[i] * g.c2) + g.epsilon);
-        p[i] = p[i] - (step + p[i] * t.decay) * g.rate;
-    }
-    store_run(t.value + at, p, valid);
-    if (t.rounded) {
-        Bfloat b[8];
+    for (uint32_t n = 0; n < kAdamRuns; ++n) {
+        const uint64_t at = base + n * 1024;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = from_float<Bfloat>(p[i]);
-        store_run((Bfloat *)t.rounded + at, b, valid);
-    }
-    if constexpr (CODES) {
-        float ms = 0.0f, vs = 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            const float grad = halves ? to_float(half[n][i]) : d[n][i];
+            if constexpr (CODES) {
+                m[n][i] = first_value(mc[n][i], ms[n]);
+                v[n][i] = second_value(vc[n][i], vs[n]);
+            }
+            m[n][i] = m[n][i] * g.beta1 + grad * g.rest1;
+            v[n][i] = v[n][i] * g.beta2 + (grad * grad) * g.rest2;
+            const float step = (m[n][i] * g.c1) * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[n][i] * g.c2) + g.epsilon);
+            p[n][i] = p[n][i] - (step + p[n][i] * t.decay) * g.rate;
+        }
+        store_run(t.value + at, p[n], valid[n]);
+        if (t.rounded) {
+            Bfloat b[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            ms = fmaxf(ms, fabsf(m[i]));                   // (values past the end are zero)
-            vs = fmaxf(vs, fabsf(v[i]));
+            for (int i = 0; i < 4; ++i) b[i] = from_float<Bfloat>(p[n][i]);
+            store_run((Bfloat *)t.rounded + at, b, valid[n]);
         }
-        ms = half_wave_max(ms);
-        vs = half_wave_max(vs);
-        ms = ms < 1.175494351e-38f ? 0.0f : ms;
-        vs = vs < 1.175494351e-38f ? 0.0f : vs;
-        const float mi = ms > 0.0f ? 1.0f / ms : 0.0f, vi = vs > 0.0f ? 1.0f / vs : 0.0f;
-        int8_t mc[8];
-        uint8_t vc[8];
+        if constexpr (CODES) {
+            // (values past the end are zero; magnitudes order as their bits do)
+            float most_m = 0.0f, most_v = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float code = rintf(sqrtf(fabsf(m[i]) * mi) * 127.0f);
-            mc[i] = (int8_t)(int)(m[i] < 0.0f ? -code : code);
-            const float ratio = fabsf(v[i]) * vi, root = rintf(sqrtf(sqrtf(ratio)) * 255.0f);
-            vc[i] = (uint8_t)(int)(ratio > 0.0f ? fmaxf(root, 1.0f) : root);
+            for (int i = 0; i < 4; ++i) {
+                most_m = fmaxf(most_m, fabsf(m[n][i]));
+                most_v = fmaxf(most_v, fabsf(v[n][i]));
+            }
+            most_m = __uint_as_float(wave_max_u32_dpp(__float_as_uint(most_m)));
+            most_v = __uint_as_float(wave_max_u32_dpp(__float_as_uint(most_v)));
+            most_m = most_m < 1.175494351e-38f ? 0.0f : most_m;
+            most_v = most_v < 1.175494351e-38f ? 0.0f : most_v;
+            const float mi = most_m > 0.0f ? 1.0f / most_m : 0.0f, vi = most_v > 0.0f ? 1.0f / most_v : 0.0f;
+            // Codes are defined by rounded roots.  The hardware's are one unit off at most, which moves 127 sqrt(x) by less than 5e-5 and
+            // 255 sqrt(sqrt(x)) by less than 1e-4: only values that close to halfway between two codes need the rounded ones
+            // (8 of 100 runs, against 16 instructions for each of three roots).
+            float ratio_m[4], ratio_v[4], code_m[4], code_v[4];
+            bool close = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                ratio_m[i] = fabsf(m[n][i]) * mi;
+                ratio_v[i] = fabsf(v[n][i]) * vi;
+                const float root_m = __builtin_amdgcn_sqrtf(ratio_m[i]) * 127.0f;
+                const float root_v = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(ratio_v[i])) * 255.0f;
+                code_m[i] = rintf(root_m);
+                code_v[i] = rintf(root_v);
+                close = close || fabsf(root_m - code_m[i]) > 0.5f - 5e-5f || fabsf(root_v - code_v[i]) > 0.5f - 1e-4f;
+            }
+            if (close) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    code_m[i] = rintf(sqrtf(ratio_m[i]) * 127.0f);
+                    code_v[i] = rintf(sqrtf(sqrtf(ratio_v[i])) * 255.0f);
+                }
+            }
+            int8_t mo[4];
+            uint8_t vo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                mo[i] = (int8_t)(int)copysignf(code_m[i], m[n][i]);
+                vo[i] = (uint8_t)(int)(ratio_v[i] > 0.0f ? fmaxf(code_v[i], 1.0f) : code_v[i]);
+            }
+            store_run((int8_t *)t.first + at, mo, valid[n]);
+            store_run((uint8_t *)t.second + at, vo, valid[n]);
+            if (valid[n] && (threadIdx.x & 63) == 0) {
+                t.first_scale[at / kBlock8] = most_m;
+                t.second_scale[at / kBlock8] = most_v;
+            }
+        } else {
+            store_run((float *)t.first + at, m[n], valid[n]);
+            store_run((float *)t.second + at, v[n], valid[n]);
         }
-        store_run((int8_t *)t.first + at, mc, valid);
-        store_run((uint8_t *)t.second + at, vc, valid);
-        if (valid && at % kBlock8 == 0) {
-            t.first_scale[block] = ms;
-            t.second_scale[block] = vs;
-        }
-    } else {
-        store_run((float *)t.first + at, m, valid);
-        store_run((float *)t.second + at, v, valid);
     }
 }
 
@@ -1022,22 +1041,31 @@ __global__ __launch_bounds__(256) void k_unpack(const AdamArgs g)
 {
     const uint32_t which = adam_tensor(g);
     const pink_hip_readout_tensor &t = g.tensor[which];
-    const uint64_t at = (uint64_t)(blockIdx.x - g.first_block[which]) * kAdamChunk + threadIdx.x * 8;
-    if (at >= t.size) return;
-    const uint32_t valid = (uint32_t)min((uint64_t)8, t.size - at);
-    int8_t mc[8];
-    uint8_t vc[8];
-    load_run(mc, (const int8_t *)t.first + at, valid);
-    load_run(vc, (const uint8_t *)t.second + at, valid);
-    const float ms = t.first_scale[at / kBlock8], vs = t.second_scale[at / kBlock8];
-    float m[8], v[8];
+    const uint64_t base = (uint64_t)(blockIdx.x - g.first_block[which]) * kAdamChunk + threadIdx.x * 4;
+    int8_t mc[kAdamRuns][4];
+    uint8_t vc[kAdamRuns][4];
+    float ms[kAdamRuns], vs[kAdamRuns];
+    uint32_t valid[kAdamRuns];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        m[i] = first_value(mc[i], ms);
-        v[i] = second_value(vc[i], vs);
+    for (uint32_t n = 0; n < kAdamRuns; ++n) {
+        const uint64_t at = base + n * 1024;
+        valid[n] = at >= t.size ? 0 : (uint32_t)min((uint64_t)4, t.size - at);
+        load_run(mc[n], (const int8_t *)t.first + at, valid[n]);
+        load_run(vc[n], (const uint8_t *)t.second + at, valid[n]);
+        ms[n] = valid[n] ? t.first_scale[at / kBlock8] : 0.0f;
+        vs[n] = valid[n] ? t.second_scale[at / kBlock8] : 0.0f;
     }
-    store_run(t.first_values + at, m, valid);
-    store_run(t.second_values + at, v, valid);
+#pragma unroll
+    for (uint32_t n = 0; n < kAdamRuns; ++n) {
+        float m[4], v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            m[i] = first_value(mc[n][i], ms[n]);
+            v[i] = second_value(vc[n][i], vs[n]);
+        }
+        store_run(t.first_values + base + n * 1024, m, valid[n]);
+        store_run(t.second_values + base + n * 1024, v, valid[n]);
+    }
 }
 
 // ---------------------------------------------------------------------------------
@@ -1095,7 +1123,7 @@ int grow(pink_hip_readout *r, size_t bytes)
 
 // What a forward call leaves for the backward one, and where.
 struct Saved {
-    size_t order, images, owner, place, offsets, tile_count, tiles, before, after, bytes;
+    size_t order, owner, place, offsets, tile_count, tiles, before, after, bytes;
     uint64_t stride;               // of before's and after's rows: whole 16-byte chunks
 };
 
@@ -1114,7 +1142,6 @@ Saved saved_layout(const pink_hip_readout *r, uint64_t images)
     };
     s.stride = (c.hidden + 16 / e - 1) / (16 / e) * (16 / e);
     s.order = take(slots * 4);
-    s.images = take(slots * 4);
     s.owner = take(slots * 4);
     s.place = take(slots * 4);
     s.offsets = take(((size_t)c.neurons + 1) * 4);
@@ -1138,7 +1165,7 @@ struct Work {
 Work work_layout(const pink_hip_readout *r, uint64_t images)
 {
     const pink_hip_readout_config &c = r->cfg;
-    const size_t slots = images * c.chosen, plan_blocks = (slots + plan_waves(c.neurons) * 64 * kPerWave - 1) / (plan_waves(c.neurons) * 64 * kPerWave);
+    const size_t slots = images * c.chosen, plan_blocks = slots / (plan_waves(c.neurons) * 64) + 1;
     Work w;
     size_t at = 0;
     const auto take = [&](size_t bytes) {
@@ -1254,17 +1281,15 @@ int plan(pink_hip_readout *r, const int32_t *neuron, uint32_t slots, char *saved
     g.neurons = c.neurons;
     g.tile_rows = tile_rows(r, slots);
     g.counts = (uint32_t *)(work + w.counts);
-    g.chosen = c.chosen;
     g.order = (uint32_t *)(saved + s.order);
-    g.images = (uint32_t *)(saved + s.images);
-    g.owner = (uint32_t *)(saved + s.owner);
+    g.owner = (int32_t *)(saved + s.owner);
     g.place = (int32_t *)(saved + s.place);
     g.offsets = (uint32_t *)(saved + s.offsets);
     g.tile_count = (uint32_t *)(saved + s.tile_count);
     g.tiles = (uint2 *)(saved + s.tiles);
-    const uint32_t waves = plan_waves(c.neurons), per_block = waves * 64 * kPerWave, blocks = (slots + per_block - 1) / per_block;
+    const uint32_t waves = plan_waves(c.neurons), per_block = waves * 64, blocks = (slots + per_block - 1) / per_block;
     const size_t lds = (size_t)waves * c.neurons * 4;
-    if (blocks == 1) {
+    if (blocks <= kPerWave<2>) {
         k_plan<2><<<1, waves * 64, lds, r->stream>>>(g);
         return launched(r, "k_plan");
     }
@@ -1320,7 +1345,6 @@ int experts(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stri
 
     ProductArgs g = {};
     g.order = (const uint32_t *)(saved + s.order);
-    g.images = (const uint32_t *)(saved + s.images);
     g.offsets = (const uint32_t *)(saved + s.offsets);
     g.tiles = (const uint2 *)(saved + s.tiles);
     g.tile_count = (const uint32_t *)(saved + s.tile_count);
@@ -1370,7 +1394,6 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
 
     ProductArgs g = {};
     g.order = (const uint32_t *)(saved + s.order);
-    g.images = (const uint32_t *)(saved + s.images);
     g.offsets = (const uint32_t *)(saved + s.offsets);
     g.tiles = (const uint2 *)(saved + s.tiles);
     g.tile_count = (const uint32_t *)(saved + s.tile_count);
@@ -1393,7 +1416,7 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
     }
     if (out.gates) {
         k_gate_gradients<E><<<(uint32_t)(((uint64_t)slots + 3) / 4), 256, 0, r->stream>>>(
-            g.partial, g.col_tiles, place, (const uint32_t *)(saved + s.owner), slots, c.chosen, (const E *)dy, dy_stride, c.outputs,
+            g.partial, g.col_tiles, place, (const int32_t *)(saved + s.owner), slots, c.chosen, (const E *)dy, dy_stride, c.outputs,
             (const E *)weights.second_bias, (E *)out.gates);
         TRY(launched(r, "k_gate_gradients"));
     }
