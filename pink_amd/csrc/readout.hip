@@ -690,10 +690,15 @@ __global__ __launch_bounds__(1024) void k_plan_offsets(const PlanArgs g, uint32_
     __shared__ unsigned long long shared[16];
     for (uint32_t n = threadIdx.x; n < g.neurons; n += blockDim.x) {
         uint32_t before = 0;
-        for (uint32_t b = 0; b < blocks; ++b) {
-            const uint32_t c = g.counts[(uint64_t)b * g.neurons + n];
-            g.counts[(uint64_t)b * g.neurons + n] = before;
-            before += c;
+        for (uint32_t b0 = 0; b0 < blocks; b0 += 16) {     // sixteen loads under way
+            uint32_t c[16];
+#pragma unroll
+            for (uint32_t b = 0; b < 16; ++b) c[b] = b0 + b < blocks ? g.counts[(uint64_t)(b0 + b) * g.neurons + n] : 0;
+#pragma unroll
+            for (uint32_t b = 0; b < 16; ++b) {
+                if (b0 + b < blocks) g.counts[(uint64_t)(b0 + b) * g.neurons + n] = before;
+                before += c[b];
+            }
         }
         totals[n] = before;
     }
@@ -1223,23 +1228,21 @@ RouteArgs route_args(const pink_hip_readout *r, const float *distances, uint32_t
 }
 
 // Rows of a product's tiles, by how many rows a neuron has on average: the weights are read once for each tile of rows, and a tile
-// that is mostly empty multiplies for nothing.
+// that is mostly empty multiplies for nothing.  bfloat16's largest tiles halve what a CU fetches for each product; measured with 640
+// rows a neuron, 1936 x 1024: 475 us in tiles of 256 x 256 against 550 in 128 x 128; with 320 rows, 512 x 1024: 84 against 95, and
+// 102 against 99 for 1024 x 512.  Float32's products are bound by the matrix cores at either.
 uint32_t tile_rows(const pink_hip_readout *r, uint64_t slots)
 {
     const uint64_t neurons = std::min<uint64_t>(r->cfg.neurons, slots);
-    return slots <= 24 * neurons ? 16 : slots <= 64 * neurons ? 64 : 128;
+    if (slots <= 24 * neurons) return 16;
+    if (slots <= 64 * neurons) return 64;
+    return slots >= 256 * neurons && r->cfg.element == PINK_HIP_ELEMENT_BFLOAT ? 256 : 128;
 }
 
-template <typename E, int OP, int PR, int QC, int PW, int QW, int M, int DEEP>
-int product_of_tile(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
+// Are the operands whole chunks at their alignment?  (`saved` and the workspace have both; what lies past a row's end there is
+// readable.)
+template <typename E, int OP> bool is_direct(const ProductArgs &g)
 {
-    constexpr bool grad = OP == kGradFirst || OP == kGradSecond;
-    g.col_tiles = grad && !g.out ? 1 : (g.cols + QC - 1) / QC;
-    g.row_tiles = grad ? (g.rows + PR - 1) / PR : 0;
-    const uint64_t tiles = grad ? (uint64_t)r->cfg.neurons * g.row_tiles : slots / PR + std::min<uint64_t>(r->cfg.neurons, slots);
-    const uint64_t blocks = tiles * g.col_tiles;
-    REFUSE(r, blocks > 0x7fffffffu, "too many images for one call");
-    // Whole chunks at their alignment?  (`saved` and the workspace have both; what lies past a row's end there is readable.)
     constexpr uint32_t per = 16 / sizeof(E);
     const auto whole = [](const void *at, uint64_t stride) { return ((uintptr_t)at & 15) == 0 && stride % per == 0; };
     bool direct = whole(g.p, g.p_stride) && whole(g.q, g.q_stride);
@@ -1249,26 +1252,52 @@ int product_of_tile(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
     if (OP == kBackInput) direct = direct && g.cols % per == 0;
     if (OP == kGradFirst) direct = direct && g.cols % per == 0;
     if (OP == kGradSecond) direct = direct && g.rows % per == 0;
-    if (direct) k_product<E, OP, PR, QC, PW, QW, M, DEEP, true><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
-    else k_product<E, OP, PR, QC, PW, QW, M, DEEP, false><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
+    return direct;
+}
+
+template <typename E, int OP, int PR, int QC, int PW, int QW, int M, int DEEP, bool DIRECT>
+int product_of_tile(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
+{
+    constexpr bool grad = OP == kGradFirst || OP == kGradSecond;
+    g.col_tiles = grad && !g.out ? 1 : (g.cols + QC - 1) / QC;
+    g.row_tiles = grad ? (g.rows + PR - 1) / PR : 0;
+    const uint64_t tiles = grad ? (uint64_t)r->cfg.neurons * g.row_tiles : slots / PR + std::min<uint64_t>(r->cfg.neurons, slots);
+    const uint64_t blocks = tiles * g.col_tiles;
+    REFUSE(r, blocks > 0x7fffffffu, "too many images for one call");
+    k_product<E, OP, PR, QC, PW, QW, M, DEEP, DIRECT><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
     return launched(r, "k_product");
 }
 
-template <typename E, int OP> int product(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
+template <typename E, int OP, bool DIRECT> int product_as(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
 {
+    constexpr bool half = sizeof(E) == 2;
     if constexpr (OP == kGradFirst || OP == kGradSecond) {
-        // Few rows a neuron: writing the gradients is what there is to do, and small tiles spread it.
-        if (slots <= 64 * (uint64_t)r->cfg.neurons) return product_of_tile<E, OP, 64, 64, 2, 2, 16, 1>(r, g, slots);
-        return product_of_tile<E, OP, 128, 128, 2, 2, 32, 1>(r, g, slots);
+        // Few rows a neuron: writing the gradients is what there is to do, and small tiles spread it.  Large tiles (590 against 640 us
+        // for 1024 x 1936 of 100 neurons) where there are enough of them to go round.
+        if (slots <= 64 * (uint64_t)r->cfg.neurons) return product_of_tile<E, OP, 64, 64, 2, 2, 16, 1, DIRECT>(r, g, slots);
+        if constexpr (half && DIRECT) {
+            const uint64_t tiles = (uint64_t)r->cfg.neurons * ((g.rows + 255) / 256) * ((g.cols + 255) / 256);
+            if (g.out && g.rows >= 256 && tiles >= 1024) return product_of_tile<E, OP, 256, 256, 2, 4, 32, 1, DIRECT>(r, g, slots);
+        }
+        return product_of_tile<E, OP, 128, 128, 2, 2, 32, 1, DIRECT>(r, g, slots);
     } else {
         // Few rows a neuron: reading the weights is what there is to do; a stage takes 512 bytes of a row so that enough of it is
         // under way.
         switch (tile_rows(r, slots)) {
-        case 16: return product_of_tile<E, OP, 16, 32, 1, 2, 16, 4>(r, g, slots);
-        case 64: return product_of_tile<E, OP, 64, 64, 2, 2, 32, 2>(r, g, slots);
-        default: return product_of_tile<E, OP, 128, 128, 2, 2, 32, 1>(r, g, slots);
+        case 16: return product_of_tile<E, OP, 16, 32, 1, 2, 16, 4, DIRECT>(r, g, slots);
+        case 64: return product_of_tile<E, OP, 64, 64, 2, 2, 32, 2, DIRECT>(r, g, slots);
+        case 256:                                          // (what passes through registers leaves fewer for sums)
+            if constexpr (half && DIRECT) return product_of_tile<E, OP, 256, 256, 2, 4, 32, 1, DIRECT>(r, g, slots);
+            else if constexpr (half) return product_of_tile<E, OP, 256, 128, 4, 2, 32, 1, DIRECT>(r, g, slots);
+            [[fallthrough]];
+        default: return product_of_tile<E, OP, 128, 128, 2, 2, 32, 1, DIRECT>(r, g, slots);
         }
     }
+}
+
+template <typename E, int OP> int product(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
+{
+    return is_direct<E, OP>(g) ? product_as<E, OP, true>(r, g, slots) : product_as<E, OP, false>(r, g, slots);
 }
 
 int plan(pink_hip_readout *r, const int32_t *neuron, uint32_t slots, char *saved, const Saved &s, const Work &w)

@@ -464,6 +464,19 @@ MODELS = [  # images, neurons, chosen, features, hidden, outputs, activation, bi
     (5, 5, 2, 33, 17, 9, "gelu", True, True, none_at_all, 2),
     (333, 9, 4, 96, 40, 24, "gelu", True, True, None, 4),
     (17, 300, 3, 72, 144, 200, "silu", True, False, None, 0),
+    # tiles of every size, each with whole chunks and without: rows a neuron 12, 40, 100, 350; more rows than are looked up at a time
+    (60, 10, 2, 64, 40, 48, "silu", True, True, None, 0),
+    (60, 10, 2, 61, 41, 47, "silu", True, True, None, 0),
+    (200, 5, 1, 264, 72, 136, "silu", True, False, None, 0),
+    (200, 5, 1, 263, 71, 135, "silu", True, False, None, 1),
+    (300, 6, 2, 520, 136, 72, "silu", False, False, None, 0),
+    (300, 6, 2, 519, 137, 73, "silu", False, False, None, 0),
+    (700, 2, 1, 136, 264, 520, "silu", True, True, None, 0),
+    (700, 2, 1, 135, 263, 519, "silu", True, True, None, 3),
+    (5000, 1, 1, 40, 24, 16, "gelu", True, False, None, 0),
+    (4300, 2, 2, 39, 23, 17, "relu", True, False, None, 0),
+    # so many neurons that gradients of weights take the largest tiles
+    (8400, 256, 2, 264, 264, 16, "silu", True, False, None, 0),
 ]
 
 
