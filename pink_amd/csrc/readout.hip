@@ -1272,6 +1272,8 @@ template <typename E, int OP, bool DIRECT> int product_as(pink_hip_readout *r, P
 {
     constexpr bool half = sizeof(E) == 2;
     if constexpr (OP == kGradFirst || OP == kGradSecond) {
+        // Matrices of few rows (the second layer of a handful of outputs): tiles of as few.
+        if (g.rows <= 32) return product_of_tile<E, OP, 32, 128, 1, 4, 32, 1, DIRECT>(r, g, slots);
         // Few rows a neuron: writing the gradients is what there is to do, and small tiles spread it.  Large tiles (590 against 640 us
         // for 1024 x 1936 of 100 neurons) where there are enough of them to go round.
         if (slots <= 64 * (uint64_t)r->cfg.neurons) return product_of_tile<E, OP, 64, 64, 2, 2, 16, 1, DIRECT>(r, g, slots);
@@ -1283,7 +1285,13 @@ template <typename E, int OP, bool DIRECT> int product_as(pink_hip_readout *r, P
     } else {
         // Few rows a neuron: reading the weights is what there is to do; a stage takes 512 bytes of a row so that enough of it is
         // under way.
-        switch (tile_rows(r, slots)) {
+        const uint32_t rows = tile_rows(r, slots);
+        if (rows > 16 && g.cols <= 32) {                   // results of few columns: tiles of as few
+            if (rows == 64) return product_of_tile<E, OP, 64, 32, 2, 1, 32, 2, DIRECT>(r, g, slots);
+            if (rows == 128) return product_of_tile<E, OP, 128, 32, 4, 1, 32, 1, DIRECT>(r, g, slots);
+            return product_of_tile<E, OP, 256, 32, 4, 1, 32, 1, DIRECT>(r, g, slots);
+        }
+        switch (rows) {
         case 16: return product_of_tile<E, OP, 16, 32, 1, 2, 16, 4, DIRECT>(r, g, slots);
         case 64: return product_of_tile<E, OP, 64, 64, 2, 2, 32, 2, DIRECT>(r, g, slots);
         case 256:                                          // (what passes through registers leaves fewer for sums)
@@ -1438,6 +1446,7 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
         g.depth = c.outputs;
         g.cols = c.hidden;
         g.before = saved + s.before;
+        g.after = saved + s.after;
         g.out = dbefore;
         g.out_stride = s.stride;
         g.partial = (float *)(work + w.partial);

@@ -475,6 +475,13 @@ MODELS = [  # images, neurons, chosen, features, hidden, outputs, activation, bi
     (700, 2, 1, 135, 263, 519, "silu", True, True, None, 3),
     (5000, 1, 1, 40, 24, 16, "gelu", True, False, None, 0),
     (4300, 2, 2, 39, 23, 17, "relu", True, False, None, 0),
+    # few hidden values or outputs: narrow tiles
+    (200, 5, 1, 264, 16, 8, "gelu", True, False, None, 0),
+    (200, 5, 1, 263, 17, 3, "gelu", True, True, None, 1),
+    (300, 6, 2, 136, 24, 32, "silu", True, False, None, 0),
+    (300, 6, 2, 137, 15, 10, "silu", True, False, None, 0),
+    (700, 2, 1, 136, 32, 16, "silu", True, True, None, 0),
+    (700, 2, 1, 135, 31, 1, "silu", True, True, None, 0),
     # so many neurons that gradients of weights take the largest tiles
     (8400, 256, 2, 264, 264, 16, "silu", True, False, None, 0),
 ]
