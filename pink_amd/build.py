@@ -44,11 +44,18 @@ def build(verbose=False, extra=()):
         flags = obj_flags + (SYM_FLAGS if src in (SYM_SOURCE, READOUT_SOURCE) else [])
         cmds.append([hipcc] + flags + list(extra) + ["-c", src, "-o", obj])
         objects.append(obj)
-    cmds.append([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC"] + objects + ["-o", OUT])
-    for cmd in cmds:
+    running = []
+    for cmd in cmds:                                       # side by side: the read-out's products take over a minute
         if verbose:
             print(" ".join(cmd), flush=True)
-        subprocess.check_call(cmd)
+        running.append((cmd, subprocess.Popen(cmd)))
+    for cmd, process in running:
+        if process.wait() != 0:
+            raise subprocess.CalledProcessError(process.returncode, cmd)
+    cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC"] + objects + ["-o", OUT]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
     return OUT
 
 

@@ -817,3 +817,20 @@ def test_adamw_at_addresses_of_single_elements(gpu):
             assert np.array_equal(np.roll(all_, -skip)[n:], value[n:])         # nothing outside is touched
             got.append(all_[skip:skip + n])
     assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+
+
+# ------------------------------------------------------------------------------------------------------- all together
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("options", [[], ["--state-bits", "8", "--chosen", "3"]])
+def test_read_out_of_a_small_map_learns(options):
+    # in a process of its own: PyTorch has to come before the library
+    import os
+    import re
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-u", "-m", "pink_amd.readout", "--steps", "200"] + options, cwd=root, capture_output=True, text=True, timeout=100)
+    assert run.returncode == 0, run.stderr[-2000:]
+    error, alone = map(float, re.search(r"new sources: mean squared error ([\d.]+) \(of the mean alone: ([\d.]+)\)", run.stdout).groups())
+    assert error < 0.25 * alone, run.stdout
