@@ -29,25 +29,38 @@ constexpr uint32_t kBlock8 = 256;                          // codes that share a
 
 thread_local char g_readout_error[320];
 
+// Sums and maxima over a wave by DPP, within rows of sixteen and across them into lane 63: no LDS round trips.  The order is fixed.
+#define PINK_DPP_ALL(op)                                       \
+    op(0xb1, 0xf);      /* quad_perm [1, 0, 3, 2] */           \
+    op(0x4e, 0xf);      /* quad_perm [2, 3, 0, 1] */           \
+    op(0x141, 0xf);     /* row_half_mirror */                  \
+    op(0x140, 0xf);     /* row_mirror */                       \
+    op(0x142, 0xa);     /* row_bcast:15 into rows 1 and 3 */   \
+    op(0x143, 0xc)      /* row_bcast:31 into rows 2 and 3 */
+
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
 {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, 64));
-    return v;
+#define PINK_DPP_MAX(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false))
+    PINK_DPP_ALL(PINK_DPP_MAX);
+#undef PINK_DPP_MAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 __device__ __forceinline__ float wave_sum(float v)
 {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+#define PINK_DPP_ADD(ctrl, rows) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, rows, 0xf, false))
+    PINK_DPP_ALL(PINK_DPP_ADD);
+#undef PINK_DPP_ADD
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 __device__ __forceinline__ float wave_max(float v)
 {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    return v;
+    constexpr int kLeast = (int)0xff800000;                // minus infinity, for rows that a step leaves alone
+#define PINK_DPP_MAX(ctrl, rows) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(kLeast, __float_as_int(v), ctrl, rows, 0xf, false)))
+    PINK_DPP_ALL(PINK_DPP_MAX);
+#undef PINK_DPP_MAX
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // ---------------------------------------------------------------------------------
@@ -203,21 +216,7 @@ __global__ __launch_bounds__(256) void k_route_block(const RouteArgs g)
     }
 }
 
-// The largest of the wave, by DPP within rows of sixteen and across them into lane 63.
-__device__ __forceinline__ uint32_t wave_max_u32_dpp(uint32_t v)
-{
-#define PINK_DPP_MAX(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false))
-    PINK_DPP_MAX(0xb1, 0xf);      // quad_perm [1, 0, 3, 2]
-    PINK_DPP_MAX(0x4e, 0xf);      // quad_perm [2, 3, 0, 1]
-    PINK_DPP_MAX(0x141, 0xf);     // row_half_mirror
-    PINK_DPP_MAX(0x140, 0xf);     // row_mirror
-    PINK_DPP_MAX(0x142, 0xa);     // row_bcast:15 into rows 1 and 3
-    PINK_DPP_MAX(0x143, 0xc);     // row_bcast:31 into rows 2 and 3
-#undef PINK_DPP_MAX
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-}
-
-// Sums of 64 neurons' keys per register: what a wave holds of an image, candidate 64 j + lane in key[j].
+// Neurons' keys in registers: what a wave holds of an image, candidate 64 j + lane in key[j].
 template <int J> struct Candidates {
     static constexpr int kSet = J <= 8 ? J : J % 8 ? 4 : 8, kSets = J / kSet;
     static_assert(J % kSet == 0, "whole sets");
@@ -260,12 +259,12 @@ template <int J> struct Candidates {
                 k = best[b];
                 w = where[b];
             }
-        const uint32_t most = wave_max_u32_dpp(k);
+        const uint32_t most = wave_max_u32(k);
         if (most == 0) return -1;
         const unsigned long long holders = __ballot(k == most);
         uint32_t c = w * 64 + lane;
         if (__popcll(holders) == 1) c = (uint32_t)__builtin_amdgcn_readlane((int)c, __ffsll(holders) - 1);
-        else c = ~wave_max_u32_dpp(k == most ? ~c : 0);
+        else c = ~wave_max_u32(k == most ? ~c : 0);
         remove<0>(c / 64, c % 64, lane);
         return (int)c;
     }
@@ -347,7 +346,7 @@ template <int J, int C, bool FULL> __global__ __launch_bounds__(256) void k_rout
         }
         unsigned long long all = 0;                        // the kept groups, taken one by one
         for (uint32_t k = 0; k < g.groups_kept; ++k) {
-            const uint32_t most = wave_max_u32_dpp(score);
+            const uint32_t most = wave_max_u32(score);
             if (most == 0) break;
             const unsigned long long one = __ballot(score == most) & -__ballot(score == most);
             all |= one;
@@ -602,7 +601,7 @@ __device__ __forceinline__ void plan_offsets(const PlanArgs &g, const Count &cou
     }
 }
 
-// STAGE 0: count only; 1: place rows, from counts' prefixes; 2: all in one block.
+// STAGE 0: count only; 1: place rows, from counts' prefixes; 2: all in one block, of which the first `waves` have slots.
 template <int STAGE> constexpr uint32_t kPerWave = STAGE == 2 ? 4 : 1;
 
 template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanArgs g)
@@ -610,7 +609,7 @@ template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanAr
     constexpr uint32_t PER = kPerWave<STAGE>;
     extern __shared__ __align__(16) uint32_t hist[];       // waves x N
     __shared__ unsigned long long shared[16];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = STAGE == 2 ? (g.slots + 64 * PER - 1) / (64 * PER) : blockDim.x >> 6;
     const uint64_t first = ((uint64_t)blockIdx.x * waves + wave) * 64 * PER;
     uint32_t rank[PER], id[PER];
 #pragma unroll
@@ -620,7 +619,7 @@ template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanAr
     }
     for (uint32_t i = threadIdx.x; i < waves * g.neurons; i += blockDim.x) hist[i] = 0;
     __syncthreads();
-    volatile uint32_t *const mine = hist + wave * g.neurons;
+    volatile uint32_t *const mine = hist + min(wave, waves - 1) * g.neurons;         // (a wave without slots touches nothing)
 #pragma unroll
     for (uint32_t i = 0; i < PER; ++i) {
         const bool valid = id[i] < g.neurons;
@@ -675,7 +674,7 @@ template <int STAGE> __global__ __launch_bounds__(1024) void k_plan(const PlanAr
         if (slot >= g.slots) continue;
         int32_t row = -1;
         if (id[i] < g.neurons) {
-            row = (int32_t)(hist[wave * g.neurons + id[i]] + rank[i]);
+            row = (int32_t)(mine[id[i]] + rank[i]);
             if (STAGE == 1) row += (int32_t)(g.offsets[id[i]] + g.counts[(uint64_t)blockIdx.x * g.neurons + id[i]]);
             g.order[row] = (uint32_t)slot;
         }
@@ -995,8 +994,8 @@ template <bool CODES> __global__ __launch_bounds__(256) void k_adamw(const AdamA
                 most_m = fmaxf(most_m, fabsf(m[n][i]));
                 most_v = fmaxf(most_v, fabsf(v[n][i]));
             }
-            most_m = __uint_as_float(wave_max_u32_dpp(__float_as_uint(most_m)));
-            most_v = __uint_as_float(wave_max_u32_dpp(__float_as_uint(most_v)));
+            most_m = __uint_as_float(wave_max_u32(__float_as_uint(most_m)));
+            most_v = __uint_as_float(wave_max_u32(__float_as_uint(most_v)));
             most_m = most_m < 1.175494351e-38f ? 0.0f : most_m;
             most_v = most_v < 1.175494351e-38f ? 0.0f : most_v;
             const float mi = most_m > 0.0f ? 1.0f / most_m : 0.0f, vi = most_v > 0.0f ? 1.0f / most_v : 0.0f;
@@ -1263,8 +1262,10 @@ int product_of_tile(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
     g.row_tiles = grad ? (g.rows + PR - 1) / PR : 0;
     const uint64_t tiles = grad ? (uint64_t)r->cfg.neurons * g.row_tiles : slots / PR + std::min<uint64_t>(r->cfg.neurons, slots);
     const uint64_t blocks = tiles * g.col_tiles;
-    REFUSE(r, blocks > 0x7fffffffu, "too many images for one call");
-    k_product<E, OP, PR, QC, PW, QW, M, DEEP, DIRECT><<<(uint32_t)blocks, 64 * PW * QW, 0, r->stream>>>(g);
+    REFUSE(r, blocks > 0x7fffffffu - kFillBlocks, "too many images for one call");
+    g.slots = (uint32_t)slots;
+    const uint32_t more = (OP == kAnswer || OP == kBackInput) && g.place ? kFillBlocks : 0;
+    k_product<E, OP, PR, QC, PW, QW, M, DEEP, DIRECT><<<(uint32_t)blocks + more, 64 * PW * QW, 0, r->stream>>>(g);
     return launched(r, "k_product");
 }
 
@@ -1327,7 +1328,9 @@ int plan(pink_hip_readout *r, const int32_t *neuron, uint32_t slots, char *saved
     const uint32_t waves = plan_waves(c.neurons), per_block = waves * 64, blocks = (slots + per_block - 1) / per_block;
     const size_t lds = (size_t)waves * c.neurons * 4;
     if (blocks <= kPerWave<2>) {
-        k_plan<2><<<1, waves * 64, lds, r->stream>>>(g);
+        // as many waves as there are slots for, or a thread for each neuron
+        const uint32_t with_slots = (slots + 64 * kPerWave<2> - 1) / (64 * kPerWave<2>), all = std::min(16u, std::max(with_slots, (c.neurons + 63) / 64));
+        k_plan<2><<<1, all * 64, (size_t)with_slots * c.neurons * 4, r->stream>>>(g);
         return launched(r, "k_plan");
     }
     k_plan<0><<<blocks, waves * 64, lds, r->stream>>>(g);
@@ -1408,6 +1411,14 @@ int experts(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stri
     g.depth = c.hidden;
     g.cols = c.outputs;
     g.bias = weights.second_bias;
+    if (c.chosen == 1) {
+        g.place = (const int32_t *)(saved + s.place);
+        g.residual = residual;
+        g.residual_stride = residual_stride;
+        g.out = y;
+        g.out_stride = y_stride;
+        return product<E, kAnswer>(r, g, slots);
+    }
     g.out = work + w.rows;
     g.out_stride = whole_rows(c.outputs);
     TRY((product<E, kAnswer>(r, g, slots)));
@@ -1466,10 +1477,17 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
         g.q_matrix = (uint64_t)c.hidden * c.features;
         g.depth = c.hidden;
         g.cols = c.features;
-        g.out = work + w.rows;
-        g.out_stride = whole_rows(c.features);
-        TRY((product<E, kBackInput>(r, g, slots)));
-        TRY(combine<E>(r, (const float *)(work + w.rows), place, images, c.features, nullptr, 0, out.features, dx_stride));
+        if (c.chosen == 1) {
+            g.place = place;
+            g.out = out.features;
+            g.out_stride = dx_stride;
+            TRY((product<E, kBackInput>(r, g, slots)));
+        } else {
+            g.out = work + w.rows;
+            g.out_stride = whole_rows(c.features);
+            TRY((product<E, kBackInput>(r, g, slots)));
+            TRY(combine<E>(r, (const float *)(work + w.rows), place, images, c.features, nullptr, 0, out.features, dx_stride));
+        }
     }
     if (out.first || out.first_bias) {
         g.p = dbefore;
