@@ -595,6 +595,42 @@ def test_experts_adds_to_its_residual_in_place(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("t, h, f", [(20, 33, 64), (90, 33, 128), (300, 42, 256), (700, 9, 136)])
+def test_experts_read_nothing_that_they_did_not_write(gpu, t, h, f, bf16):
+    """Workspace and saved rows are padded; what lies there, NaN from a larger call before, takes part in nothing."""
+    rng = np.random.default_rng(t)
+    element, n, k, o = Element(bf16), 2, 1, 16
+    stored, value, neuron, gates = experts_inputs(rng, element, t, n, k, f, h, o)
+    dy_stored, dy = element.store(rng.standard_normal((t, o)))
+    want = experts_reference(value, element, "silu", neuron, gates, dy)
+    nan = 0x7fc0 if bf16 else np.nan
+    names = dict(dx=(t, f), dgates=(t, k), dw1=(n, h, f), db1=(n, h), dw2=(n, o, h), db2=(n, o))
+    with capi.Readout(n, k, f, h, o, activation=capi.ACT_SILU, element=element.id) as ro, \
+            capi.Readout(n, 2, f, h, o, activation=capi.ACT_SILU, element=element.id) as before:
+        p = {i: gpu.up(v) for i, v in stored.items()}
+        weights = [p[i] for i in ("w1", "b1", "w2", "b2")]
+        ro.reserve(8 * t)
+        big = 8 * t                                        # two slots' rows of NaN each, wherever this handle puts them
+        for handle, c in ((ro, 1), (before, 2)):
+            where = gpu.up(np.tile(np.arange(n, dtype=np.int32), big * c)[:big * c]), gpu.up(np.ones(big * c, np.float32))
+            x_nan, dy_nan = gpu.up(np.full((big, f), nan, element.dtype)), gpu.up(np.full((big, o), nan, element.dtype))
+            junk = [gpu.new(s, element.dtype) for s in ((big, f), (big, c), (n, h, f), (n, h), (n, o, h), (n, o))]
+            keep = gpu.new(handle.saved_bytes(big), np.int8)
+            handle.experts(x_nan, big, *where, weights, gpu.new((big, o), element.dtype), dev_saved=keep)
+            handle.experts(x_nan, big, *where, weights, gpu.new((big, o), element.dtype))
+            handle.experts_backward(x_nan, big, where[1], weights, keep, dy_nan, junk)
+        saved = gpu.up(np.full(ro.saved_bytes(t) // 2, 0x7fff, np.uint16))     # NaN in either type
+        y, grads, where = gpu.new((t, o), element.dtype), {i: gpu.new(s, element.dtype) for i, s in names.items()}, (gpu.up(neuron), gpu.up(gates))
+        ro.experts(p["x"], t, *where, weights, y, dev_saved=saved)
+        ro.experts_backward(p["x"], t, where[1], weights, saved, gpu.up(dy_stored), [grads[i] for i in names])
+        ro.synchronize()
+        assert_within(element.values(gpu.down(y, (t, o), element.dtype)), *want["y"], "y")
+        for i, s in names.items():
+            assert_within(element.values(gpu.down(grads[i], s, element.dtype)), *want[i], i)
+
+
+@pytest.mark.gpu
 def test_no_images(gpu):
     with capi.Readout(5, 2, 8, 4, 3) as ro:
         weights = [gpu.new(60, np.float32)] * 4
