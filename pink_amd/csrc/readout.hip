@@ -1260,7 +1260,7 @@ template <typename E, int OP> bool is_direct(const ProductArgs &g)
     if (OP == kHidden || OP == kAnswer || OP == kBackHidden || OP == kBackInput) direct = direct && g.q_matrix % per == 0;
     if (OP == kHidden || OP == kAnswer) direct = direct && g.depth % per == 0;
     if (OP == kBackHidden) direct = direct && g.depth % per == 0 && g.cols % per == 0;
-    if (OP == kBackInput) direct = direct && g.depth % per == 0 && g.cols % per == 0;      // (no product with what pads a row)
+    if (OP == kBackInput) direct = direct && g.cols % per == 0;          // (its rows are padded with zeros)
     if (OP == kGradFirst) direct = direct && g.cols % per == 0;
     if (OP == kGradSecond) direct = direct && g.rows % per == 0;
     return direct;
@@ -1305,7 +1305,9 @@ template <typename E, int OP, bool DIRECT> int product_as(pink_hip_readout *r, P
             return product_of_tile<E, OP, 256, 32, 4, 1, 32, 1, DIRECT>(r, g, slots);
         }
         switch (rows) {
-        case 16: return product_of_tile<E, OP, 16, 32, 1, 2, 16, 4, DIRECT>(r, g, slots);
+        case 16:                                           // (short sums, as the backward pass has: more blocks at once instead)
+            if constexpr (OP == kBackHidden || OP == kBackInput) return product_of_tile<E, OP, 16, 64, 1, 4, 16, 2, DIRECT>(r, g, slots);
+            else return product_of_tile<E, OP, 16, 32, 1, 2, 16, 4, DIRECT>(r, g, slots);
         case 64: return product_of_tile<E, OP, 64, 64, 2, 2, 32, 2, DIRECT>(r, g, slots);
         case 256:                                          // (what passes through registers leaves fewer for sums)
             if constexpr (half && DIRECT) return product_of_tile<E, OP, 256, 256, 2, 4, 32, 1, DIRECT>(r, g, slots);
