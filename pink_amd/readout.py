@@ -17,6 +17,7 @@ module first does that).
 trains a small map on synthetic sources and a read-out of their size and axis ratio.
 """
 import argparse
+import functools
 import math
 
 import numpy as np
@@ -35,9 +36,22 @@ def _check_one_runtime():
         raise pink.exception(-4, "import torch (or this module) before the library is first used: two HIP runtimes are loaded, " + ", ".join(sorted(runtimes)))
 
 
+def _on_its_device(call):
+    @functools.wraps(call)
+    def run(self, *args, **options):
+        with torch.cuda.device(self.device):
+            self._follow_stream()
+            return call(self, *args, **options)
+    return run
+
+
 class MapReadout:
     """Two-layer models of a map's neurons on its heatmap; `chosen` of them answer for an image, weighted by the softmax of
-    sharpness * (radius - distance)."""
+    sharpness * (radius - distance).
+
+    It lives on the device that is current when it is made.  Calls run on that device's stream that is current when they are made, and
+    what they return is that stream's; a call on another stream than the last one's waits for that one first, so a stream that
+    was used has to exist until then."""
 
     def __init__(self, som, outputs, hidden=32, chosen=2, activation=capi.ACT_GELU, learning_rate=3e-3, weight_decay=1e-3, balance_rate=1e-3,
                  state_bits=32, number_of_rotations=360, use_flip=True, euclidean_distance_dim=None,
@@ -50,19 +64,24 @@ class MapReadout:
         _check_one_runtime()
         capi.Readout.check(n, chosen, n, hidden, outputs, activation=activation)
         torch.cuda.init()
-        self.readout = capi.Readout(n, chosen, n, hidden, outputs, activation=activation)
-        self.readout.set_stream(torch.cuda.current_stream().cuda_stream)
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self.readout = capi.Readout(n, chosen, n, hidden, outputs, activation=activation, device=self.device.index)
+        self._stream = None
+        self._follow_stream()
         self._mapper = None
-        gen = torch.Generator(device="cuda").manual_seed(seed)
+        gen = torch.Generator(device=self.device).manual_seed(seed)
+
+        def zeros(shape, dtype=torch.float32):
+            return torch.zeros(shape, dtype=dtype, device=self.device)
 
         def randn(*shape, scale):
-            return torch.randn(shape, device="cuda", generator=gen) * scale
+            return torch.randn(shape, device=self.device, generator=gen) * scale
 
-        self.parameters = {"sharpness": torch.ones(n, device="cuda"), "radius": torch.zeros(n, device="cuda"),
-                           "first": randn(n, hidden, n, scale=1 / math.sqrt(n)), "first_bias": torch.zeros((n, hidden), device="cuda"),
-                           "second": randn(n, outputs, hidden, scale=1 / math.sqrt(hidden)), "second_bias": torch.zeros((n, outputs), device="cuda")}
+        self.parameters = {"sharpness": zeros(n) + 1, "radius": zeros(n),
+                           "first": randn(n, hidden, n, scale=1 / math.sqrt(n)), "first_bias": zeros((n, hidden)),
+                           "second": randn(n, outputs, hidden, scale=1 / math.sqrt(hidden)), "second_bias": zeros((n, outputs))}
         self.gradients = {k: torch.zeros_like(v) for k, v in self.parameters.items()}
-        state, blocks = (lambda v, t: torch.zeros(v.numel(), dtype=t, device="cuda")), lambda v: torch.zeros(-(-v.numel() // 256), device="cuda")
+        state, blocks = (lambda v, t: zeros(v.numel(), t)), lambda v: zeros(-(-v.numel() // 256))
         if state_bits == 8:
             self.states = {k: dict(first=state(v, torch.int8), second=state(v, torch.uint8), first_scale=blocks(v), second_scale=blocks(v))
                            for k, v in self.parameters.items()}
@@ -71,19 +90,28 @@ class MapReadout:
         self._tensors = self.readout.tensors([
             dict(value=v.data_ptr(), gradient=self.gradients[k].data_ptr(), size=v.numel(), decay=weight_decay if k in ("first", "second") else 0.0,
                  **{s: x.data_ptr() for s, x in self.states[k].items()}) for k, v in self.parameters.items()])
-        self.bias = torch.zeros(n, device="cuda")          # for an even load; takes part in the choice of neurons only
+        self.bias = zeros(n)                               # for an even load; takes part in the choice of neurons only
         self.steps, self._level = 0, None
 
+    def _follow_stream(self):
+        """What was queued for the read-out so far is complete, and the handle works on the caller's current stream."""
+        stream = torch.cuda.current_stream(self.device)
+        if stream != self._stream:
+            self.readout.set_stream(stream.cuda_stream)    # waits for the stream that it leaves, PyTorch's work there too
+            self._stream = stream
+
+    @_on_its_device
     def distances(self, images):
         """The images' heatmaps, (images, neurons) on the GPU.  Images: a float32 array or CUDA tensor (images[, channels], edge, edge)."""
-        images = torch.as_tensor(images, dtype=torch.float32, device="cuda").contiguous()
+        images = torch.as_tensor(images, dtype=torch.float32, device=self.device).contiguous()
         channels, edge = self._geometry(images)
         if self._mapper is None or self._mapper.I != edge:
             rotations, flip, region = self._map_args
             _, neuron_dim = pink._image_geometry(self.som.neuron_shape, self.som.neuron_layout, "neuron")
-            self._mapper = capi.Context(self.som.number_of_neurons, channels, edge, neuron_dim, rotations, flip, region, ed_type=self._map_type)
+            self._mapper = capi.Context(self.som.number_of_neurons, channels, edge, neuron_dim, rotations, flip, region, ed_type=self._map_type,
+                                        device=self.device.index)
             self._mapper.set_som(self.som._rows())
-        heat = torch.empty((images.shape[0], self.som.number_of_neurons), device="cuda")
+        heat = torch.empty((images.shape[0], self.som.number_of_neurons), device=self.device)
         torch.cuda.synchronize()                           # the mapper runs on a stream of its own
         self._mapper.map_device(images.data_ptr(), images.shape[0], heat.data_ptr())
         self._mapper.synchronize()
@@ -109,24 +137,26 @@ class MapReadout:
     def _forward(self, heat, keep):
         r, p, t = self.readout, self.parameters, heat.shape[0]
         x = self._features(heat)
-        neuron = torch.empty((t, self.chosen), dtype=torch.int32, device="cuda")
-        gates, y = torch.empty((t, self.chosen), device="cuda"), torch.empty((t, self.outputs), device="cuda")
-        saved = torch.empty(r.saved_bytes(t), dtype=torch.uint8, device="cuda") if keep else None
+        neuron = torch.empty((t, self.chosen), dtype=torch.int32, device=self.device)
+        gates, y = torch.empty((t, self.chosen), device=self.device), torch.empty((t, self.outputs), device=self.device)
+        saved = torch.empty(r.saved_bytes(t), dtype=torch.uint8, device=self.device) if keep else None
         r.route(heat.data_ptr(), t, p["sharpness"].data_ptr(), p["radius"].data_ptr(), self.bias.data_ptr(), neuron.data_ptr(), gates.data_ptr())
         r.experts(x.data_ptr(), t, neuron.data_ptr(), gates.data_ptr(), self._weights(), y.data_ptr(), dev_saved=saved.data_ptr() if keep else None)
         return x, neuron, gates, y, saved
 
+    @_on_its_device
     def __call__(self, images):
         """Answers, (images, outputs) on the GPU."""
         return self._forward(self.distances(images), False)[3]
 
+    @_on_its_device
     def step(self, images, targets):
         """One step of AdamW on the mean squared error of a batch; returns the error before the step, on the GPU."""
         r, p, g = self.readout, self.parameters, self.gradients
         heat = self.distances(images)
         t = heat.shape[0]
         x, neuron, gates, y, saved = self._forward(heat, True)
-        off = y - torch.as_tensor(targets, dtype=torch.float32, device="cuda").reshape(t, self.outputs)
+        off = y - torch.as_tensor(targets, dtype=torch.float32, device=self.device).reshape(t, self.outputs)
         dy, dgates = off * (2.0 / off.numel()), torch.empty_like(gates)
         r.experts_backward(x.data_ptr(), t, gates.data_ptr(), self._weights(), saved.data_ptr(), dy.data_ptr(),
                            [None, dgates.data_ptr()] + [g[k].data_ptr() for k in ("first", "first_bias", "second", "second_bias")])

@@ -1,0 +1,126 @@
+"""MapReadout, the read-out of a map from images to answers: on which stream it works, and what it keeps of its map and its first images."""
+import contextlib
+import os
+import subprocess
+import sys
+import textwrap
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+# ------------------------------------------------------------------------------------------------------- without a GPU
+
+class Recorder:
+    """In the place of capi.Readout and of PyTorch's streams: what was called on which stream."""
+
+    def __init__(self):
+        self.calls, self.at, self.current = [], "own", "first"
+
+    def set_stream(self, stream):
+        self.at = stream
+
+    def saved_bytes(self, images):
+        return 16
+
+    def __getattr__(self, name):
+        if name.startswith("_"):
+            raise AttributeError(name)
+        return lambda *args, **options: self.calls.append((name, self.at, self.current))
+
+
+class Stream:
+    def __init__(self, name):
+        self.cuda_stream = name
+
+    def __eq__(self, other):
+        return isinstance(other, Stream) and other.cuda_stream == self.cuda_stream
+
+
+@pytest.fixture
+def made(monkeypatch):
+    """A MapReadout on the CPU, whose handle only records."""
+    torch = pytest.importorskip("torch")
+    from pink_amd import capi, pink, readout
+    import numpy as np
+    recorder = Recorder()
+    monkeypatch.setattr(capi, "Readout", type("Readout", (), dict(check=staticmethod(lambda *a, **o: None), __new__=lambda cls, *a, **o: recorder)))
+    recorder.tensors = lambda described: described
+    monkeypatch.setattr(readout, "_check_one_runtime", lambda: None)
+    monkeypatch.setattr(torch.cuda, "init", lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(recorder.current))
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
+    real = torch.device
+    monkeypatch.setattr(torch, "device", lambda *a: real("cpu"))
+    som = pink.SOM(np.zeros((2, 3, 4, 4), np.float32))
+    answers = readout.MapReadout(som, outputs=2, euclidean_distance_dim=3)
+    monkeypatch.setattr(torch, "device", real)
+    answers.distances = lambda images: torch.as_tensor(images)
+    return answers, recorder, torch
+
+
+def test_calls_go_to_the_stream_that_is_current_when_they_are_made(made):
+    answers, recorder, torch = made
+    heat = torch.rand(5, 6)
+    for stream in ("first", "second", "second", "first", "third"):
+        recorder.current = stream
+        answers.step(heat, targets=torch.zeros(5, 2))
+        answers(heat)
+    assert {name for name, *_ in recorder.calls} == {"route", "experts", "experts_backward", "route_backward", "adamw", "balance"}
+    assert all(at == current for _, at, current in recorder.calls)
+
+
+# ------------------------------------------------------------------------------------------------------------ on a GPU
+
+def run(code):
+    """In a process of its own: PyTorch has to come before the library."""
+    code = """
+import numpy as np, torch
+from pink_amd import capi, pink, readout
+EDGE, REGION = 32, 22
+images, targets = readout.synthetic_sources(192, EDGE, np.random.default_rng(1))
+def a_map(seed=2):
+    return pink.SOM(np.random.default_rng(seed).random((4, 4, EDGE, EDGE), dtype=np.float32))
+def made(som, **options):
+    return readout.MapReadout(som, **{**dict(outputs=2, number_of_rotations=36, euclidean_distance_dim=REGION), **options})
+def state(answers):
+    return [v.cpu().numpy() for v in answers.parameters.values()] + [v.cpu().numpy() for s in answers.states.values() for v in s.values()]
+""" + textwrap.dedent(code) + "\nprint('ok', flush=True)\n"
+    done = subprocess.run([sys.executable, "-u", "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and done.stdout.strip().endswith("ok"), done.stdout[-1000:] + done.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_steps_on_changing_streams_are_the_steps_on_one():
+    run("""
+    def train(streams, made_on):
+        with torch.cuda.stream(made_on):
+            answers = made(a_map())
+        out = []
+        for i in range(9):
+            with torch.cuda.stream(streams[i % len(streams)]):
+                at = slice(i % 3 * 64, i % 3 * 64 + 64)
+                loss = answers.step(images[at], targets[at])
+                out.append((loss + 0).cpu().numpy())           # the caller's own work, on its stream
+                out.append(answers(images[at]).cpu().numpy())
+        torch.cuda.synchronize()
+        return out + state(answers)
+    one, two, default = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.default_stream()
+    want = train([default], default)
+    for streams, first in (([one], default), ([one, two], one), ([default, one, two, one], two)):
+        for a, b in zip(train(streams, first), want):
+            assert np.array_equal(a, b)
+    """)
+
+
+@pytest.mark.gpu
+def test_the_callers_device_stays_current():
+    run("""
+    answers = made(a_map())
+    assert answers.device == torch.device("cuda", 0)
+    answers.step(images=images[:32], targets=targets[:32])
+    assert torch.cuda.current_device() == 0
+    assert answers(images[:3]).device == answers.device and answers.distances(images[:3]).device == answers.device
+    """)
