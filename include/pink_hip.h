@@ -267,9 +267,13 @@ int pink_hip_make_update_factors(uint32_t layout, const uint32_t *dims, uint32_t
  *
  * All data pointers are device pointers.  Calls are asynchronous on the handle's stream: its own, or
  * one given with pink_hip_readout_set_stream; inputs made on another stream have to be complete (or
- * ordered by events) before.  The handle holds a workspace that grows to what its calls need (a call
- * that makes it grow waits for the stream, allocates, and cannot be captured into a graph:
- * pink_hip_readout_reserve grows it beforehand).  A handle must not be used from two threads at once.
+ * ordered by events) before.  The handle holds a workspace that grows to what its calls need; a call
+ * that makes it grow waits for the stream and allocates (pink_hip_readout_reserve grows it beforehand),
+ * and is refused with PINK_HIP_ESTATE while the stream is captured into a graph.  A graph of recorded
+ * calls works in the workspace they were recorded with: the handle keeps that one, also past its growing,
+ * until it is destroyed, and no such graph may be launched afterwards; launches and other calls of
+ * the handle have to follow one another as calls on one stream do.  A handle must not be used from
+ * two threads at once.
  * Results do not depend on the order in which blocks run: the same call gives the same bits.
  */
 typedef struct pink_hip_readout pink_hip_readout;

@@ -19,7 +19,14 @@ struct pink_hip_readout {
     hipStream_t own, stream;
     void *work;
     size_t work_bytes;
+    bool recorded;                 // a graph holds the address of `work`
+    struct Former *former;         // workspaces that graphs hold and calls have outgrown
     char err[320];
+};
+
+struct Former {
+    void *work;
+    Former *next;
 };
 
 namespace {
@@ -1125,13 +1132,28 @@ size_t element_bytes(const pink_hip_readout *r) { return r->cfg.element == PINK_
 
 uint32_t group_size(const pink_hip_readout_config &c) { return (c.neurons + c.groups - 1) / c.groups; }
 
+// The workspace holds so many bytes from here on.  One whose address a recorded graph may hold is kept beside the next until the handle
+// is destroyed.
 int grow(pink_hip_readout *r, size_t bytes)
 {
+    hipStreamCaptureStatus capture;
+    HIP_TRY(r, hipStreamIsCapturing(r->stream, &capture));
+    if (capture != hipStreamCaptureStatusNone) {
+        if (bytes > r->work_bytes) return fail(r, PINK_HIP_ESTATE, "a recorded call needs a larger workspace: pink_hip_readout_reserve before");
+        r->recorded = true;
+    }
     if (bytes <= r->work_bytes) return PINK_HIP_OK;
     HIP_TRY(r, hipStreamSynchronize(r->stream));
-    if (r->work) HIP_TRY(r, hipFree(r->work));
+    if (r->recorded) {
+        Former *const kept = new (std::nothrow) Former{r->work, r->former};
+        if (!kept) return fail(r, PINK_HIP_ENOMEM, "pink_hip_readout: out of memory");
+        r->former = kept;
+    } else if (r->work) {
+        HIP_TRY(r, hipFree(r->work));
+    }
     r->work = nullptr;
     r->work_bytes = 0;
+    r->recorded = false;
     HIP_TRY(r, hipMalloc(&r->work, bytes));
     r->work_bytes = bytes;
     return PINK_HIP_OK;
@@ -1603,6 +1625,11 @@ void pink_hip_readout_destroy(pink_hip_readout *r)
     if (r->stream != r->own) (void)hipStreamSynchronize(r->stream);
     (void)hipStreamSynchronize(r->own);
     if (r->work) (void)hipFree(r->work);
+    while (Former *const kept = r->former) {
+        (void)hipFree(kept->work);
+        r->former = kept->next;
+        delete kept;
+    }
     (void)hipStreamDestroy(r->own);
     delete r;
 }
