@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from pink_amd import capi
-from test_readout import Element, experts_inputs, gpu  # noqa: F401  (gpu: fixture)
+from test_readout import ACT, BENT, S, STEEP, Element, assert_within, experts_inputs, experts_reference, f_and_slope, gpu, to_bf16  # noqa: F401  (gpu: fixture)
 
 
 # -------------------------------------------------------------------------------------------- graphs and the workspace
@@ -107,3 +107,67 @@ def test_recorded_calls_do_not_grow_the_workspace(gpu):  # noqa: F811
         recording.launch()
         ro.synchronize()
         recording.close()
+
+
+# ----------------------------------------------------------------------------------------------- what is kept of a model
+
+KEPT_GATES = [0.0, -0.0, 1e-45, 1e-25, 1e-21, 1e-19, 1e-10, 0.5, -0.75]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("act", ["identity", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("size", [1.0, 1e3, 1e5, 1e20])
+def test_gradients_of_gates_that_are_small(gpu, act, bf16, size):  # noqa: F811
+    """A gate's gradient does not depend on the gate: right at any gate, and for values before the activation of any size."""
+    rng = np.random.default_rng(6)
+    element, t, n, k, f, h, o = Element(bf16), 90, 3, 3, 16, 24, 8
+    stored, value, neuron, _ = experts_inputs(rng, element, t, n, k, f, h, o)
+    for i in ("w1", "b1"):
+        stored[i], value[i] = element.store(value[i] * size)
+    gates = np.resize(np.array(KEPT_GATES, np.float32), (t, k))
+    dy_stored, dy = element.store(rng.standard_normal((t, o)))
+    with np.errstate(over="ignore", under="ignore"):
+        want = experts_reference(value, element, act, neuron, gates, dy)
+    with capi.Readout(n, k, f, h, o, activation=ACT[act], element=element.id) as ro:
+        p = {i: gpu.up(v) for i, v in stored.items()}
+        weights, saved, y = [p[i] for i in ("w1", "b1", "w2", "b2")], gpu.new(ro.saved_bytes(t), np.int8), gpu.new((t, o), element.dtype)
+        g, dgates = gpu.up(gates), gpu.new((t, k), element.dtype)
+        ro.experts(p["x"], t, gpu.up(neuron), g, weights, y, dev_saved=saved)
+        ro.experts_backward(p["x"], t, g, weights, saved, gpu.up(dy_stored), [None, dgates, None, None, None, None])
+        ro.synchronize()
+        assert_within(element.values(gpu.down(dgates, (t, k), element.dtype)), *want["dgates"], "of gates")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_slopes_from_what_bfloat16_models_keep(gpu, act):  # noqa: F811
+    """Of a before GELU and SILU 11 bits are kept, so a slope near zero is off by 2^-11 of a, not by 2^-8; a value comes from gate f(a),
+    rounded once.  One image a neuron and one hidden value: bias gradients are da itself."""
+    element, n = Element(True), 2048
+    rng = np.random.default_rng(8)
+    # a = x w1 + b1 is a number of 32 bits; slopes cross zero at -0.75 (GELU) and -1.28 (SILU)
+    _, x = element.store(np.ones((n, 1)))
+    w1s, w1 = element.store(rng.uniform(-2, 1, (n, 1, 1)))
+    b1s, b1 = element.store(rng.uniform(-0.25, 0.25, (n, 1)))
+    w2s, w2 = element.store(rng.uniform(0.5, 1, (n, 1, 1)))
+    dys, dy = element.store(rng.uniform(0.5, 1, (n, 1)))
+    gates = rng.uniform(0.1, 1, (n, 1)).astype(np.float32)
+    a, g, back = w1[:, 0, 0] + b1[:, 0], gates[:, 0].astype(np.float64), dy[:, 0] * w2[:, 0, 0]
+    v, slope = f_and_slope(act, a)
+    off_a = 4 * S * np.abs(a) + 2.0 ** -11 * np.abs(a)
+    da = g * back * slope
+    off_da = np.abs(g * back) * (BENT[act] * off_a + 8 * S * (1 + np.abs(a))) + 4 * S * np.abs(da)
+    dg = back * v
+    off_dg = np.abs(back) * (8 * S * (np.abs(a) + np.abs(v)) + element.u * np.abs(v)) + 8 * S * np.abs(dg)
+    assert (np.abs(g * back) * BENT[act] * 2.0 ** -9 * np.abs(a) > 1.5 * (off_da + element.u * np.abs(da))).any()        # 8 bits would show
+    with capi.Readout(n, 1, 1, 1, 1, activation=ACT[act], element=element.id) as ro:
+        weights = [gpu.up(w1s), gpu.up(b1s), gpu.up(w2s), None]
+        saved, y, db1, dgates = gpu.new(ro.saved_bytes(n), np.int8), gpu.new((n, 1), np.uint16), gpu.new((n, 1), np.uint16), gpu.new((n, 1), np.uint16)
+        xs, at, gd = gpu.up(to_bf16(x)), gpu.up(np.arange(n, dtype=np.int32)[:, None]), gpu.up(gates)
+        ro.experts(xs, n, at, gd, weights, y, dev_saved=saved)
+        ro.experts_backward(xs, n, gd, weights, saved, gpu.up(dys), [None, dgates, None, db1, None, None])
+        ro.synchronize()
+        # (da is rounded as it is kept, and a sum of one term of that is the same number)
+        assert_within(element.values(gpu.down(db1, (n, 1), np.uint16))[:, 0], da, off_da + element.u * (np.abs(da) + off_da), "da")
+        assert_within(element.values(gpu.down(dgates, (n, 1), np.uint16))[:, 0], dg, off_dg + element.u * (np.abs(dg) + off_dg), "of gates")
