@@ -948,11 +948,13 @@ __device__ __forceinline__ float second_value(uint8_t code, float scale)
 
 // A thread has kAdamRuns times four neighbouring values, 1024 apart, so that a wave's access is a run of memory and a block of 256
 // codes belongs to a wave.  All that is read is asked for before anything is done with it.  The states follow by sums, products,
-// roots and reciprocals that are each rounded (the codes are whole numbers and must not go by how they were computed); the
-// value's own step takes the hardware's root and reciprocal, one unit off at most, which is 2^-23 of a step.
+// roots and reciprocals that are each rounded (the codes are whole numbers and must not go by how they were computed).  The
+// value's own step takes the hardware's root and reciprocal, each off by one unit at most: 2^-22 of a step.  They take subnormal
+// numbers for 0, which is as little where epsilon is 2^-38 or more (the root of a subnormal number is below 2^-63).  Below that
+// SMALL_EPSILON divides by what is rounded; so a step without a gradient is 0 at any epsilon.
 // 224 M values, bfloat16 gradients and copies, 8-bit states: 737 us for 3.6 GB (4.9 TB/s; a copy reaches 4.8); with every root
 // rounded it was 821 us and bound by the vector ALU (117 instructions a value, now 77).  44 M values, float32 states: 224 us, 5.5 TB/s.
-template <bool CODES> __global__ __launch_bounds__(256) void k_adamw(const AdamArgs g)
+template <bool CODES, bool SMALL_EPSILON> __global__ __launch_bounds__(256) void k_adamw(const AdamArgs g)
 {
     const uint32_t which = adam_tensor(g);
     const pink_hip_readout_tensor &t = g.tensor[which];
@@ -994,7 +996,8 @@ template <bool CODES> __global__ __launch_bounds__(256) void k_adamw(const AdamA
             }
             m[n][i] = m[n][i] * g.beta1 + grad * g.rest1;
             v[n][i] = v[n][i] * g.beta2 + (grad * grad) * g.rest2;
-            const float step = (m[n][i] * g.c1) * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[n][i] * g.c2) + g.epsilon);
+            const float step = SMALL_EPSILON ? (m[n][i] * g.c1) / (sqrtf(v[n][i] * g.c2) + g.epsilon)
+                                             : (m[n][i] * g.c1) * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[n][i] * g.c2) + g.epsilon);
             p[n][i] = p[n][i] - (step + p[n][i] * t.decay) * g.rate;
         }
         store_run(t.value + at, p[n], valid[n]);
@@ -1840,8 +1843,11 @@ int pink_hip_readout_adamw(pink_hip_readout *r, const pink_hip_readout_tensor *t
             return PINK_HIP_OK;
         },
         [&](uint32_t blocks) {
-            if (state_bits == 8) k_adamw<true><<<blocks, 256, 0, r->stream>>>(g);
-            else k_adamw<false><<<blocks, 256, 0, r->stream>>>(g);
+            const bool small = epsilon < 0x1p-38f;
+            if (state_bits == 8 && small) k_adamw<true, true><<<blocks, 256, 0, r->stream>>>(g);
+            else if (state_bits == 8) k_adamw<true, false><<<blocks, 256, 0, r->stream>>>(g);
+            else if (small) k_adamw<false, true><<<blocks, 256, 0, r->stream>>>(g);
+            else k_adamw<false, false><<<blocks, 256, 0, r->stream>>>(g);
         });
 }
 

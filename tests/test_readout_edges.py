@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from pink_amd import capi
-from test_readout import ACT, BENT, S, STEEP, Element, assert_within, experts_inputs, experts_reference, f_and_slope, gpu, to_bf16  # noqa: F401  (gpu: fixture)
+from test_readout import ACT, BENT, S, STEEP, Element, assert_within, experts_inputs, experts_reference, f_and_slope, gpu, pack, to_bf16  # noqa: F401  (gpu: fixture)
 
 
 # -------------------------------------------------------------------------------------------- graphs and the workspace
@@ -107,6 +107,52 @@ def test_recorded_calls_do_not_grow_the_workspace(gpu):  # noqa: F811
         recording.launch()
         ro.synchronize()
         recording.close()
+
+
+# --------------------------------------------------------------------------------------------------------------- AdamW
+
+F = np.float32
+
+
+def adamw_tensor(gpu, value, grad, bits, m=None, v=None, decay=0.0):  # noqa: F811
+    """(the descriptor, pointers to the two states' values)"""
+    n = value.size
+    m, v = (np.zeros(n, F) if x is None else x for x in (m, v))
+    t = dict(value=gpu.up(value), gradient=gpu.up(grad), size=n, decay=decay)
+    if bits == 8:
+        (mc, ms), (vc, vs) = pack(m, False), pack(v, True)
+        t.update(first=gpu.up(mc), second=gpu.up(vc), first_scale=gpu.up(ms), second_scale=gpu.up(vs), first_values=gpu.new(n, F), second_values=gpu.new(n, F))
+        return t, ("first_values", "second_values")
+    t.update(first=gpu.up(m), second=gpu.up(v))
+    return t, ("first", "second")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("epsilon", [1e-45, 1e-40, 2.0 ** -126, 1e-30, 1e-20, 2.0 ** -39, 2.0 ** -38, 1e-8, 1.0])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_small_gradients_and_epsilons(gpu, bits, epsilon):  # noqa: F811
+    # whole blocks of gradients of one size, from those that are no gradient at all to those whose square is subnormal, or 0
+    rng = np.random.default_rng(3)
+    sizes = np.array([0, 1e-37, 1e-30, 1e-24, 3e-23, 1e-21, 1e-20, 1e-19, 1e-18, 1e-8, 1], F)
+    grad = (np.repeat(sizes, 256) * rng.choice([-1, 1], sizes.size * 256)).astype(F)
+    value = rng.standard_normal(grad.size).astype(F)
+    lr, b1, b2, step = F(2e-3), F(0.9), F(0.99), 1
+    with capi.Readout(4) as ro:
+        t, _ = adamw_tensor(gpu, value, grad, bits)
+        ro.adamw(ro.tensors([t]), step, learning_rate=lr, beta_first=b1, beta_second=b2, epsilon=epsilon, bits=bits)
+        ro.synchronize()
+        got = gpu.down(t["value"], grad.size, F).astype(np.float64)
+    m, v = (grad * (F(1) - b1)).astype(F).astype(np.float64), ((grad * grad) * (F(1) - b2)).astype(F).astype(np.float64)
+    eps, c1, c2 = float(F(epsilon)), 1 / (1 - float(b1) ** step), 1 / (1 - float(b2) ** step)
+    root = np.sqrt(v * c2)
+    # c2 second is rounded, below 2^-126 to multiples of 2^-149; a root moves by no more than d / root, nor than sqrt(d)
+    d = 2 * S * v * c2 + 2.0 ** -150
+    off_root = np.minimum(np.sqrt(d), d / np.maximum(root, 1e-300)) * (v > 0)
+    change = m * c1 / (root + eps)
+    off = np.abs(change) * (16 * S + off_root / (np.maximum(root - off_root, 0) + eps)) + 2.0 ** -148 * c1 / (root + eps)
+    want = value.astype(np.float64) - float(lr) * change
+    assert_within(got, want, float(lr) * off + 2 * S * np.abs(want), "value")
+    assert np.array_equal(got[:256], value[:256])          # where there was no gradient nothing moves
 
 
 # ----------------------------------------------------------------------------------------------- what is kept of a model
