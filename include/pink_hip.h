@@ -382,7 +382,8 @@ typedef struct pink_hip_readout_tensor {
  * value -= learning_rate * (c1 first / (sqrt(c2 second) + epsilon) + decay * value),  ci = 1 / (1 - beta_i^step)
  * in float32, over all tensors at once.  With state_bits 8 the states are held as codes: q in -127..127
  * is sign(q) (q/127)^2 and q in 0..255 is (q/255)^4 times the scale, the block's largest magnitude (0
- * where that is below 2^-126); a second state above zero never becomes zero by packing. */
+ * where that is below 2^-126); a second state above zero never becomes zero by packing.  All of a block
+ * with a state that is not finite stands for NaN. */
 int pink_hip_readout_adamw(pink_hip_readout *readout, const pink_hip_readout_tensor *tensors, uint32_t count, uint32_t state_bits,
                            uint64_t step, float learning_rate, float beta_first, float beta_second, float epsilon);
 /* The values that the tensors' 8-bit states stand for, into first_values and second_values. */

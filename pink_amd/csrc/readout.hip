@@ -1008,15 +1008,14 @@ template <bool CODES, bool SMALL_EPSILON> __global__ __launch_bounds__(256) void
             store_run((Bfloat *)t.rounded + at, b, valid[n]);
         }
         if constexpr (CODES) {
-            // (values past the end are zero; magnitudes order as their bits do)
-            float most_m = 0.0f, most_v = 0.0f;
+            // (values past the end are zero; magnitudes order as their bits do, and NaN is the largest)
+            uint32_t bits_m = 0, bits_v = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                most_m = fmaxf(most_m, fabsf(m[n][i]));
-                most_v = fmaxf(most_v, fabsf(v[n][i]));
+                bits_m = max(bits_m, __float_as_uint(fabsf(m[n][i])));
+                bits_v = max(bits_v, __float_as_uint(fabsf(v[n][i])));
             }
-            most_m = __uint_as_float(wave_max_u32(__float_as_uint(most_m)));
-            most_v = __uint_as_float(wave_max_u32(__float_as_uint(most_v)));
+            float most_m = __uint_as_float(wave_max_u32(bits_m)), most_v = __uint_as_float(wave_max_u32(bits_v));
             most_m = most_m < 1.175494351e-38f ? 0.0f : most_m;
             most_v = most_v < 1.175494351e-38f ? 0.0f : most_v;
             const float mi = most_m > 0.0f ? 1.0f / most_m : 0.0f, vi = most_v > 0.0f ? 1.0f / most_v : 0.0f;
@@ -1033,13 +1032,13 @@ template <bool CODES, bool SMALL_EPSILON> __global__ __launch_bounds__(256) void
                 const float root_v = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(ratio_v[i])) * 255.0f;
                 code_m[i] = rintf(root_m);
                 code_v[i] = rintf(root_v);
-                close = close || fabsf(root_m - code_m[i]) > 0.5f - 5e-5f || fabsf(root_v - code_v[i]) > 0.5f - 1e-4f;
+                close = close || !(fabsf(root_m - code_m[i]) <= 0.5f - 5e-5f && fabsf(root_v - code_v[i]) <= 0.5f - 1e-4f);
             }
-            if (close) {
+            if (close) {                                   // (and NaN: code 0 of a scale that is not finite is NaN again)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    code_m[i] = rintf(sqrtf(ratio_m[i]) * 127.0f);
-                    code_v[i] = rintf(sqrtf(sqrtf(ratio_v[i])) * 255.0f);
+                    code_m[i] = ratio_m[i] >= 0.0f ? rintf(sqrtf(ratio_m[i]) * 127.0f) : 0.0f;
+                    code_v[i] = ratio_v[i] >= 0.0f ? rintf(sqrtf(sqrtf(ratio_v[i])) * 255.0f) : 0.0f;
                 }
             }
             int8_t mo[4];

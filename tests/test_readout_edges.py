@@ -155,6 +155,42 @@ def test_adamw_of_small_gradients_and_epsilons(gpu, bits, epsilon):  # noqa: F81
     assert np.array_equal(got[:256], value[:256])          # where there was no gradient nothing moves
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_gradients_that_are_not_finite(gpu, bits):  # noqa: F811
+    """They go into the value and the states; of 8-bit states a block's scale is its largest magnitude, so the block holds NaN from then on."""
+    rng = np.random.default_rng(4)
+    n, options = 5 * 256 + 100, dict(learning_rate=2e-3, beta_first=0.9, beta_second=0.99, epsilon=1e-8)
+    value, grad = rng.standard_normal(n).astype(F), rng.standard_normal(n).astype(F)
+    m, v = (0.1 * rng.standard_normal(n)).astype(F), (0.01 * rng.standard_normal(n) ** 2).astype(F)
+    bad = {300: np.nan, 256 * 2 + 255: np.inf, 256 * 3: -np.inf, n - 1: np.nan}
+    for at, x in bad.items():
+        grad[at] = x
+    with capi.Readout(4) as ro:
+        t, states = adamw_tensor(gpu, value, grad, bits, m, v)
+        clean = grad.copy()
+        clean[list(bad)] = 0
+        other, _ = adamw_tensor(gpu, value, clean, bits, m, v)
+        table, without = ro.tensors([t]), ro.tensors([other])
+        hurt = np.isin(np.arange(n), list(bad))
+        block = np.isin(np.arange(n) // 256, [at // 256 for at in bad])
+        for step in (1, 2):
+            for x in (table, without):
+                ro.adamw(x, step, bits=bits, **options)
+                if bits == 8:
+                    ro.adamw_unpack(x)
+            ro.synchronize()
+            got, want = gpu.down(t["value"], n, F), gpu.down(other["value"], n, F)
+            of_value = block if bits == 8 and step == 2 else hurt
+            assert np.isnan(got[of_value]).all() and np.array_equal(got[~of_value], want[~of_value])
+            for name in states:
+                got, want = gpu.down(t[name], n, F), gpu.down(other[name], n, F)
+                of_state = block if bits == 8 else hurt
+                assert not np.isfinite(got[of_state]).any() and np.array_equal(got[~of_state], want[~of_state])
+                if bits == 8:
+                    assert np.isnan(got[of_state]).all()
+
+
 # ----------------------------------------------------------------------------------------------- what is kept of a model
 
 KEPT_GATES = [0.0, -0.0, 1e-45, 1e-25, 1e-21, 1e-19, 1e-10, 0.5, -0.75]
