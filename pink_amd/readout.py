@@ -49,7 +49,7 @@ class MapReadout:
     """Two-layer models of a map's neurons on its heatmap; `chosen` of them answer for an image, weighted by the softmax of
     sharpness * (radius - distance).
 
-    It lives on the device that is current when it is made.  Calls run on that device's stream that is current when they are made, and
+    The map is copied when it is made, as a pink.Mapper does: its models are trained on that map.  It lives on the device that is current when it is made.  Calls run on that device's stream that is current when they are made, and
     what they return is that stream's; a call on another stream than the last one's waits for that one first, so a stream that
     was used has to exist until then."""
 
@@ -61,6 +61,8 @@ class MapReadout:
         self._map_args = (int(number_of_rotations), bool(use_flip), int(euclidean_distance_dim))
         self._map_type = int(euclidean_distance_type)
         n = som.number_of_neurons
+        self._rows = som._rows().copy()
+        self._neuron_channels, self._neuron_dim = pink._image_geometry(som.neuron_shape, som.neuron_layout, "neuron")
         _check_one_runtime()
         capi.Readout.check(n, chosen, n, hidden, outputs, activation=activation)
         torch.cuda.init()
@@ -107,11 +109,10 @@ class MapReadout:
         channels, edge = self._geometry(images)
         if self._mapper is None or self._mapper.I != edge:
             rotations, flip, region = self._map_args
-            _, neuron_dim = pink._image_geometry(self.som.neuron_shape, self.som.neuron_layout, "neuron")
-            self._mapper = capi.Context(self.som.number_of_neurons, channels, edge, neuron_dim, rotations, flip, region, ed_type=self._map_type,
+            self._mapper = capi.Context(len(self._rows), channels, edge, self._neuron_dim, rotations, flip, region, ed_type=self._map_type,
                                         device=self.device.index)
-            self._mapper.set_som(self.som._rows())
-        heat = torch.empty((images.shape[0], self.som.number_of_neurons), device=self.device)
+            self._mapper.set_som(self._rows)
+        heat = torch.empty((images.shape[0], len(self._rows)), device=self.device)
         torch.cuda.synchronize()                           # the mapper runs on a stream of its own
         self._mapper.map_device(images.data_ptr(), images.shape[0], heat.data_ptr())
         self._mapper.synchronize()
@@ -119,8 +120,7 @@ class MapReadout:
 
     def _geometry(self, images):
         channels = 1 if images.dim() == 3 else images.shape[1]
-        neuron_channels, _ = pink._image_geometry(self.som.neuron_shape, self.som.neuron_layout, "neuron")
-        if images.dim() not in (3, 4) or images.shape[-1] != images.shape[-2] or channels != neuron_channels:
+        if images.dim() not in (3, 4) or images.shape[-1] != images.shape[-2] or channels != self._neuron_channels:
             raise pink.exception(-1, "images must be (images, edge, edge) or (images, channels, edge, edge) with the neurons' channels")
         return int(channels), int(images.shape[-1])
 

@@ -124,3 +124,19 @@ def test_the_callers_device_stays_current():
     assert torch.cuda.current_device() == 0
     assert answers(images[:3]).device == answers.device and answers.distances(images[:3]).device == answers.device
     """)
+
+
+@pytest.mark.gpu
+def test_the_map_is_the_one_it_was_made_with():
+    run("""
+    som = a_map()
+    answers, same = made(som), made(a_map())
+    answers.step(images[:64], targets[:64])
+    want = answers(images[:32]).cpu().numpy()
+    small = images[:32, 2:-2, 2:-2].copy()
+    np.asarray(som)[...] = np.asarray(a_map(7))                # the map is trained further
+    assert np.array_equal(answers(images[:32]).cpu().numpy(), want)
+    assert np.array_equal(answers.distances(small).cpu().numpy(), same.distances(small).cpu().numpy())     # images of another edge
+    assert np.array_equal(answers(images[:32]).cpu().numpy(), want)
+    assert not np.array_equal(made(som).distances(small).cpu().numpy(), same.distances(small).cpu().numpy())
+    """)
