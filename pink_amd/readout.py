@@ -49,7 +49,11 @@ class MapReadout:
     """Two-layer models of a map's neurons on its heatmap; `chosen` of them answer for an image, weighted by the softmax of
     sharpness * (radius - distance).
 
-    The map is copied when it is made, as a pink.Mapper does: its models are trained on that map.  It lives on the device that is current when it is made.  Calls run on that device's stream that is current when they are made, and
+    The map is copied when it is made, as a pink.Mapper does: its models are trained on that map.  The first step's images set `level`,
+    the scale of the features, and where sharpness and radius start; answers asked for before go by the scale of their own images.
+    What a trained read-out consists of: parameters, states, bias, level and steps.
+
+    It lives on the device that is current when it is made.  Calls run on that device's stream that is current when they are made, and
     what they return is that stream's; a call on another stream than the last one's waits for that one first, so a stream that
     was used has to exist until then."""
 
@@ -93,7 +97,7 @@ class MapReadout:
             dict(value=v.data_ptr(), gradient=self.gradients[k].data_ptr(), size=v.numel(), decay=weight_decay if k in ("first", "second") else 0.0,
                  **{s: x.data_ptr() for s, x in self.states[k].items()}) for k, v in self.parameters.items()])
         self.bias = zeros(n)                               # for an even load; takes part in the choice of neurons only
-        self.steps, self._level = 0, None
+        self.steps, self.level = 0, None                   # level: mean and spread of the distances
 
     def _follow_stream(self):
         """What was queued for the read-out so far is complete, and the handle works on the caller's current stream."""
@@ -124,23 +128,26 @@ class MapReadout:
             raise pink.exception(-1, "images must be (images, edge, edge) or (images, channels, edge, edge) with the neurons' channels")
         return int(channels), int(images.shape[-1])
 
-    def _features(self, heat):
-        if self._level is None:                            # the first images set the scale, and the radius where routing starts
-            self._level = heat.mean(), heat.std() + 1e-6
-            self.parameters["sharpness"].fill_(1.0).div_(self._level[1])
-            self.parameters["radius"].copy_(heat.mean(0))
-        return ((heat - self._level[0]) / self._level[1]).contiguous()
+    def _levels(self, heat):
+        """(mean and spread of the images' distances, sharpness and radius to start from).  Distances that are not finite take no part."""
+        part = torch.isfinite(heat)
+        count, known = part.sum(), torch.where(part, heat, 0.0)
+        mean = known.sum() / count.clamp(min=1)
+        spread = (torch.where(part, heat - mean, 0.0).square().sum() / (count - 1).clamp(min=1)).sqrt() + 1e-6
+        each = part.sum(0)
+        return torch.stack((mean, spread)), (1 / spread).repeat(heat.shape[1]), torch.where(each > 0, known.sum(0) / each.clamp(min=1), mean)
 
     def _weights(self):
         return [self.parameters[k].data_ptr() for k in ("first", "first_bias", "second", "second_bias")]
 
     def _forward(self, heat, keep):
         r, p, t = self.readout, self.parameters, heat.shape[0]
-        x = self._features(heat)
+        level, sharpness, radius = (self.level, p["sharpness"], p["radius"]) if self.level is not None else self._levels(heat)
+        x = torch.where(torch.isfinite(heat), (heat - level[0]) / level[1], 0.0)
         neuron = torch.empty((t, self.chosen), dtype=torch.int32, device=self.device)
         gates, y = torch.empty((t, self.chosen), device=self.device), torch.empty((t, self.outputs), device=self.device)
         saved = torch.empty(r.saved_bytes(t), dtype=torch.uint8, device=self.device) if keep else None
-        r.route(heat.data_ptr(), t, p["sharpness"].data_ptr(), p["radius"].data_ptr(), self.bias.data_ptr(), neuron.data_ptr(), gates.data_ptr())
+        r.route(heat.data_ptr(), t, sharpness.data_ptr(), radius.data_ptr(), self.bias.data_ptr(), neuron.data_ptr(), gates.data_ptr())
         r.experts(x.data_ptr(), t, neuron.data_ptr(), gates.data_ptr(), self._weights(), y.data_ptr(), dev_saved=saved.data_ptr() if keep else None)
         return x, neuron, gates, y, saved
 
@@ -155,6 +162,14 @@ class MapReadout:
         r, p, g = self.readout, self.parameters, self.gradients
         heat = self.distances(images)
         t = heat.shape[0]
+        if t == 0:
+            raise pink.exception(-1, "a step needs images")
+        if self.level is None:
+            if not torch.isfinite(heat).any():
+                raise pink.exception(-1, "the first step needs an image with a finite distance")
+            self.level, sharpness, radius = self._levels(heat)
+            p["sharpness"].copy_(sharpness)
+            p["radius"].copy_(radius)
         x, neuron, gates, y, saved = self._forward(heat, True)
         off = y - torch.as_tensor(targets, dtype=torch.float32, device=self.device).reshape(t, self.outputs)
         dy, dgates = off * (2.0 / off.numel()), torch.empty_like(gates)

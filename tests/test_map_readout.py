@@ -140,3 +140,70 @@ def test_the_map_is_the_one_it_was_made_with():
     assert np.array_equal(answers(images[:32]).cpu().numpy(), want)
     assert not np.array_equal(made(som).distances(small).cpu().numpy(), same.distances(small).cpu().numpy())
     """)
+
+
+@pytest.mark.gpu
+def test_answers_before_the_first_step_change_nothing():
+    run("""
+    asked, not_asked = made(a_map()), made(a_map())
+    assert np.isfinite(asked(images[100:103]).cpu().numpy()).all() and tuple(asked(images[:0]).shape) == (0, 2)
+    assert asked.level is None
+    for answers in (asked, not_asked):
+        for i in range(3):
+            answers.step(images[:64], targets[:64])
+    heat = not_asked.distances(images[:64]).cpu().numpy().astype(np.float64)
+    assert np.allclose(not_asked.level.cpu().numpy(), [heat.mean(), heat.std(ddof=1) + 1e-6], rtol=1e-5)
+    for a, b in zip(state(asked), state(not_asked)):
+        assert np.array_equal(a, b)
+    """)
+
+
+@pytest.mark.gpu
+def test_distances_that_are_not_finite():
+    # a neuron out of the competition, an image without any distance, a few entries: of the first images, and of later ones
+    run("""
+    clean, masked = made(a_map(), chosen=3), made(a_map(), chosen=3)
+    heat = clean.distances(images[:64])
+    hurt = heat.clone()
+    hurt[:, 5], hurt[9], hurt[3, 7], hurt[4, 8] = float("inf"), float("nan"), float("nan"), float("-inf")
+    for answers in (clean, masked):
+        answers.distances = lambda images: torch.as_tensor(images, device="cuda")
+    part = np.isfinite(hurt.cpu().numpy())
+    known = hurt.cpu().numpy().astype(np.float64)[part]
+    for i in range(4):
+        loss = masked.step(hurt, targets[:64])
+        assert np.isfinite(float(loss))
+        if i == 0:
+            assert np.allclose(masked.level.cpu().numpy(), [known.mean(), known.std(ddof=1) + 1e-6], rtol=1e-5)
+    assert all(np.isfinite(x).all() for x in state(masked) if x.dtype == np.float32)
+    assert not masked.states["second"]["first"].reshape(16, -1)[5].any()     # the neuron answered for nobody
+    y = masked(hurt).cpu().numpy()
+    assert np.isfinite(y).all() and not y[9].any()
+    clean.step(heat, targets[:64])
+    before = clean(heat).cpu().numpy()
+    far = int(heat[0].argmax())                                # not among the three that answer for image 0
+    one = heat[:1].clone()
+    one[0, far] = float("inf")
+    assert np.isfinite(clean(one).cpu().numpy()).all() and np.isfinite(before).all()
+    """)
+
+
+@pytest.mark.gpu
+def test_steps_that_are_refused():
+    run("""
+    answers = made(a_map())
+    real, none = answers.distances, torch.full((4, 16), float("inf"), device="cuda")
+    for heat, text in ((none[:0], "needs images"), (none, "finite distance")):
+        answers.distances = lambda images: heat
+        try:
+            answers.step(None, targets[:len(heat)])
+        except pink.exception as e:
+            assert text in str(e)
+        else:
+            raise AssertionError("taken")
+        assert answers.level is None and answers.steps == 0
+    answers.distances = real
+    one = readout.MapReadout(pink.SOM(np.ones((1, 1, EDGE, EDGE), np.float32)), outputs=2, chosen=1, number_of_rotations=36, euclidean_distance_dim=REGION)
+    assert np.isfinite(float(one.step(images[:1], targets[:1]))) and np.isfinite(one(images[:5]).cpu().numpy()).all()       # one distance in all
+    assert np.isfinite(float(answers.step(images[:64], targets[:64])))
+    """)
