@@ -6,6 +6,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
+import test_readout as base
 from pink_amd import capi
 from test_readout import ACT, BENT, S, STEEP, Element, assert_within, experts_inputs, experts_reference, f_and_slope, gpu, pack, to_bf16  # noqa: F401  (gpu: fixture)
 
@@ -253,3 +254,70 @@ def test_slopes_from_what_bfloat16_models_keep(gpu, act):  # noqa: F811
         # (da is rounded as it is kept, and a sum of one term of that is the same number)
         assert_within(element.values(gpu.down(db1, (n, 1), np.uint16))[:, 0], da, off_da + element.u * (np.abs(da) + off_da), "da")
         assert_within(element.values(gpu.down(dgates, (n, 1), np.uint16))[:, 0], dg, off_dg + element.u * (np.abs(dg) + off_dg), "of gates")
+
+
+# ------------------------------------------------------------------------------------------ large maps and long batches
+
+LARGE_ROUTES = [  # images, neurons, chosen, sigmoid, renormalise, groups, kept, bias, ties; one for every number of registers
+    (9, 200, 3, False, False, 1, 1, True, False), (9, 200, 64, True, True, 1, 1, False, True),
+    (5, 380, 7, False, False, 1, 1, False, True), (9, 500, 5, False, True, 1, 1, True, True),
+    (9, 700, 64, False, False, 1, 1, False, True), (9, 768, 2, True, False, 1, 1, True, False),
+    (6, 1000, 9, False, True, 1, 1, True, True), (6, 1024, 64, False, False, 1, 1, True, False),
+    (6, 1200, 33, True, True, 1, 1, False, True), (6, 1280, 8, False, False, 1, 1, False, False),
+    (5, 1500, 64, False, True, 1, 1, True, True), (5, 1536, 1, False, False, 1, 1, True, True),
+    (5, 1600, 8, True, False, 1, 1, True, False), (5, 1600, 64, False, False, 1, 1, False, True),
+    (5, 1700, 17, False, True, 1, 1, True, True), (5, 1800, 64, False, False, 1, 1, True, True),
+    (4, 2048, 64, True, True, 1, 1, False, True), (4, 2047, 5, False, False, 1, 1, True, False),
+    # groups whose kept neurons are more than eight registers, and fewer, beside as many of all neurons
+    (4, 1600, 64, False, True, 40, 20, True, True), (4, 2000, 9, False, False, 10, 9, False, False), (4, 700, 64, True, True, 7, 7, True, True),
+    (4, 700, 20, False, False, 35, 5, True, True), (4, 1000, 6, False, True, 50, 3, False, False), (4, 1270, 4, False, False, 64, 2, True, True),
+    (4, 1500, 8, True, False, 2, 1, False, True), (4, 2048, 8, False, True, 64, 16, True, False), (4, 2040, 8, False, True, 2, 2, True, False),
+    (2, 32768, 64, False, False, 1, 1, True, False), (2, 20000, 9, True, True, 1000, 30, False, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", LARGE_ROUTES, ids=lambda c: "-".join(str(int(x)) for x in c))
+def test_route_of_large_maps(gpu, case):  # noqa: F811
+    base.test_route(gpu, *case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [c for c in LARGE_ROUTES if c[1] <= 2048 and not c[2] == 64] + [
+    # blocks of up to 64 images each
+    (16500, 9, 2, False, False, 1, 1, True, False), (16384, 9, 3, False, True, 3, 2, False, False), (16400, 5, 2, True, True, 1, 1, False, False),
+    (20001, 9, 1, True, False, 1, 1, True, False), (4099, 260, 2, False, False, 1, 1, False, False),
+], ids=lambda c: "-".join(str(int(x)) for x in c))
+def test_route_backward_of_large_maps_and_long_batches(gpu, case):  # noqa: F811
+    base.test_route_backward(gpu, *case, bf16=case[1] % 2 == 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t, n, k", [(20000, 32768, 3), (70000, 1600, 4), (3, 32768, 64)])
+def test_balance_of_large_maps(gpu, t, n, k):  # noqa: F811
+    rng = np.random.default_rng(t)
+    neuron = (n * rng.random((t, k)) ** 3).astype(np.int32)
+    neuron[rng.random((t, k)) < 0.1] = -1
+    load = np.bincount(neuron[neuron >= 0], minlength=n)
+    bias = rng.standard_normal(n).astype(np.float32)
+    with capi.Readout(n, k) as ro:
+        p, got = gpu.up(bias), gpu.new(n, np.int32)
+        ro.balance(gpu.up(neuron), t, 0.01, p, got)
+        ro.synchronize()
+        assert np.array_equal(gpu.down(got, n, np.int32), load)
+        assert np.array_equal(gpu.down(p, n, np.float32), bias + np.float32(0.01) * np.sign(load.sum() - load * n).astype(np.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("t, n, k, f, h, o", [
+    # rows sorted by one block, and by several, where a thread has several neurons; fewer waves to a block from 2048 neurons on
+    (300, 1600, 2, 24, 16, 8), (3000, 1600, 2, 24, 16, 8), (300, 1024, 3, 8, 8, 8), (1400, 1025, 3, 9, 7, 5), (300, 5000, 2, 16, 8, 4), (1600, 5000, 2, 15, 9, 3),
+    (100, 32768, 2, 3, 2, 2), (350, 32768, 2, 8, 8, 8),
+])
+def test_models_of_large_maps(gpu, t, n, k, f, h, o, bf16):  # noqa: F811
+    def spread(rng, shape):                                # most on few neurons, the others anywhere; some places unused
+        neuron = np.where(rng.random(shape) < 0.5, rng.integers(n - 3, n, shape), rng.integers(0, n, shape))
+        return np.where(rng.random(shape) < 0.1, -1, neuron)
+
+    base.test_experts(gpu, t, n, k, f, h, o, "silu", True, True, spread, 0, bf16)
