@@ -1202,7 +1202,8 @@ struct Work {
     size_t counts, totals, rows, partial, few, saved, bytes;
 };
 
-Work work_layout(const pink_hip_readout *r, uint64_t images)
+// `saved`: bytes in the place of a caller's buffer (forward calls that keep nothing) or of gradients of `before`.
+Work work_layout(const pink_hip_readout *r, uint64_t images, size_t saved)
 {
     const pink_hip_readout_config &c = r->cfg;
     const size_t slots = images * c.chosen, plan_blocks = slots / (plan_waves(c.neurons) * 64) + 1;
@@ -1215,10 +1216,10 @@ Work work_layout(const pink_hip_readout *r, uint64_t images)
     };
     w.counts = take(plan_blocks * c.neurons * 4);
     w.totals = take((size_t)c.neurons * 4);
-    w.rows = take(slots * whole_rows(std::max(c.features, c.outputs)) * 4);
+    w.rows = take(c.chosen > 1 ? slots * whole_rows(std::max(c.features, c.outputs)) * 4 : 0);       // (one neuron's go straight to the image)
     w.partial = take(slots * ((c.hidden + 31) / 32) * 4);
     w.few = take(std::min<size_t>(slots, kFewSlots) * c.hidden * 4);
-    w.saved = take(saved_layout(r, images).bytes);         // forward calls that keep nothing; gradients of `before`
+    w.saved = take(saved);
     w.bytes = at;
     return w;
 }
@@ -1405,7 +1406,7 @@ int experts(pink_hip_readout *r, const void *x, uint32_t images, uint64_t x_stri
 {
     const pink_hip_readout_config &c = r->cfg;
     const Saved s = saved_layout(r, images);
-    const Work w = work_layout(r, images);
+    const Work w = work_layout(r, images, keep ? 0 : s.bytes);
     TRY(grow(r, w.bytes));
     char *const work = (char *)r->work, *const saved = keep ? (char *)keep : work + w.saved;
     const uint32_t slots = images * c.chosen;
@@ -1470,13 +1471,13 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
 {
     const pink_hip_readout_config &c = r->cfg;
     const Saved s = saved_layout(r, images);
-    const Work w = work_layout(r, images);
+    const uint32_t slots = images * c.chosen;
+    const Work w = work_layout(r, images, slots * s.stride * element_bytes(r));
     TRY(grow(r, w.bytes));
     char *const work = (char *)r->work;
     const char *const saved = (const char *)keep;
-    const uint32_t slots = images * c.chosen;
     const int32_t *const place = (const int32_t *)(saved + s.place);
-    void *const dbefore = work + w.saved;                  // (slots x stride: `saved` is larger)
+    void *const dbefore = work + w.saved;                  // slots x stride
 
     ProductArgs g = {};
     g.order = (const uint32_t *)(saved + s.order);
@@ -1753,7 +1754,7 @@ int pink_hip_readout_reserve(pink_hip_readout *r, uint32_t images)
     TRY(check_images(r, images));
     HIP_TRY(r, hipSetDevice(r->cfg.device));
     const size_t parts = ((size_t)images / 4 + 1) * r->cfg.neurons * 8;
-    return grow(r, std::max(parts, r->cfg.features ? work_layout(r, images).bytes : 0));
+    return grow(r, std::max(parts, r->cfg.features ? work_layout(r, images, saved_layout(r, images).bytes).bytes : 0));
 }
 
 size_t pink_hip_readout_saved_bytes(pink_hip_readout *r, uint32_t images)

@@ -110,6 +110,28 @@ def test_recorded_calls_do_not_grow_the_workspace(gpu):  # noqa: F811
         recording.close()
 
 
+@pytest.mark.gpu
+def test_the_workspace_takes_what_calls_need(gpu):  # noqa: F811
+    """No rows to be added up where one neuron answers, no second place for what a caller's buffer holds."""
+    def free():
+        now, all_ = C.c_size_t(), C.c_size_t()
+        gpu.ok(gpu.rt.hipMemGetInfo(C.byref(now), C.byref(all_)))
+        return now.value
+
+    t, wide, allowed = 65536, 4096, 64 << 20               # wide rows in float32 would take 1 GiB
+    with capi.Readout(4, 1, 8, 8, wide) as ro:
+        before = free()
+        ro.reserve(t)
+        assert before - free() < allowed
+    with capi.Readout(4, 1, 8, wide, 8) as ro:
+        x, y, at, g = gpu.new((t, 8), np.float32), gpu.new((t, 8), np.float32), gpu.up(np.arange(t, dtype=np.int32) % 4), gpu.new(t, np.float32)
+        weights, saved = [gpu.new((4, wide, 8), np.float32)] * 4, gpu.new(ro.saved_bytes(t), np.int8)
+        before = free()
+        ro.experts(x, t, at, g, weights, y, dev_saved=saved)
+        ro.synchronize()
+        assert before - free() < allowed
+
+
 # --------------------------------------------------------------------------------------------------------------- AdamW
 
 F = np.float32
