@@ -1128,6 +1128,9 @@ int launched(pink_hip_readout *r, const char *what)
     return e == hipSuccess ? PINK_HIP_OK : fail(r, PINK_HIP_EDEVICE, what, hipGetErrorString(e));
 }
 
+// A launch has at most 2^32 - 1 threads.
+bool too_many(uint64_t blocks, uint32_t threads) { return blocks * threads > 0xffffffffu; }
+
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 size_t element_bytes(const pink_hip_readout *r) { return r->cfg.element == PINK_HIP_ELEMENT_BFLOAT ? 2 : 4; }
@@ -1299,7 +1302,7 @@ int product_of_tile(pink_hip_readout *r, ProductArgs &g, uint64_t slots)
     g.row_tiles = grad ? (g.rows + PR - 1) / PR : 0;
     const uint64_t tiles = grad ? (uint64_t)r->cfg.neurons * g.row_tiles : slots / PR + std::min<uint64_t>(r->cfg.neurons, slots);
     const uint64_t blocks = tiles * g.col_tiles;
-    REFUSE(r, blocks > 0x7fffffffu - kFillBlocks, "too many images for one call");
+    REFUSE(r, too_many(blocks + kFillBlocks, 64 * PW * QW), "too many images for one call");
     g.slots = (uint32_t)slots;
     const uint32_t more = (OP == kAnswer || OP == kBackInput) && g.place ? kFillBlocks : 0;
     k_product<E, OP, PR, QC, PW, QW, M, DEEP, DIRECT><<<(uint32_t)blocks + more, 64 * PW * QW, 0, r->stream>>>(g);
@@ -1385,7 +1388,7 @@ int combine(pink_hip_readout *r, const float *rows, const int32_t *place, uint32
             uint64_t residual_stride, void *out, uint64_t out_stride)
 {
     const uint64_t blocks = (images * (whole_rows(cols) / 4) + 255) / 256;
-    REFUSE(r, blocks > 0x7fffffffu, "too many images for one call");
+    REFUSE(r, too_many(blocks, 256), "too many images for one call");
     k_combine<E><<<(uint32_t)blocks, 256, 0, r->stream>>>(rows, place, images, r->cfg.chosen, cols, (const E *)residual, residual_stride, (E *)out, out_stride);
     return launched(r, "k_combine");
 }
@@ -1503,6 +1506,7 @@ int experts_backward(pink_hip_readout *r, const void *x, uint32_t images, uint64
         TRY((product<E, kBackHidden>(r, g, slots)));
     }
     if (out.gates) {
+        REFUSE(r, too_many(((uint64_t)slots + 3) / 4, 256), "too many images for one call");
         k_gate_gradients<E><<<(uint32_t)(((uint64_t)slots + 3) / 4), 256, 0, r->stream>>>(
             g.partial, g.col_tiles, place, (const int32_t *)(saved + s.owner), slots, c.chosen, (const E *)dy, dy_stride, c.outputs,
             (const E *)weights.second_bias, (E *)out.gates);
@@ -1567,12 +1571,15 @@ template <typename Check, typename Launch>
 int over_tensors(pink_hip_readout *r, const pink_hip_readout_tensor *tensors, uint32_t count, AdamArgs &g, const Check &ok, const Launch &launch)
 {
     for (uint32_t i = 0; i < count; ++i)
-        if (tensors[i].size) TRY(ok(tensors[i]));
+        if (tensors[i].size) {
+            TRY(ok(tensors[i]));
+            REFUSE(r, too_many((tensors[i].size + kAdamChunk - 1) / kAdamChunk, 256), "too many values in one tensor");
+        }
     uint64_t blocks = 0;
     g.count = 0;
     for (uint32_t i = 0; i <= count; ++i) {
         const uint64_t more = i < count ? (tensors[i].size + kAdamChunk - 1) / kAdamChunk : 0;
-        if (g.count && (i == count || g.count == kAdamTensors || blocks + more > 0x7fffffffu)) {
+        if (g.count && (i == count || g.count == kAdamTensors || too_many(blocks + more, 256))) {
             g.first_block[g.count] = (uint32_t)blocks;
             launch((uint32_t)blocks);
             TRY(launched(r, "k_adamw"));
@@ -1669,7 +1676,9 @@ int pink_hip_readout_route(pink_hip_readout *r, const float *distances, uint32_t
     g.neuron = neuron;
     g.gates = gates;
     const uint32_t candidates = std::max(g.neurons, g.groups_kept * g.group_size);
-    if (candidates > 2048 || (g.groups > 1 && g.groups > 64)) {
+    const bool by_block = candidates > 2048 || g.groups > 64;
+    REFUSE(r, too_many(by_block ? images : (images + 3) / 4, 256), "too many images for one call");
+    if (by_block) {
         k_route_block<<<images, 256, (g.neurons + (g.groups > 1 ? g.groups : 0)) * 4, r->stream>>>(g);
         return launched(r, "k_route_block");
     }

@@ -343,3 +343,16 @@ def test_models_of_large_maps(gpu, t, n, k, f, h, o, bf16):  # noqa: F811
         return np.where(rng.random(shape) < 0.1, -1, neuron)
 
     base.test_experts(gpu, t, n, k, f, h, o, "silu", True, True, spread, 0, bf16)
+
+
+@pytest.mark.gpu
+def test_calls_of_more_threads_than_a_launch_has(gpu):  # noqa: F811
+    buffer = gpu.new(4096, np.float32)
+    with capi.Readout(3, 1) as ro, capi.Readout(3000, 1) as large:
+        calls = [lambda: ro.route(buffer, 2 ** 28, buffer, buffer, None, buffer, buffer),
+                 lambda: large.route(buffer, 2 ** 24, buffer, buffer, None, buffer, buffer),
+                 lambda: ro.adamw(ro.tensors([dict(value=buffer, gradient=buffer, first=buffer, second=buffer, size=2 ** 36)]), 1)]
+        for call in calls:
+            with pytest.raises(capi.PinkError) as e:
+                call()
+            assert e.value.status == -1 and "too many" in str(e.value)
