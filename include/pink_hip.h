@@ -278,8 +278,10 @@ int pink_hip_make_update_factors(uint32_t layout, const uint32_t *dims, uint32_t
  */
 typedef struct pink_hip_readout pink_hip_readout;
 
-/* Element type of features, weights, answers and their gradients.  Distances, gates and the router's
- * parameters are float32 always; sums are float32 at least. */
+/* Element type of features, weights, answers and their gradients, and of the hidden values between a
+ * model's layers as they are kept: gate f(a), its gradient, and a itself (where the slope is needed, 11 bits
+ * in place of bfloat16's 8).  Handfuls of slots without a backward pass keep them in float32.  Distances,
+ * gates and the router's parameters are float32 always; sums are float32 at least. */
 typedef enum { PINK_HIP_ELEMENT_FLOAT = 0, PINK_HIP_ELEMENT_BFLOAT = 1 } pink_hip_element;
 typedef enum { PINK_HIP_SCORE_SOFTMAX = 0, PINK_HIP_SCORE_SIGMOID = 1 } pink_hip_score;
 /* GELU is the exact one (error function); SILU is a * sigmoid(a). */

@@ -127,6 +127,7 @@ __device__ __forceinline__ float gate_of(const RouteArgs &g, float z, bool valid
 
 // The general form, a block per image: keys in LDS, the groups kept by counting how many go before each, then the largest key
 // `chosen` times, each a pass over LDS.  For what k_route_wave does not take: more than 2048 neurons, or more than 64 groups.
+// 16000 images, 8 chosen: 146 us of 2500 neurons, 240 of 5000 (34 and 67 for reading them); 424 with 10 of 50 groups of 2500.
 __global__ __launch_bounds__(256) void k_route_block(const RouteArgs g)
 {
     extern __shared__ __align__(16) uint32_t lds[];
@@ -416,7 +417,8 @@ constexpr uint32_t kChunkMost = 64;
 //   renormalised: dz_c = g_c (G_c - sum_s g_s G_s) [sigmoid: times 1 - sigmoid(z_c)];  sigmoid: dz_c = G_c s (1 - s);
 //   softmax: dz_n = [n chosen] g_n G_n - share_n sum_s g_s G_s
 // Sums over images are formed a chunk at a time and then over the chunks, always in the same order.  Bound by latency at the sizes
-// of a batch: 1001 images x 331 neurons, full softmax, 9 us and 4 us for the sums over 251 chunks.
+// of a batch: 1001 images x 331 neurons, full softmax, 9 us and 4 us for the sums over 251 chunks.  16000 x 1600: 80 us, with the full
+// softmax 481 (every strip forms its images' maxima and sums anew), where reading and writing alone would take 43.
 template <typename E> __global__ __launch_bounds__(256) void k_route_backward(const RouteBackwardArgs a)
 {
     const RouteArgs &g = a.r;
@@ -520,7 +522,7 @@ __global__ __launch_bounds__(1024) void k_route_sums(const float *sharpness_part
     if (out) out[n] = sum;
 }
 
-// One block: how often each neuron was chosen, then a step of the bias against the mean.
+// One block: how often each neuron was chosen, then a step of the bias against the mean.  4004 slots 5.6 us, 64000 slots 15 us.
 __global__ __launch_bounds__(1024) void k_balance(const int32_t *neuron, uint64_t slots, uint32_t neurons, float rate, float *bias, int32_t *load)
 {
     extern __shared__ __align__(16) uint32_t counts[];
@@ -952,8 +954,8 @@ __device__ __forceinline__ float second_value(uint8_t code, float scale)
 // value's own step takes the hardware's root and reciprocal, each off by one unit at most: 2^-22 of a step.  They take subnormal
 // numbers for 0, which is as little where epsilon is 2^-38 or more (the root of a subnormal number is below 2^-63).  Below that
 // SMALL_EPSILON divides by what is rounded; so a step without a gradient is 0 at any epsilon.
-// 224 M values, bfloat16 gradients and copies, 8-bit states: 737 us for 3.6 GB (4.9 TB/s; a copy reaches 4.8); with every root
-// rounded it was 821 us and bound by the vector ALU (117 instructions a value, now 77).  44 M values, float32 states: 224 us, 5.5 TB/s.
+// 224 M values, bfloat16 gradients and copies, 8-bit states: 726 us for 3.6 GB (4.9 TB/s; a copy reaches 4.8); with every root
+// rounded it was 821 us and bound by the vector ALU (117 instructions a value, now 80).  44 M values, float32 states: 226 us, 5.4 TB/s.
 template <bool CODES, bool SMALL_EPSILON> __global__ __launch_bounds__(256) void k_adamw(const AdamArgs g)
 {
     const uint32_t which = adam_tensor(g);
@@ -1267,9 +1269,12 @@ RouteArgs route_args(const pink_hip_readout *r, const float *distances, uint32_t
 }
 
 // Rows of a product's tiles, by how many rows a neuron has on average: the weights are read once for each tile of rows, and a tile
-// that is mostly empty multiplies for nothing.  bfloat16's largest tiles halve what a CU fetches for each product; measured with 640
-// rows a neuron, 1936 x 1024: 475 us in tiles of 256 x 256 against 550 in 128 x 128; with 320 rows, 512 x 1024: 84 against 95, and
-// 102 against 99 for 1024 x 512.  Float32's products are bound by the matrix cores at either.
+// that is mostly empty multiplies for nothing.  Measured forward (us): tiles of 16 / 64 rows, bfloat16 1024 x 512 x 1024 of 100 neurons,
+// 12 rows a neuron 70 / 72, 24 rows 93 / 78; float32 2025 x 200 x 45 of 331 neurons, 12 rows 171 / 284, 24 rows 238 / 288, 36 rows 313 / 290.
+// Tiles of 64 / 128 rows, bfloat16, 36 rows 83 / 85, 64 rows 103 / 94, 96 rows 128 / 99; float32's stay ahead in 64 past that bound
+// (64 rows 377 / 638, 160 rows 728 / 941; training 1269 / 1560 and 2446 / 2544).  bfloat16's largest tiles halve what a CU fetches for
+// each product; measured with 640 rows a neuron, 1936 x 1024: 475 us in tiles of 256 x 256 against 550 in 128 x 128; with 320 rows,
+// 512 x 1024: 84 against 95, and 102 against 99 for 1024 x 512.
 uint32_t tile_rows(const pink_hip_readout *r, uint64_t slots)
 {
     const uint64_t neurons = std::min<uint64_t>(r->cfg.neurons, slots);
@@ -1315,8 +1320,10 @@ template <typename E, int OP, bool DIRECT> int product_as(pink_hip_readout *r, P
     if constexpr (OP == kGradFirst || OP == kGradSecond) {
         // Matrices of few rows (the second layer of a handful of outputs): tiles of as few.
         if (g.rows <= 32) return product_of_tile<E, OP, 32, 128, 1, 4, 32, 1, DIRECT>(r, g, slots);
-        // Few rows a neuron: writing the gradients is what there is to do, and small tiles spread it.  Large tiles (590 against 640 us
-        // for 1024 x 1936 of 100 neurons) where there are enough of them to go round.
+        // Few rows a neuron: writing the gradients is what there is to do, and small tiles spread it over more blocks.  A training step in small /
+        // large tiles (us): float32 784 x 96 x 40 of 64 neurons, 16 rows a neuron 61 / 68, 64 rows 112 / 130; where large tiles are many
+        // they are ahead at any number of rows, which the rule does not go by (bfloat16 1936 x 1024 x 256 of 100, 16 rows 467 / 441, 64 rows
+        // 612 / 583).  The largest tiles (590 against 640 us for 1024 x 1936 of 100 neurons) where there are enough of them to go round.
         if (slots <= 64 * (uint64_t)r->cfg.neurons) return product_of_tile<E, OP, 64, 64, 2, 2, 16, 1, DIRECT>(r, g, slots);
         if constexpr (half && DIRECT) {
             const uint64_t tiles = (uint64_t)r->cfg.neurons * ((g.rows + 255) / 256) * ((g.cols + 255) / 256);
