@@ -19,6 +19,7 @@ trains a small map on synthetic sources and a read-out of their size and axis ra
 import argparse
 import functools
 import math
+import types
 
 import numpy as np
 import torch
@@ -51,7 +52,8 @@ class MapReadout:
 
     The map is copied when it is made, as a pink.Mapper does: its models are trained on that map.  The first step's images set `level`,
     the scale of the features, and where sharpness and radius start; answers asked for before go by the scale of their own images.
-    What a trained read-out consists of: parameters, states, bias, level and steps.
+    What a trained read-out consists of (parameters, states, bias, level and steps) is saved by state_dict() and put back by
+    load_state_dict() of one that was made alike; its tensors can be written to but not replaced, as AdamW holds their addresses.
 
     It lives on the device that is current when it is made.  Calls run on that device's stream that is current when they are made, and
     what they return is that stream's; a call on another stream than the last one's waits for that one first, so a stream that
@@ -96,8 +98,14 @@ class MapReadout:
         self._tensors = self.readout.tensors([
             dict(value=v.data_ptr(), gradient=self.gradients[k].data_ptr(), size=v.numel(), decay=weight_decay if k in ("first", "second") else 0.0,
                  **{s: x.data_ptr() for s, x in self.states[k].items()}) for k, v in self.parameters.items()])
+        self.parameters, self.gradients = types.MappingProxyType(self.parameters), types.MappingProxyType(self.gradients)
+        self.states = types.MappingProxyType({k: types.MappingProxyType(v) for k, v in self.states.items()})
         self.bias = zeros(n)                               # for an even load; takes part in the choice of neurons only
         self.steps, self.level = 0, None                   # level: mean and spread of the distances
+
+    def _held(self):
+        return {**{"parameters." + k: v for k, v in self.parameters.items()},
+                **{"states.%s.%s" % (k, name): v for k, held in self.states.items() for name, v in held.items()}, "bias": self.bias}
 
     def _follow_stream(self):
         """What was queued for the read-out so far is complete, and the handle works on the caller's current stream."""
@@ -105,6 +113,25 @@ class MapReadout:
         if stream != self._stream:
             self.readout.set_stream(stream.cuda_stream)    # waits for the stream that it leaves, PyTorch's work there too
             self._stream = stream
+
+    @_on_its_device
+    def state_dict(self):
+        """Copies of all that a trained read-out consists of, by name: tensors, the number of steps, and the level (None before the first step)."""
+        return {**{k: v.clone() for k, v in self._held().items()}, "level": None if self.level is None else self.level.clone(), "steps": self.steps}
+
+    @_on_its_device
+    def load_state_dict(self, saved):
+        """Goes on from what state_dict() gave, of a read-out with as many neurons, hidden values and outputs and the same state_bits."""
+        held = self._held()
+        if set(saved) != set(held) | {"level", "steps"}:
+            raise pink.exception(-1, "not the state of such a read-out: " + ", ".join(sorted(set(saved) ^ (set(held) | {"level", "steps"}))))
+        wrong = [k for k, v in held.items() if saved[k].shape != v.shape or saved[k].dtype != v.dtype]
+        if wrong or (saved["level"] is not None and tuple(saved["level"].shape) != (2,)):
+            raise pink.exception(-1, "not the state of such a read-out: shape or type of " + ", ".join(wrong or ["level"]))
+        for k, v in held.items():
+            v.copy_(saved[k])
+        self.level = None if saved["level"] is None else saved["level"].to(self.device, torch.float32, copy=True)
+        self.steps = int(saved["steps"])
 
     @_on_its_device
     def distances(self, images):

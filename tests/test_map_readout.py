@@ -72,6 +72,28 @@ def test_calls_go_to_the_stream_that_is_current_when_they_are_made(made):
     assert all(at == current for _, at, current in recorder.calls)
 
 
+def test_what_the_optimiser_holds_is_not_replaced(made):
+    answers, _, torch = made
+    for held in (answers.parameters, answers.gradients, answers.states, answers.states["first"]):
+        with pytest.raises(TypeError):
+            held["first"] = torch.zeros(1)
+    answers.parameters["first"].fill_(2.0)
+
+
+def test_states_that_are_refused(made):
+    from pink_amd import pink
+    answers, _, torch = made
+    good = answers.state_dict()
+    before = {k: v.clone() for k, v in answers._held().items()}
+    for change in ({"bias": torch.zeros(7)}, {"parameters.first": good["parameters.first"].double()}, {"more": torch.zeros(1)}, {"level": torch.zeros(3)}):
+        with pytest.raises(pink.exception):
+            answers.load_state_dict({**{k: v if not torch.is_tensor(v) else v + 1 for k, v in good.items()}, **change})
+    with pytest.raises(pink.exception):
+        answers.load_state_dict({k: v for k, v in good.items() if k != "steps"})
+    assert all(torch.equal(v, before[k]) for k, v in answers._held().items()) and answers.level is None
+    answers.load_state_dict(good)
+
+
 # ------------------------------------------------------------------------------------------------------------ on a GPU
 
 def run(code):
@@ -207,3 +229,24 @@ def test_steps_that_are_refused():
     assert np.isfinite(float(one.step(images[:1], targets[:1]))) and np.isfinite(one(images[:5]).cpu().numpy()).all()       # one distance in all
     assert np.isfinite(float(answers.step(images[:64], targets[:64])))
     """)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_training_goes_on_from_what_was_saved(bits):
+    run("""
+    import os, tempfile
+    def train(answers, steps):
+        for i in steps:
+            at = slice(i %% 3 * 64, i %% 3 * 64 + 64)
+            answers.step(images[at], targets[at])
+        return state(answers) + [answers(images[:40]).cpu().numpy()]
+    one, two = made(a_map(), state_bits=%d), made(a_map(), state_bits=%d, seed=5)
+    train(one, range(4))
+    with tempfile.TemporaryDirectory() as folder:
+        torch.save(one.state_dict(), os.path.join(folder, "read-out"))
+        two.load_state_dict(torch.load(os.path.join(folder, "read-out"), weights_only=True))
+    assert two.steps == 4
+    for a, b in zip(train(one, range(4, 8)), train(two, range(4, 8))):
+        assert np.array_equal(a, b)
+    """ % (bits, bits))
