@@ -391,6 +391,73 @@ int pink_hip_readout_adamw(pink_hip_readout *readout, const pink_hip_readout_ten
 /* The values that the tensors' 8-bit states stand for, into first_values and second_values. */
 int pink_hip_readout_unpack(pink_hip_readout *readout, const pink_hip_readout_tensor *tensors, uint32_t count);
 
+/* Layer norm of rows of `width` elements (at most 2^20): y = weight (x - mean) scale + bias, scale = 1 / sqrt(variance + epsilon), the
+ * variance being the mean of (x - mean)^2.  weight and bias (`width` elements) may be NULL, y may be x.  mean and scale (a
+ * float32 each row; what the backward call needs) are left where they are not NULL. */
+int pink_hip_readout_norm(pink_hip_readout *readout, const void *dev_x, uint32_t images, uint32_t width, uint64_t x_stride,
+                          const void *dev_weight, const void *dev_bias, float epsilon, void *dev_y, uint64_t y_stride,
+                          float *dev_mean_out, float *dev_scale_out);
+/* Gradients for those of y, dy: of x, to which residual (NULL: nothing; images x width) is added, and of weight and bias, summed over the images.
+ * x, weight, mean and scale as in the forward call.  Gradients that are not wanted are NULL; dx may be dy or residual, not x. */
+int pink_hip_readout_norm_backward(pink_hip_readout *readout, const void *dev_x, uint32_t images, uint32_t width, uint64_t x_stride,
+                                   const void *dev_weight, const float *dev_mean, const float *dev_scale, const void *dev_dy, uint64_t dy_stride,
+                                   const void *dev_residual, uint64_t residual_stride, void *dev_dx_out, uint64_t dx_stride,
+                                   void *dev_weight_gradients_out, void *dev_bias_gradients_out);
+/* Grows the workspace to what calls on up to so many rows of that width need. */
+int pink_hip_readout_norm_reserve(pink_hip_readout *readout, uint32_t images, uint32_t width);
+
+/* A gated feed-forward block, one for all images: y[t] = residual[t] + down h + down_bias, h = f(gate x[t] + gate_bias) * (up x[t] + up_bias).
+ * Matrices row-major: gate and up hidden x features, down outputs x hidden; biases may be NULL.  Sizes are at least 1 and at most 2^20. */
+typedef struct pink_hip_readout_gated_config {
+    uint32_t features, hidden, outputs;
+    uint32_t activation;     /* pink_hip_activation: f */
+} pink_hip_readout_gated_config;
+typedef struct pink_hip_readout_gated_weights {
+    const void *gate, *gate_bias, *up, *up_bias, *down, *down_bias;
+} pink_hip_readout_gated_weights;
+/* Where gradients go, same shapes; features images x features.  NULL where one is not wanted. */
+typedef struct pink_hip_readout_gated_gradients {
+    void *features, *gate, *gate_bias, *up, *up_bias, *down, *down_bias;
+} pink_hip_readout_gated_gradients;
+/* residual may be NULL; y may be x or residual.  What a backward pass needs is left in `saved` (pink_hip_readout_gated_saved_bytes bytes, which
+ * is 0 for arguments that are refused; 256-byte aligned) unless it is NULL: h and the two factors of its gradient, f(a) and
+ * f'(a) times the other, rounded to the handle's element type. */
+size_t pink_hip_readout_gated_saved_bytes(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, uint32_t images);
+int pink_hip_readout_gated(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, const void *dev_x, uint32_t images,
+                           uint64_t x_stride, const pink_hip_readout_gated_weights *dev_weights, const void *dev_residual,
+                           uint64_t residual_stride, void *dev_y, uint64_t y_stride, void *dev_saved);
+/* Gradients for those of y; x and weights as in the forward call that left `saved`.  (The residual's are those of y.) */
+int pink_hip_readout_gated_backward(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, const void *dev_x, uint32_t images,
+                                    uint64_t x_stride, const pink_hip_readout_gated_weights *dev_weights, const void *dev_saved,
+                                    const void *dev_y_gradients, uint64_t y_gradient_stride,
+                                    const pink_hip_readout_gated_gradients *dev_gradients_out, uint64_t x_gradient_stride);
+/* Grows the workspace to what forward and backward calls on so many images need. */
+int pink_hip_readout_gated_reserve(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, uint32_t images);
+
+/* Losses of answers that are logits of classes, against what was kept of a teacher's logits, its largest, and against labels:
+ *    weight * (teacher_weight * temperature^2 * sum of p log(p / q) + label_weight * -log softmax(logits)[label])
+ * A class whose logit is minus infinity takes no part.  q is the softmax of logits / temperature.  A teacher's place takes part if its class does,
+ * is in [0, classes) and no earlier place's, and its logit is not minus infinity.  Without the teacher's normaliser p is the softmax of the
+ * places' logits / temperature over those that take part; with it (the logarithm of the sum over all of the teacher's classes of exp(logit /
+ * temperature)) p is exp(logit / temperature - normaliser), and what the places leave of 1 is one more term, against the
+ * sum of q over the classes without a place.  A label outside [0, classes), or of a class that takes no part, is none.  An image of weight 0
+ * has loss and gradients 0, whatever its logits; else a logit that is NaN or plus infinity gives NaN. */
+typedef struct pink_hip_readout_distil_config {
+    uint32_t classes;        /* at least 1 and at most 2^20              */
+    uint32_t places;         /* of the teacher, an image; at most 1024   */
+    float temperature;       /* of the teacher's part; larger than 0     */
+    float teacher_weight, label_weight;
+} pink_hip_readout_distil_config;
+/* losses (a float32 each) and gradients of the losses' sum (images x classes) may each be NULL; so may be the teacher's arrays where
+ * there are no places (places: images x places), normalisers, labels (no image has one) and image weights (1 each).  gradients may not
+ * lie where logits do. */
+int pink_hip_readout_distil(pink_hip_readout *readout, const pink_hip_readout_distil_config *config, const void *dev_logits, uint32_t images,
+                            uint64_t logit_stride, const int32_t *dev_teacher_class, const float *dev_teacher_logits,
+                            const float *dev_teacher_normaliser, const int32_t *dev_label, const float *dev_image_weights,
+                            float *dev_losses_out, void *dev_logit_gradients_out, uint64_t gradient_stride);
+/* Grows the workspace to what calls on up to so many images need. */
+int pink_hip_readout_distil_reserve(pink_hip_readout *readout, uint32_t images, uint32_t classes);
+
 int pink_hip_abi_version(void);
 
 #ifdef __cplusplus

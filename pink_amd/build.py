@@ -22,7 +22,7 @@ SYM_SOURCE = os.path.join(HERE, "csrc", "mfma_u8_sym.hip")
 SYM_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 # The read-out's products keep their sums in the architectural registers too: 64 to 128 a lane, which fit there, and the default
 # moves them between the two kinds in every step.
-READOUT_SOURCE = os.path.join(HERE, "csrc", "readout.hip")
+READOUT_SOURCES = [os.path.join(HERE, "csrc", name) for name in ("readout.hip", "readout_gated.hip", "readout_rows.hip")]
 OUT = os.path.join(HERE, "lib", "libpink_hip.so")
 
 HIPCC_FLAGS = [
@@ -39,9 +39,9 @@ def build(verbose=False, extra=()):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     obj_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
     objects, cmds = [], []
-    for src in SOURCES + [SYM_SOURCE, READOUT_SOURCE]:
+    for src in SOURCES + [SYM_SOURCE] + READOUT_SOURCES:
         obj = os.path.join(HERE, "lib", os.path.splitext(os.path.basename(src))[0] + ".o")
-        flags = obj_flags + (SYM_FLAGS if src in (SYM_SOURCE, READOUT_SOURCE) else [])
+        flags = obj_flags + (SYM_FLAGS if src in [SYM_SOURCE] + READOUT_SOURCES else [])
         cmds.append([hipcc] + flags + list(extra) + ["-c", src, "-o", obj])
         objects.append(obj)
     running = []

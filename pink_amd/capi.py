@@ -41,6 +41,9 @@ EXPORTS = (
     "pink_hip_readout_set_stream", "pink_hip_readout_synchronize", "pink_hip_readout_reserve", "pink_hip_readout_route",
     "pink_hip_readout_route_backward", "pink_hip_readout_balance", "pink_hip_readout_saved_bytes", "pink_hip_readout_experts",
     "pink_hip_readout_experts_backward", "pink_hip_readout_adamw", "pink_hip_readout_unpack",
+    "pink_hip_readout_norm", "pink_hip_readout_norm_backward", "pink_hip_readout_norm_reserve",
+    "pink_hip_readout_gated", "pink_hip_readout_gated_backward", "pink_hip_readout_gated_saved_bytes", "pink_hip_readout_gated_reserve",
+    "pink_hip_readout_distil", "pink_hip_readout_distil_reserve",
 )
 
 
@@ -71,6 +74,22 @@ class _Weights(C.Structure):
 
 class _Gradients(C.Structure):
     _fields_ = [(name, C.c_void_p) for name in ("features", "gates", "first", "first_bias", "second", "second_bias")]
+
+
+class _GatedConfig(C.Structure):
+    _fields_ = [(name, C.c_uint32) for name in ("features", "hidden", "outputs", "activation")]
+
+
+class _GatedWeights(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("gate", "gate_bias", "up", "up_bias", "down", "down_bias")]
+
+
+class _GatedGradients(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("features", "gate", "gate_bias", "up", "up_bias", "down", "down_bias")]
+
+
+class _DistilConfig(C.Structure):
+    _fields_ = [("classes", C.c_uint32), ("places", C.c_uint32), ("temperature", C.c_float), ("teacher_weight", C.c_float), ("label_weight", C.c_float)]
 
 
 class ReadoutTensor(C.Structure):
@@ -153,6 +172,16 @@ def lib():
         L.pink_hip_readout_saved_bytes.restype = C.c_size_t
         L.pink_hip_readout_experts.argtypes = [vp, vp, u32, u64, vp, vp, C.POINTER(_Weights), vp, u64, vp, u64, vp]
         L.pink_hip_readout_experts_backward.argtypes = [vp, vp, u32, u64, vp, C.POINTER(_Weights), vp, vp, u64, C.POINTER(_Gradients), u64]
+        L.pink_hip_readout_norm.argtypes = [vp, vp, u32, u32, u64, vp, vp, C.c_float, vp, u64, vp, vp]
+        L.pink_hip_readout_norm_backward.argtypes = [vp, vp, u32, u32, u64, vp, vp, vp, vp, u64, vp, u64, vp, u64, vp, vp]
+        L.pink_hip_readout_norm_reserve.argtypes = [vp, u32, u32]
+        L.pink_hip_readout_gated_saved_bytes.argtypes = [vp, vp, u32]
+        L.pink_hip_readout_gated_saved_bytes.restype = C.c_size_t
+        L.pink_hip_readout_gated_reserve.argtypes = [vp, vp, u32]
+        L.pink_hip_readout_gated.argtypes = [vp, vp, vp, u32, u64, vp, vp, u64, vp, u64, vp]
+        L.pink_hip_readout_gated_backward.argtypes = [vp, vp, vp, u32, u64, vp, vp, vp, u64, vp, u64]
+        L.pink_hip_readout_distil.argtypes = [vp, vp, vp, u32, u64, vp, vp, vp, vp, vp, vp, vp, u64]
+        L.pink_hip_readout_distil_reserve.argtypes = [vp, u32, u32]
         L.pink_hip_readout_adamw.argtypes = [vp, C.POINTER(ReadoutTensor), u32, u32, u64, f32, f32, f32, f32]
         L.pink_hip_readout_unpack.argtypes = [vp, C.POINTER(ReadoutTensor), u32]
         _lib = L
@@ -509,3 +538,53 @@ class Readout:
     def adamw_unpack(self, tensors):
         """The values of 8-bit states, into first_values and second_values."""
         self._check(self._L.pink_hip_readout_unpack(self._h, tensors, len(tensors)))
+
+    def norm(self, dev_x, images, width, dev_weight, dev_bias, epsilon, dev_y, dev_mean=None, dev_scale=None, x_stride=0, y_stride=0):
+        """Layer norm; dev_mean and dev_scale receive what norm_backward() needs."""
+        self._check(self._L.pink_hip_readout_norm(self._h, dev_x, images, width, x_stride, dev_weight, dev_bias, epsilon, dev_y, y_stride,
+                                                  dev_mean, dev_scale))
+
+    def norm_backward(self, dev_x, images, width, dev_weight, dev_mean, dev_scale, dev_dy, dev_dx=None, dev_weight_gradients=None,
+                      dev_bias_gradients=None, dev_residual=None, x_stride=0, dy_stride=0, residual_stride=0, dx_stride=0):
+        """Gradients of x (with `dev_residual` added), of the weight and of the bias; those that are not wanted are None."""
+        self._check(self._L.pink_hip_readout_norm_backward(
+            self._h, dev_x, images, width, x_stride, dev_weight, dev_mean, dev_scale, dev_dy, dy_stride, dev_residual, residual_stride, dev_dx,
+            dx_stride, dev_weight_gradients, dev_bias_gradients))
+
+    def norm_reserve(self, images, width):
+        """Grows the workspace to what norm() and norm_backward() on up to so many rows need, so that neither allocates."""
+        self._check(self._L.pink_hip_readout_norm_reserve(self._h, images, width))
+
+    def gated_saved_bytes(self, shape, images):
+        """Size of the buffer in which gated() leaves what gated_backward() needs.  `shape`: features, hidden, outputs and the activation."""
+        return int(self._L.pink_hip_readout_gated_saved_bytes(self._h, C.byref(_GatedConfig(*shape)), images))
+
+    def gated_reserve(self, shape, images):
+        """Grows the workspace to what gated() and gated_backward() on so many images need."""
+        self._check(self._L.pink_hip_readout_gated_reserve(self._h, C.byref(_GatedConfig(*shape)), images))
+
+    def gated(self, shape, dev_x, images, weights, dev_y, dev_residual=None, dev_saved=None, x_stride=0, residual_stride=0, y_stride=0):
+        """The gated feed-forward block.  `shape`: features, hidden, outputs and the activation; `weights`: pointers to gate, gate_bias,
+        up, up_bias, down and down_bias."""
+        c, w = _GatedConfig(*shape), _GatedWeights(*weights)
+        self._check(self._L.pink_hip_readout_gated(self._h, C.byref(c), dev_x, images, x_stride, C.byref(w), dev_residual, residual_stride, dev_y,
+                                                   y_stride, dev_saved))
+
+    def gated_backward(self, shape, dev_x, images, weights, dev_saved, dev_y_gradients, gradients, x_stride=0, y_gradient_stride=0,
+                       x_gradient_stride=0):
+        """`gradients`: pointers to where those of the features and of the weights, in their order, go; None where one is not wanted."""
+        c, w, g = _GatedConfig(*shape), _GatedWeights(*weights), _GatedGradients(*gradients)
+        self._check(self._L.pink_hip_readout_gated_backward(self._h, C.byref(c), dev_x, images, x_stride, C.byref(w), dev_saved, dev_y_gradients,
+                                                            y_gradient_stride, C.byref(g), x_gradient_stride))
+
+    def distil(self, dev_logits, images, classes, dev_losses, dev_gradients=None, dev_teacher_class=None, dev_teacher_logits=None, places=0,
+               dev_teacher_normaliser=None, dev_label=None, dev_image_weights=None, temperature=1.0, teacher_weight=1.0, label_weight=0.0,
+               logit_stride=0, gradient_stride=0):
+        """Losses against a teacher's largest logits and against labels, and the gradients of the losses' sum."""
+        c = _DistilConfig(classes, places, temperature, teacher_weight, label_weight)
+        self._check(self._L.pink_hip_readout_distil(self._h, C.byref(c), dev_logits, images, logit_stride, dev_teacher_class, dev_teacher_logits,
+                                                    dev_teacher_normaliser, dev_label, dev_image_weights, dev_losses, dev_gradients, gradient_stride))
+
+    def distil_reserve(self, images, classes):
+        """Grows the workspace to what distil() of up to so many images needs."""
+        self._check(self._L.pink_hip_readout_distil_reserve(self._h, images, classes))

@@ -1,0 +1,351 @@
+// readout_gated.hip -- the gated feed-forward block of the read-out (pink_hip_readout_gated* of include/pink_hip.h), forward and backward.
+#include "readout_handle.h"
+
+#include <type_traits>
+
+#include "readout_tile.inc"
+#include "readout_gated.inc"
+
+namespace {
+
+typedef pink_hip_readout_gated_config Shape;
+
+struct GatedLayout {
+    uint64_t stride;               // elements between rows of hidden values: whole 16-byte chunks
+    size_t row_bytes;              // of one such matrix
+};
+
+GatedLayout gated_layout(const pink_hip_readout *r, const Shape &c, uint64_t images)
+{
+    const uint64_t per = 16 / element_bytes(r);
+    GatedLayout l;
+    l.stride = (c.hidden + per - 1) / per * per;
+    l.row_bytes = align256(images * l.stride * element_bytes(r));
+    return l;
+}
+
+constexpr uint32_t kLeastM = 16, kSumRows = 512;
+
+size_t parts_bytes(uint64_t count, uint32_t cols) { return align256((count + kSumRows - 1) / kSumRows * cols * 4); }
+
+// Of a call's workspace.  Backward: gradients of both hidden values, sums of them down runs of rows, shares of those, and of the
+// products' depth.
+struct GatedWork {
+    size_t hidden, partial, parts, shares, bytes;
+};
+
+constexpr uint64_t kSplitTiles = 256;                      // tiles that fill the card: fewer of them are split along the depth
+
+struct Split {
+    uint32_t splits, each;
+};
+
+// A product of few results over a long depth is cut into runs of 512 at least, whose sums are float32 and joined afterwards.
+template <int PR, int QC> Split split_of(uint32_t rows, uint32_t cols, uint32_t depth)
+{
+    const uint64_t tiles = (uint64_t)((rows + PR - 1) / PR) * ((cols + QC - 1) / QC);
+    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(kSplitTiles / tiles, depth / 512));
+    const uint32_t each = (uint32_t)(((depth + splits - 1) / splits + 127) / 128 * 128);
+    return {(depth + each - 1) / each, each};
+}
+
+size_t shares_bytes(uint32_t rows, uint32_t cols, uint32_t depth)
+{
+    const Split s = split_of<64, 64>(rows, cols, depth);
+    return s.splits > 1 ? align256((size_t)s.splits * rows * cols * 4) : 0;
+}
+
+GatedWork gated_work(const pink_hip_readout *r, const Shape &c, uint64_t images, bool backward)
+{
+    const GatedLayout l = gated_layout(r, c, images);
+    GatedWork w = {};
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += align256(bytes);
+        return here;
+    };
+    w.hidden = take(l.row_bytes * (backward ? 2 : 1));
+    if (backward) {
+        const uint64_t runs = (images + 255) / 256 * (256 / kLeastM);
+        w.partial = take(runs * 2 * l.stride * 4);
+        w.parts = take(std::max(parts_bytes(runs, (uint32_t)(2 * l.stride)), parts_bytes(images, c.outputs)));
+        w.shares = take(std::max(shares_bytes((uint32_t)(2 * l.stride), c.features, (uint32_t)images), shares_bytes(c.outputs, c.hidden, (uint32_t)images)));
+    }
+    w.bytes = at;
+    return w;
+}
+
+template <typename E, int OP> bool is_direct(const DenseArgs &g)
+{
+    constexpr uint32_t per = 16 / sizeof(E);
+    const auto whole = [](const void *at, uint64_t stride) { return ((uintptr_t)at & 15) == 0 && stride % per == 0; };
+    bool direct = whole(g.p, g.p_stride) && whole(g.q, g.q_stride) && (!g.q2 || whole(g.q2, g.q_stride));
+    if (OP == kGate || OP == kDown || OP == kBackGate) direct = direct && g.depth % per == 0;
+    if (OP == kBackGate || OP == kBackInput || OP == kGradGate) direct = direct && g.cols % per == 0;
+    if (OP == kGradDown) direct = direct && g.rows % per == 0;
+    return direct;
+}
+
+template <typename E, int OP, int PR, int QC, int PW, int QW, int KW, int M, int DEEP, bool DIRECT>
+int dense_of_tile(pink_hip_readout *r, DenseArgs &g, uint32_t *runs)
+{
+    constexpr uint32_t cols_of_tile = OP == kGate ? QC / 2 : QC;
+    const uint32_t over = OP == kGate ? (uint32_t)g.out_stride : OP == kBackGate ? g.half : g.cols;      // (padding is written too)
+    g.row_tiles = (g.rows + PR - 1) / PR;
+    g.col_tiles = (over + cols_of_tile - 1) / cols_of_tile;
+    if (runs) *runs = g.row_tiles * (PR / M);
+    const uint64_t blocks = (uint64_t)g.row_tiles * g.col_tiles * g.splits;
+    REFUSE(r, too_many(blocks, 64 * PW * QW * KW), "too many images for one call");
+    k_dense<E, OP, PR, QC, PW, QW, KW, M, DEEP, DIRECT><<<(uint32_t)blocks, 64 * PW * QW * KW, 0, r->stream>>>(g);
+    return launched(r, "k_dense");
+}
+
+template <typename E, int OP, bool DIRECT> int dense_as(pink_hip_readout *r, DenseArgs &g, uint32_t *runs)
+{
+    const auto tiles = [&](uint32_t pr, uint32_t qc) { return (uint64_t)((g.rows + pr - 1) / pr) * ((g.cols * (OP == kGate ? 2ull : 1ull) + qc - 1) / qc); };
+    if (g.splits > 1) return dense_of_tile<E, OP, 64, 64, 1, 1, 4, 32, 2, DIRECT>(r, g, runs);
+    if (g.rows <= 16) return dense_of_tile<E, OP, 16, 32, 1, 1, 4, 16, 4, DIRECT>(r, g, runs);
+    if constexpr (sizeof(E) == 2 && DIRECT)
+        if (tiles(256, 256) >= 192) return dense_of_tile<E, OP, 256, 256, 2, 4, 1, 32, 1, DIRECT>(r, g, runs);
+    if (tiles(128, 128) >= 192) return dense_of_tile<E, OP, 128, 128, 2, 2, 1, 32, 1, DIRECT>(r, g, runs);
+    if (tiles(64, 64) >= 128) return dense_of_tile<E, OP, 64, 64, 1, 1, 4, 32, 2, DIRECT>(r, g, runs);
+    return dense_of_tile<E, OP, 32, 32, 1, 1, 4, 16, 4, DIRECT>(r, g, runs);
+}
+
+template <typename E, int OP> int dense(pink_hip_readout *r, DenseArgs &g, uint32_t *runs = nullptr)
+{
+    g.splits = 1;
+    g.depth_each = g.depth;
+    if constexpr (OP == kGradGate || OP == kGradDown) {
+        const Split s = split_of<64, 64>(g.rows, g.cols, g.depth);
+        g.splits = s.splits;
+        g.depth_each = s.each;
+        if (s.splits == 1) g.shares = nullptr;
+    }
+    TRY((is_direct<E, OP>(g) ? dense_as<E, OP, true>(r, g, runs) : dense_as<E, OP, false>(r, g, runs)));
+    if (g.splits == 1) return PINK_HIP_OK;
+    const uint64_t blocks = ((uint64_t)g.rows * g.cols + 255) / 256;
+    REFUSE(r, too_many(blocks, 256), "too many images for one call");
+    k_join<E><<<(uint32_t)blocks, 256, 0, r->stream>>>(g.shares, g.splits, g.rows, g.cols, nullptr, nullptr, 0, (E *)g.out, (E *)g.out2, g.out_stride, g.half,
+                                                       g.hidden);
+    return launched(r, "k_join");
+}
+
+// Sums by column over `count` rows, by way of shares of 512 rows each where there are more.
+template <typename V, typename E>
+int sum_columns(pink_hip_readout *r, const V *rows, uint64_t stride, uint32_t count, uint32_t cols, float *parts, void *out, void *out2, uint32_t half, uint32_t hidden)
+{
+    const uint32_t blocks = (cols + 63) / 64, shares = (count + kSumRows - 1) / kSumRows;
+    if (shares <= 1) {
+        k_sum_parts<V, E><<<blocks, 1024, 0, r->stream>>>(rows, stride, count, count, cols, nullptr, (E *)out, (E *)out2, half, hidden);
+        return launched(r, "k_sum_parts");
+    }
+    REFUSE(r, shares > 65535, "too many images for one call");
+    k_sum_parts<V, E><<<dim3(blocks, shares), 1024, 0, r->stream>>>(rows, stride, count, kSumRows, cols, parts, nullptr, nullptr, 0, 0);
+    TRY(launched(r, "k_sum_parts"));
+    k_sum_parts<float, E><<<blocks, 1024, 0, r->stream>>>(parts, cols, shares, shares, cols, nullptr, (E *)out, (E *)out2, half, hidden);
+    return launched(r, "k_sum_parts");
+}
+
+template <typename E>
+int gated(pink_hip_readout *r, const Shape &c, const void *x, uint32_t images, uint64_t x_stride, const pink_hip_readout_gated_weights &weights,
+          const void *residual, uint64_t residual_stride, void *y, uint64_t y_stride, void *keep)
+{
+    const GatedLayout l = gated_layout(r, c, images);
+    if (!keep) TRY(grow(r, gated_work(r, c, images, false).bytes));
+    char *const saved = keep ? (char *)keep : (char *)r->work;
+    DenseArgs g = {};
+    g.activation = c.activation;
+    g.rows = images;
+    g.p = x;
+    g.p_stride = x_stride;
+    g.q = weights.gate;
+    g.q2 = weights.up;
+    g.q_stride = c.features;
+    g.cols = c.hidden;
+    g.depth = c.features;
+    g.bias = weights.gate_bias;
+    g.bias2 = weights.up_bias;
+    g.out = saved;
+    g.out2 = keep ? saved + l.row_bytes : nullptr;
+    g.out3 = keep ? saved + 2 * l.row_bytes : nullptr;
+    g.out_stride = l.stride;
+    TRY((dense<E, kGate>(r, g)));
+    g.p = saved;
+    g.p_stride = l.stride;
+    g.q = weights.down;
+    g.q2 = nullptr;
+    g.q_stride = c.hidden;
+    g.cols = c.outputs;
+    g.depth = c.hidden;
+    g.bias = weights.down_bias;
+    g.residual = residual;
+    g.residual_stride = residual_stride;
+    g.out = y;
+    g.out2 = g.out3 = nullptr;
+    g.out_stride = y_stride;
+    return dense<E, kDown>(r, g);
+}
+
+template <typename E>
+int gated_backward(pink_hip_readout *r, const Shape &c, const void *x, uint32_t images, uint64_t x_stride, const pink_hip_readout_gated_weights &weights,
+                   const void *keep, const void *dy, uint64_t dy_stride, const pink_hip_readout_gated_gradients &out, uint64_t dx_stride)
+{
+    const GatedLayout l = gated_layout(r, c, images);
+    const GatedWork w = gated_work(r, c, images, true);
+    TRY(grow(r, w.bytes));
+    char *const work = (char *)r->work;
+    const char *const saved = (const char *)keep;
+    const uint32_t half = (uint32_t)l.stride;
+    const bool biases = out.gate_bias || out.up_bias, matrices = out.gate || out.up;
+    if (out.features || matrices || biases) {
+        DenseArgs g = {};
+        g.rows = images;
+        g.p = dy;
+        g.p_stride = dy_stride;
+        g.q = weights.down;
+        g.q_stride = c.hidden;
+        g.cols = c.hidden;
+        g.depth = c.outputs;
+        g.half = half;
+        g.hidden = c.hidden;
+        g.value = saved + l.row_bytes;
+        g.slope = saved + 2 * l.row_bytes;
+        g.out = work + w.hidden;
+        g.out_stride = 2 * l.stride;
+        g.partial = biases ? (float *)(work + w.partial) : nullptr;
+        uint32_t runs = 0;
+        TRY((dense<E, kBackGate>(r, g, &runs)));
+        if (biases)
+            TRY((sum_columns<float, E>(r, g.partial, 2 * l.stride, runs, 2 * half, (float *)(work + w.parts), out.gate_bias, out.up_bias, half, c.hidden)));
+    }
+    if (out.features) {
+        DenseArgs g = {};
+        g.rows = images;
+        g.p = work + w.hidden;
+        g.p_stride = 2 * l.stride;
+        g.q = weights.gate;
+        g.q2 = weights.up;
+        g.q_stride = c.features;
+        g.cols = c.features;
+        g.depth = 2 * half;
+        g.half = half;
+        g.hidden = c.hidden;
+        g.out = out.features;
+        g.out_stride = dx_stride;
+        TRY((dense<E, kBackInput>(r, g)));
+    }
+    if (matrices) {
+        DenseArgs g = {};
+        g.rows = 2 * half;
+        g.p = work + w.hidden;
+        g.p_stride = 2 * l.stride;
+        g.q = x;
+        g.q_stride = x_stride;
+        g.cols = c.features;
+        g.depth = images;
+        g.half = half;
+        g.hidden = c.hidden;
+        g.out = out.gate;
+        g.out2 = out.up;
+        g.out_stride = c.features;
+        g.shares = (float *)(work + w.shares);
+        TRY((dense<E, kGradGate>(r, g)));
+    }
+    if (out.down) {
+        DenseArgs g = {};
+        g.rows = c.outputs;
+        g.p = dy;
+        g.p_stride = dy_stride;
+        g.q = saved;
+        g.q_stride = l.stride;
+        g.cols = c.hidden;
+        g.depth = images;
+        g.out = out.down;
+        g.out_stride = c.hidden;
+        g.shares = (float *)(work + w.shares);
+        TRY((dense<E, kGradDown>(r, g)));
+    }
+    if (out.down_bias)
+        TRY((sum_columns<E, E>(r, (const E *)dy, dy_stride, images, c.outputs, (float *)(work + w.parts), out.down_bias, nullptr, 0, 0)));
+    return PINK_HIP_OK;
+}
+
+int check_shape(pink_hip_readout *r, const Shape *c, uint32_t images)
+{
+    REFUSE(r, !c, "pink_hip_readout_gated: null argument");
+    REFUSE(r, !c->features || !c->hidden || !c->outputs || c->features > kMaxSize || c->hidden > kMaxSize || c->outputs > kMaxSize,
+           "pink_hip_readout_gated: features, hidden and outputs must be between 1 and 1048576");
+    REFUSE(r, c->activation > PINK_HIP_SILU, "unknown activation");
+    REFUSE(r, images > 0x7fffff00u, "too many images for one call");
+    return PINK_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pink_hip_readout_gated_saved_bytes(pink_hip_readout *r, const pink_hip_readout_gated_config *c, uint32_t images)
+{
+    return !r || check_shape(r, c, images) != PINK_HIP_OK ? 0 : 3 * gated_layout(r, *c, images).row_bytes;
+}
+
+int pink_hip_readout_gated_reserve(pink_hip_readout *r, const pink_hip_readout_gated_config *c, uint32_t images)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    TRY(check_shape(r, c, images));
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    return grow(r, gated_work(r, *c, images, true).bytes);
+}
+
+int pink_hip_readout_gated(pink_hip_readout *r, const pink_hip_readout_gated_config *c, const void *x, uint32_t images, uint64_t x_stride,
+                           const pink_hip_readout_gated_weights *weights, const void *residual, uint64_t residual_stride, void *y, uint64_t y_stride,
+                           void *saved)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    TRY(check_shape(r, c, images));
+    x_stride = x_stride ? x_stride : c->features;
+    y_stride = y_stride ? y_stride : c->outputs;
+    residual_stride = residual_stride ? residual_stride : c->outputs;
+    REFUSE(r, x_stride < c->features || y_stride < c->outputs || residual_stride < c->outputs, "pink_hip_readout_gated: rows overlap");
+    REFUSE(r, (uintptr_t)saved & 255, "pink_hip_readout_gated: saved must be aligned to 256 bytes");
+    if (images == 0) return PINK_HIP_OK;
+    REFUSE(r, !x || !weights || !weights->gate || !weights->up || !weights->down || !y, "pink_hip_readout_gated: null argument");
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    if (r->cfg.element == PINK_HIP_ELEMENT_BFLOAT) return gated<Bfloat>(r, *c, x, images, x_stride, *weights, residual, residual_stride, y, y_stride, saved);
+    return gated<float>(r, *c, x, images, x_stride, *weights, residual, residual_stride, y, y_stride, saved);
+}
+
+int pink_hip_readout_gated_backward(pink_hip_readout *r, const pink_hip_readout_gated_config *c, const void *x, uint32_t images, uint64_t x_stride,
+                                    const pink_hip_readout_gated_weights *weights, const void *saved, const void *dy, uint64_t dy_stride,
+                                    const pink_hip_readout_gated_gradients *out, uint64_t dx_stride)
+{
+    if (!r) return PINK_HIP_EINVAL;
+    TRY(check_shape(r, c, images));
+    x_stride = x_stride ? x_stride : c->features;
+    dx_stride = dx_stride ? dx_stride : c->features;
+    dy_stride = dy_stride ? dy_stride : c->outputs;
+    REFUSE(r, x_stride < c->features || dx_stride < c->features || dy_stride < c->outputs, "pink_hip_readout_gated_backward: rows overlap");
+    REFUSE(r, (uintptr_t)saved & 255, "pink_hip_readout_gated_backward: saved must be aligned to 256 bytes");
+    REFUSE(r, !out, "pink_hip_readout_gated_backward: null argument");
+    HIP_TRY(r, hipSetDevice(r->cfg.device));
+    if (images == 0) {                                     // sums over nothing
+        const size_t e = element_bytes(r);
+        const auto clear = [&](void *at, uint64_t n) {
+            if (at) k_clear<<<1024, 256, 0, r->stream>>>((uint8_t *)at, n * e);
+        };
+        clear(out->gate, (uint64_t)c->hidden * c->features);
+        clear(out->gate_bias, c->hidden);
+        clear(out->up, (uint64_t)c->hidden * c->features);
+        clear(out->up_bias, c->hidden);
+        clear(out->down, (uint64_t)c->outputs * c->hidden);
+        clear(out->down_bias, c->outputs);
+        return launched(r, "k_clear");
+    }
+    REFUSE(r, !x || !weights || !weights->gate || !weights->up || !weights->down || !saved || !dy, "pink_hip_readout_gated_backward: null argument");
+    if (r->cfg.element == PINK_HIP_ELEMENT_BFLOAT) return gated_backward<Bfloat>(r, *c, x, images, x_stride, *weights, saved, dy, dy_stride, *out, dx_stride);
+    return gated_backward<float>(r, *c, x, images, x_stride, *weights, saved, dy, dy_stride, *out, dx_stride);
+}
+
+}  // extern "C"
