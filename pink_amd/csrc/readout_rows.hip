@@ -54,7 +54,8 @@ int pink_hip_readout_norm_reserve(pink_hip_readout *r, uint32_t images, uint32_t
     REFUSE(r, width == 0 || width > kMaxSize, "pink_hip_readout_norm: width must be between 1 and 1048576");
     REFUSE(r, images > kMaxRows, "too many images for one call");
     HIP_TRY(r, hipSetDevice(r->cfg.device));
-    return grow(r, (size_t)norm_parts(kMaxRows, width) * 2 * width * 4);
+    // (no more rows have fewer parts than images or kNormFew, whose rows are a block's)
+    return grow(r, (size_t)std::max(norm_parts(images, width), norm_parts(std::min(images, kNormFew), width)) * 2 * width * 4);
 }
 
 int pink_hip_readout_norm_backward(pink_hip_readout *r, const void *x, uint32_t images, uint32_t width, uint64_t x_stride,
