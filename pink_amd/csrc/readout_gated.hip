@@ -101,13 +101,32 @@ int dense_of_tile(pink_hip_readout *r, DenseArgs &g, uint32_t *runs)
     return launched(r, "k_dense");
 }
 
+// k_dense_large's offsets within a tile have 31 bits, and a stage of kBackInput is of one matrix.
+template <int OP> bool is_large(const DenseArgs &g)
+{
+    const uint64_t lines_p = OP == kGradGate || OP == kGradDown ? 64 : 256, lines_q = OP == kGate || OP == kDown ? 256 : 64;
+    return (lines_p * g.p_stride + 256) * 2 < 0x80000000u && (lines_q * g.q_stride + 256) * 2 < 0x80000000u && (OP != kBackInput || g.half % 64 == 0);
+}
+
+template <int OP> int dense_large(pink_hip_readout *r, DenseArgs &g, uint32_t *runs)
+{
+    const uint32_t over = OP == kGate ? (uint32_t)g.out_stride : OP == kBackGate ? g.half : g.cols;      // (padding is written too)
+    g.row_tiles = (g.rows + 255) / 256;
+    g.col_tiles = (over + (OP == kGate ? 127 : 255)) / (OP == kGate ? 128 : 256);
+    if (runs) *runs = g.row_tiles * (256 / 32);
+    const uint64_t blocks = (uint64_t)g.row_tiles * g.col_tiles;
+    REFUSE(r, too_many(blocks, 512), "too many images for one call");
+    k_dense_large<OP><<<(uint32_t)blocks, 512, 0, r->stream>>>(g);
+    return launched(r, "k_dense_large");
+}
+
 template <typename E, int OP, bool DIRECT> int dense_as(pink_hip_readout *r, DenseArgs &g, uint32_t *runs)
 {
     const auto tiles = [&](uint32_t pr, uint32_t qc) { return (uint64_t)((g.rows + pr - 1) / pr) * ((g.cols * (OP == kGate ? 2ull : 1ull) + qc - 1) / qc); };
     if (g.splits > 1) return dense_of_tile<E, OP, 64, 64, 1, 1, 4, 32, 2, DIRECT>(r, g, runs);
     if (g.rows <= 16) return dense_of_tile<E, OP, 16, 32, 1, 1, 4, 16, 4, DIRECT>(r, g, runs);
     if constexpr (sizeof(E) == 2 && DIRECT)
-        if (tiles(256, 256) >= 192) return dense_of_tile<E, OP, 256, 256, 2, 4, 1, 32, 1, DIRECT>(r, g, runs);
+        if (tiles(256, 256) >= 192 && is_large<OP>(g)) return dense_large<OP>(r, g, runs);
     if (tiles(128, 128) >= 192) return dense_of_tile<E, OP, 128, 128, 2, 2, 1, 32, 1, DIRECT>(r, g, runs);
     if (tiles(64, 64) >= 128) return dense_of_tile<E, OP, 64, 64, 1, 1, 4, 32, 2, DIRECT>(r, g, runs);
     return dense_of_tile<E, OP, 32, 32, 1, 1, 4, 16, 4, DIRECT>(r, g, runs);
