@@ -114,9 +114,9 @@ template <int OP> int dense_large(pink_hip_readout *r, DenseArgs &g, uint32_t *r
     g.row_tiles = (g.rows + 255) / 256;
     g.col_tiles = (over + (OP == kGate ? 127 : 255)) / (OP == kGate ? 128 : 256);
     if (runs) *runs = g.row_tiles * (256 / 32);
-    const uint64_t blocks = (uint64_t)g.row_tiles * g.col_tiles;
-    REFUSE(r, too_many(blocks, 512), "too many images for one call");
-    k_dense_large<OP><<<(uint32_t)blocks, 512, 0, r->stream>>>(g);
+    const uint64_t tiles = (uint64_t)g.row_tiles * g.col_tiles;
+    REFUSE(r, tiles > 0xffffffffu, "too many images for one call");
+    k_dense_large<OP><<<(uint32_t)std::min<uint64_t>(tiles, 256), 512, 0, r->stream>>>(g);              // one a CU
     return launched(r, "k_dense_large");
 }
 
