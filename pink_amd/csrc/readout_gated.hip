@@ -189,6 +189,7 @@ int gated(pink_hip_readout *r, const Shape &c, const void *x, uint32_t images, u
     g.out = saved;
     g.out2 = keep ? saved + l.row_bytes : nullptr;
     g.out3 = keep ? saved + 2 * l.row_bytes : nullptr;
+    g.lower = (uint16_t *)(saved + 3 * l.row_bytes);       // (bfloat16)
     g.out_stride = l.stride;
     TRY((dense<E, kGate>(r, g)));
     g.p = saved;
@@ -231,6 +232,7 @@ int gated_backward(pink_hip_readout *r, const Shape &c, const void *x, uint32_t 
         g.hidden = c.hidden;
         g.value = saved + l.row_bytes;
         g.slope = saved + 2 * l.row_bytes;
+        g.value_lower = (const uint16_t *)(saved + 3 * l.row_bytes);
         g.out = work + w.hidden;
         g.out_stride = 2 * l.stride;
         g.partial = biases ? (float *)(work + w.partial) : nullptr;
@@ -307,7 +309,7 @@ extern "C" {
 
 size_t pink_hip_readout_gated_saved_bytes(pink_hip_readout *r, const pink_hip_readout_gated_config *c, uint32_t images)
 {
-    return !r || check_shape(r, c, images) != PINK_HIP_OK ? 0 : 3 * gated_layout(r, *c, images).row_bytes;
+    return !r || check_shape(r, c, images) != PINK_HIP_OK ? 0 : (element_bytes(r) == 2 ? 4 : 3) * gated_layout(r, *c, images).row_bytes;
 }
 
 int pink_hip_readout_gated_reserve(pink_hip_readout *r, const pink_hip_readout_gated_config *c, uint32_t images)
