@@ -34,6 +34,8 @@ struct GatedWork {
     size_t hidden, partial, parts, shares, bytes;
 };
 
+constexpr uint32_t kFewRows = 32;
+
 constexpr uint64_t kSplitTiles = 256;                      // tiles that fill the card: fewer of them are split along the depth
 
 struct Split {
@@ -136,6 +138,14 @@ template <typename E, int OP> int dense(pink_hip_readout *r, DenseArgs &g, uint3
 {
     g.splits = 1;
     g.depth_each = g.depth;
+    if constexpr (OP == kGate || OP == kDown) {
+        if (g.rows <= kFewRows && !g.out2) {
+            const uint32_t blocks = (uint32_t)(((OP == kGate ? g.out_stride : g.cols) + 15) / 16);
+            if (g.rows <= 16) k_few<E, OP, 1, 8><<<blocks, 512, 0, r->stream>>>(g);
+            else k_few<E, OP, 2, 8><<<blocks, 512, 0, r->stream>>>(g);
+            return launched(r, "k_few");
+        }
+    }
     if constexpr (OP == kGradGate || OP == kGradDown) {
         const Split s = split_of<64, 64>(g.rows, g.cols, g.depth);
         g.splits = s.splits;
