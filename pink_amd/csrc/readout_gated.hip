@@ -36,26 +36,30 @@ struct GatedWork {
 
 constexpr uint32_t kFewRows = 32;
 
-constexpr uint64_t kSplitTiles = 256;                      // tiles that fill the card: fewer of them are split along the depth
-
 struct Split {
     uint32_t splits, each;
 };
 
-// A product of few results over a long depth is cut into runs of 512 at least, whose sums are float32 and joined afterwards.
-template <int PR, int QC> Split split_of(uint32_t rows, uint32_t cols, uint32_t depth)
+constexpr uint32_t kFullTiles = 160, kSplitTiles = 256;    // tiles of 64 x 64: that nearly fill the card; that a product is split into
+
+// A product of few results over a long axis is cut into runs, whose sums are float32 and joined afterwards by a launch of its own (4 to 5 us).
+// Runs are 512 long at least where they are sums over rows, 1024 where they are not, whose other forms for few tiles are faster.  Measured (us, whole /
+// split): 64 rows, bfloat16, kBackInput of 4096 hidden values, 1024 columns 33 / 14; 2000 rows, kGradDown of 784 x 512 float32 30 / 24.
+Split split_of(uint32_t rows, uint32_t cols, uint32_t depth, uint32_t least)
 {
-    const uint64_t tiles = (uint64_t)((rows + PR - 1) / PR) * ((cols + QC - 1) / QC);
-    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(kSplitTiles / tiles, depth / 512));
+    const uint64_t tiles = (uint64_t)((rows + 63) / 64) * ((cols + 63) / 64);
+    const uint64_t splits = tiles >= kFullTiles ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(kSplitTiles / tiles, depth / least));
     const uint32_t each = (uint32_t)(((depth + splits - 1) / splits + 127) / 128 * 128);
     return {(depth + each - 1) / each, each};
 }
 
-size_t shares_bytes(uint32_t rows, uint32_t cols, uint32_t depth)
+size_t shares_bytes(uint32_t rows, uint32_t cols, uint32_t depth, uint32_t least)
 {
-    const Split s = split_of<64, 64>(rows, cols, depth);
+    const Split s = split_of(rows, cols, depth, least);
     return s.splits > 1 ? align256((size_t)s.splits * rows * cols * 4) : 0;
 }
+
+template <int OP> constexpr uint32_t kLeastRun = OP == kGradGate || OP == kGradDown ? 512 : 1024;
 
 GatedWork gated_work(const pink_hip_readout *r, const Shape &c, uint64_t images, bool backward)
 {
@@ -68,12 +72,16 @@ GatedWork gated_work(const pink_hip_readout *r, const Shape &c, uint64_t images,
         return here;
     };
     w.hidden = take(l.row_bytes * (backward ? 2 : 1));
+    size_t shares = shares_bytes((uint32_t)images, c.outputs, c.hidden, kLeastRun<kDown>);
     if (backward) {
         const uint64_t runs = (images + 255) / 256 * (256 / kLeastM);
         w.partial = take(runs * 2 * l.stride * 4);
         w.parts = take(std::max(parts_bytes(runs, (uint32_t)(2 * l.stride)), parts_bytes(images, c.outputs)));
-        w.shares = take(std::max(shares_bytes((uint32_t)(2 * l.stride), c.features, (uint32_t)images), shares_bytes(c.outputs, c.hidden, (uint32_t)images)));
+        shares = std::max({shares, shares_bytes((uint32_t)images, c.features, (uint32_t)(2 * l.stride), kLeastRun<kBackInput>),
+                           shares_bytes((uint32_t)(2 * l.stride), c.features, (uint32_t)images, kLeastRun<kGradGate>),
+                           shares_bytes(c.outputs, c.hidden, (uint32_t)images, kLeastRun<kGradDown>)});
     }
+    w.shares = take(shares);
     w.bytes = at;
     return w;
 }
@@ -122,16 +130,24 @@ template <int OP> int dense_large(pink_hip_readout *r, DenseArgs &g, uint32_t *r
     return launched(r, "k_dense_large");
 }
 
+// Tiles as large as there are enough of, to fetch less for each product; of the smallest the four waves share a stage's steps, as there a
+// block's way through the depth is what takes time.  Measured (us; tiles of 16 x 32 / 32 x 32 / 64 x 64 / 128 x 128):
+//   bfloat16  500 rows, 784 columns, depth 512 (104 tiles of 64 x 64)      8.2 /   6.1 /  7.4 /  14     500 x 512, 784 (64)        6.2 / 7.4 / 11 / 15
+//             304 x 2048, 2048 (160)                                       18 /    20 /    17 /  30     1000 x 1024, 1024 (256)     17 /  15 / 12 / 20
+//             2000 x 8192, 1024 (4096, of 128 x 128 1024)                 210 /   202 /    81 /  52     1024 x 4096, 2000 (256)    138 /  85 / 37 / 33
+//   float32   304 x 2048, 2048 (160)                                       41 /    43 /    45 / 136     2000 x 1024, 784 (512)      56 /  55 / 38 / 60
+//             4096 x 4096, 1024 (4096, of 128 x 128 1024)                 459 /   446 /   326 / 308     1024 x 2048, 4096 (128)    248 / 212 / 168 / 299
+// and of 256 x 256 as in the header of k_dense_large.
 template <typename E, int OP, bool DIRECT> int dense_as(pink_hip_readout *r, DenseArgs &g, uint32_t *runs)
 {
     const auto tiles = [&](uint32_t pr, uint32_t qc) { return (uint64_t)((g.rows + pr - 1) / pr) * ((g.cols * (OP == kGate ? 2ull : 1ull) + qc - 1) / qc); };
-    if (g.splits > 1) return dense_of_tile<E, OP, 64, 64, 1, 1, 4, 32, 2, DIRECT>(r, g, runs);
-    if (g.rows <= 16) return dense_of_tile<E, OP, 16, 32, 1, 1, 4, 16, 4, DIRECT>(r, g, runs);
+    if (g.splits > 1) return dense_of_tile<E, OP, 64, 64, 2, 2, 1, 16, 2, DIRECT>(r, g, runs);
     if constexpr (sizeof(E) == 2 && DIRECT)
         if (tiles(256, 256) >= 192 && is_large<OP>(g)) return dense_large<OP>(r, g, runs);
-    if (tiles(128, 128) >= 192) return dense_of_tile<E, OP, 128, 128, 2, 2, 1, 32, 1, DIRECT>(r, g, runs);
-    if (tiles(64, 64) >= 128) return dense_of_tile<E, OP, 64, 64, 1, 1, 4, 32, 2, DIRECT>(r, g, runs);
-    return dense_of_tile<E, OP, 32, 32, 1, 1, 4, 16, 4, DIRECT>(r, g, runs);
+    if (tiles(128, 128) >= 256) return dense_of_tile<E, OP, 128, 128, 2, 2, 1, 32, 1, DIRECT>(r, g, runs);
+    if (tiles(64, 64) >= (sizeof(E) == 2 ? kFullTiles : 192)) return dense_of_tile<E, OP, 64, 64, 2, 2, 1, 16, 2, DIRECT>(r, g, runs);
+    if (tiles(32, 32) >= 384) return dense_of_tile<E, OP, 32, 32, 1, 1, 4, 16, 4, DIRECT>(r, g, runs);
+    return dense_of_tile<E, OP, 16, 32, 1, 1, 4, 16, 4, DIRECT>(r, g, runs);
 }
 
 template <typename E, int OP> int dense(pink_hip_readout *r, DenseArgs &g, uint32_t *runs = nullptr)
@@ -146,8 +162,8 @@ template <typename E, int OP> int dense(pink_hip_readout *r, DenseArgs &g, uint3
             return launched(r, "k_few");
         }
     }
-    if constexpr (OP == kGradGate || OP == kGradDown) {
-        const Split s = split_of<64, 64>(g.rows, g.cols, g.depth);
+    if constexpr (OP != kGate && OP != kBackGate) {
+        const Split s = split_of(g.rows, g.cols, g.depth, kLeastRun<OP>);
         g.splits = s.splits;
         g.depth_each = s.each;
         if (s.splits == 1) g.shares = nullptr;
@@ -156,8 +172,9 @@ template <typename E, int OP> int dense(pink_hip_readout *r, DenseArgs &g, uint3
     if (g.splits == 1) return PINK_HIP_OK;
     const uint64_t blocks = ((uint64_t)g.rows * g.cols + 255) / 256;
     REFUSE(r, too_many(blocks, 256), "too many images for one call");
-    k_join<E><<<(uint32_t)blocks, 256, 0, r->stream>>>(g.shares, g.splits, g.rows, g.cols, nullptr, nullptr, 0, (E *)g.out, (E *)g.out2, g.out_stride, g.half,
-                                                       g.hidden);
+    k_join<E><<<(uint32_t)blocks, 256, 0, r->stream>>>(g.shares, g.splits, g.rows, g.cols, OP == kDown ? (const E *)g.bias : nullptr,
+                                                       OP == kDown ? (const E *)g.residual : nullptr, g.residual_stride, (E *)g.out, (E *)g.out2, g.out_stride,
+                                                       OP == kGradGate ? g.half : 0, g.hidden);
     return launched(r, "k_join");
 }
 
@@ -182,7 +199,8 @@ int gated(pink_hip_readout *r, const Shape &c, const void *x, uint32_t images, u
           const void *residual, uint64_t residual_stride, void *y, uint64_t y_stride, void *keep)
 {
     const GatedLayout l = gated_layout(r, c, images);
-    if (!keep) TRY(grow(r, gated_work(r, c, images, false).bytes));
+    const GatedWork w = gated_work(r, c, images, false);
+    TRY(grow(r, w.bytes));
     char *const saved = keep ? (char *)keep : (char *)r->work;
     DenseArgs g = {};
     g.activation = c.activation;
@@ -212,6 +230,7 @@ int gated(pink_hip_readout *r, const Shape &c, const void *x, uint32_t images, u
     g.bias = weights.down_bias;
     g.residual = residual;
     g.residual_stride = residual_stride;
+    g.shares = (float *)((char *)r->work + w.shares);
     g.out = y;
     g.out2 = g.out3 = nullptr;
     g.out_stride = y_stride;
@@ -265,6 +284,7 @@ int gated_backward(pink_hip_readout *r, const Shape &c, const void *x, uint32_t 
         g.hidden = c.hidden;
         g.out = out.features;
         g.out_stride = dx_stride;
+        g.shares = (float *)(work + w.shares);
         TRY((dense<E, kBackInput>(r, g)));
     }
     if (matrices) {
