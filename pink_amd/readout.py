@@ -12,11 +12,18 @@ mirrored, as the map's distances do not.  Everything between the images and the 
 has to be imported before the library is loaded, so that both run on one HIP runtime and share a stream (importing this
 module first does that).
 
-    python -m pink_amd.readout [--steps N]
+Answers may be logits of classes instead, learned from labels and from what a larger read-out answers:
 
-trains a small map on synthetic sources and a read-out of their size and axis ratio.
+    teacher.learn(images, labels)
+    student.learn(images, labels, teacher.teach(images, places=8))
+
+    python -m pink_amd.readout [--steps N] [--blocks N] [--distil]
+
+trains a small map on synthetic sources and a read-out of their size and axis ratio (with --distil: of classes of both, and a smaller one
+from it).
 """
 import argparse
+import collections
 import functools
 import math
 import types
@@ -46,9 +53,19 @@ def _on_its_device(call):
     return run
 
 
+# What a read-out answered about images: its largest logits and their classes, and the logarithm of the sum over all classes of
+# exp(logit / temperature).
+Teacher = collections.namedtuple("Teacher", "classes logits normaliser temperature")
+
+_EPSILON = 1e-5              # of the blocks' layer norm
+
+
 class MapReadout:
     """Two-layer models of a map's neurons on its heatmap; `chosen` of them answer for an image, weighted by the softmax of
     sharpness * (radius - distance).
+
+    With `blocks` the features go through as many blocks first, x + gated(norm(x)), which all neurons share: layer norm and a gated
+    feed-forward block of `block_hidden` hidden values (twice the neurons unless given), nothing but x to start with.
 
     The map is copied when it is made, as a pink.Mapper does: its models are trained on that map.  The first step's images set `level`,
     the scale of the features, and where sharpness and radius start; answers asked for before go by the scale of their own images.
@@ -61,7 +78,7 @@ class MapReadout:
 
     def __init__(self, som, outputs, hidden=32, chosen=2, activation=capi.ACT_GELU, learning_rate=3e-3, weight_decay=1e-3, balance_rate=1e-3,
                  state_bits=32, number_of_rotations=360, use_flip=True, euclidean_distance_dim=None,
-                 euclidean_distance_type=pink.DataType.UINT8, seed=0):
+                 euclidean_distance_type=pink.DataType.UINT8, seed=0, blocks=0, block_hidden=None):
         self.som, self.outputs, self.hidden, self.chosen, self.state_bits = som, outputs, hidden, chosen, state_bits
         self.learning_rate, self.weight_decay, self.balance_rate = learning_rate, weight_decay, balance_rate
         self._map_args = (int(number_of_rotations), bool(use_flip), int(euclidean_distance_dim))
@@ -69,6 +86,10 @@ class MapReadout:
         n = som.number_of_neurons
         self._rows = som._rows().copy()
         self._neuron_channels, self._neuron_dim = pink._image_geometry(som.neuron_shape, som.neuron_layout, "neuron")
+        self.blocks, self.block_hidden = int(blocks), int(2 * n if block_hidden is None else block_hidden)
+        if self.blocks < 0 or not 1 <= self.block_hidden <= 2 ** 20:
+            raise pink.exception(-1, "blocks must be 0 or more, and their hidden values between 1 and 1048576")
+        self._shape = (n, self.block_hidden, n, capi.ACT_SILU)
         _check_one_runtime()
         capi.Readout.check(n, chosen, n, hidden, outputs, activation=activation)
         torch.cuda.init()
@@ -88,6 +109,11 @@ class MapReadout:
         self.parameters = {"sharpness": zeros(n) + 1, "radius": zeros(n),
                            "first": randn(n, hidden, n, scale=1 / math.sqrt(n)), "first_bias": zeros((n, hidden)),
                            "second": randn(n, outputs, hidden, scale=1 / math.sqrt(hidden)), "second_bias": zeros((n, outputs))}
+        for b in range(self.blocks):
+            h = self.block_hidden
+            self.parameters |= {"block%d.%s" % (b, k): v for k, v in {
+                "weight": zeros(n) + 1, "bias": zeros(n), "gate": randn(h, n, scale=1 / math.sqrt(n)), "gate_bias": zeros(h),
+                "up": randn(h, n, scale=1 / math.sqrt(n)), "up_bias": zeros(h), "down": zeros((n, h)), "down_bias": zeros(n)}.items()}
         self.gradients = {k: torch.zeros_like(v) for k, v in self.parameters.items()}
         state, blocks = (lambda v, t: zeros(v.numel(), t)), lambda v: zeros(-(-v.numel() // 256))
         if state_bits == 8:
@@ -96,7 +122,7 @@ class MapReadout:
         else:
             self.states = {k: dict(first=state(v, torch.float32), second=state(v, torch.float32)) for k, v in self.parameters.items()}
         self._tensors = self.readout.tensors([
-            dict(value=v.data_ptr(), gradient=self.gradients[k].data_ptr(), size=v.numel(), decay=weight_decay if k in ("first", "second") else 0.0,
+            dict(value=v.data_ptr(), gradient=self.gradients[k].data_ptr(), size=v.numel(), decay=weight_decay if k.split(".")[-1] in ("first", "second", "gate", "up", "down") else 0.0,
                  **{s: x.data_ptr() for s, x in self.states[k].items()}) for k, v in self.parameters.items()])
         self.parameters, self.gradients = types.MappingProxyType(self.parameters), types.MappingProxyType(self.gradients)
         self.states = types.MappingProxyType({k: types.MappingProxyType(v) for k, v in self.states.items()})
@@ -167,6 +193,41 @@ class MapReadout:
     def _weights(self):
         return [self.parameters[k].data_ptr() for k in ("first", "first_bias", "second", "second_bias")]
 
+    def _block(self, b, which=None):
+        """Addresses of a block's parameters, or of their gradients: the layer norm's, and the gated block's."""
+        of = self.parameters if which is None else which
+        at = [of["block%d.%s" % (b, k)].data_ptr() for k in ("weight", "bias", "gate", "gate_bias", "up", "up_bias", "down", "down_bias")]
+        return at[:2], at[2:]
+
+    def _through_blocks(self, x, keep):
+        """The features that the neurons' models see, and what a backward pass through the blocks needs."""
+        r, (t, n), kept = self.readout, x.shape, []
+        for b in range(self.blocks):
+            norm, weights = self._block(b)
+            normed, out = torch.empty_like(x), torch.empty_like(x)
+            mean, scale, saved = None, None, None
+            if keep:
+                mean, scale = torch.empty(t, device=self.device), torch.empty(t, device=self.device)
+                saved = torch.empty(r.gated_saved_bytes(self._shape, t), dtype=torch.uint8, device=self.device)
+                kept.append((x, mean, scale, normed, saved))
+            r.norm(x.data_ptr(), t, n, *norm, _EPSILON, normed.data_ptr(), mean.data_ptr() if keep else None, scale.data_ptr() if keep else None)
+            r.gated(self._shape, normed.data_ptr(), t, weights, out.data_ptr(), dev_residual=x.data_ptr(), dev_saved=saved.data_ptr() if keep else None)
+            x = out
+        return x, kept
+
+    def _back_through_blocks(self, kept, dx):
+        """The blocks' gradients for those of the features that the models saw."""
+        r, (t, n) = self.readout, dx.shape
+        for b in reversed(range(self.blocks)):
+            x, mean, scale, normed, saved = kept[b]
+            (norm_weight, _), weights = self._block(b)
+            (dweight, dbias), grads = self._block(b, self.gradients)
+            dnormed = torch.empty_like(dx)
+            r.gated_backward(self._shape, normed.data_ptr(), t, weights, saved.data_ptr(), dx.data_ptr(), [dnormed.data_ptr()] + grads)
+            # (what came in needs none: distances are not trained)
+            r.norm_backward(x.data_ptr(), t, n, norm_weight, mean.data_ptr(), scale.data_ptr(), dnormed.data_ptr(), dx.data_ptr() if b else None, dweight,
+                            dbias, dev_residual=dx.data_ptr())
+
     def _forward(self, heat, keep):
         r, p, t = self.readout, self.parameters, heat.shape[0]
         level, sharpness, radius = (self.level, p["sharpness"], p["radius"]) if self.level is not None else self._levels(heat)
@@ -174,18 +235,18 @@ class MapReadout:
         neuron = torch.empty((t, self.chosen), dtype=torch.int32, device=self.device)
         gates, y = torch.empty((t, self.chosen), device=self.device), torch.empty((t, self.outputs), device=self.device)
         saved = torch.empty(r.saved_bytes(t), dtype=torch.uint8, device=self.device) if keep else None
+        x, kept = self._through_blocks(x, keep)
         r.route(heat.data_ptr(), t, sharpness.data_ptr(), radius.data_ptr(), self.bias.data_ptr(), neuron.data_ptr(), gates.data_ptr())
         r.experts(x.data_ptr(), t, neuron.data_ptr(), gates.data_ptr(), self._weights(), y.data_ptr(), dev_saved=saved.data_ptr() if keep else None)
-        return x, neuron, gates, y, saved
+        return types.SimpleNamespace(x=x, neuron=neuron, gates=gates, y=y, saved=saved, kept=kept)
 
     @_on_its_device
     def __call__(self, images):
         """Answers, (images, outputs) on the GPU."""
-        return self._forward(self.distances(images), False)[3]
+        return self._forward(self.distances(images), False).y
 
-    @_on_its_device
-    def step(self, images, targets):
-        """One step of AdamW on the mean squared error of a batch; returns the error before the step, on the GPU."""
+    def _train(self, images, loss_of):
+        """One step of AdamW; loss_of(answers) gives the loss and its gradient for the answers."""
         r, p, g = self.readout, self.parameters, self.gradients
         heat = self.distances(images)
         t = heat.shape[0]
@@ -197,17 +258,63 @@ class MapReadout:
             self.level, sharpness, radius = self._levels(heat)
             p["sharpness"].copy_(sharpness)
             p["radius"].copy_(radius)
-        x, neuron, gates, y, saved = self._forward(heat, True)
-        off = y - torch.as_tensor(targets, dtype=torch.float32, device=self.device).reshape(t, self.outputs)
-        dy, dgates = off * (2.0 / off.numel()), torch.empty_like(gates)
-        r.experts_backward(x.data_ptr(), t, gates.data_ptr(), self._weights(), saved.data_ptr(), dy.data_ptr(),
-                           [None, dgates.data_ptr()] + [g[k].data_ptr() for k in ("first", "first_bias", "second", "second_bias")])
-        r.route_backward(heat.data_ptr(), t, p["sharpness"].data_ptr(), p["radius"].data_ptr(), self.bias.data_ptr(), neuron.data_ptr(),
-                         gates.data_ptr(), dgates.data_ptr(), None, g["sharpness"].data_ptr(), g["radius"].data_ptr())
+        f = self._forward(heat, True)
+        loss, dy = loss_of(f.y)
+        dgates, dx = torch.empty_like(f.gates), torch.empty_like(f.x) if self.blocks else None
+        r.experts_backward(f.x.data_ptr(), t, f.gates.data_ptr(), self._weights(), f.saved.data_ptr(), dy.data_ptr(),
+                           [dx.data_ptr() if self.blocks else None, dgates.data_ptr()] + [g[k].data_ptr() for k in ("first", "first_bias", "second", "second_bias")])
+        if self.blocks:
+            self._back_through_blocks(f.kept, dx)
+        r.route_backward(heat.data_ptr(), t, p["sharpness"].data_ptr(), p["radius"].data_ptr(), self.bias.data_ptr(), f.neuron.data_ptr(),
+                         f.gates.data_ptr(), dgates.data_ptr(), None, g["sharpness"].data_ptr(), g["radius"].data_ptr())
         self.steps += 1
         r.adamw(self._tensors, self.steps, learning_rate=self.learning_rate, bits=self.state_bits)
-        r.balance(neuron.data_ptr(), t, self.balance_rate, self.bias.data_ptr())
-        return (off * off).mean()
+        r.balance(f.neuron.data_ptr(), t, self.balance_rate, self.bias.data_ptr())
+        return loss()
+
+    @_on_its_device
+    def step(self, images, targets):
+        """One step of AdamW on the mean squared error of a batch; returns the error before the step, on the GPU."""
+        def squared(y):
+            off = y - torch.as_tensor(targets, dtype=torch.float32, device=self.device).reshape(y.shape)
+            return lambda: (off * off).mean(), off * (2.0 / off.numel())
+        return self._train(images, squared)
+
+    @_on_its_device
+    def teach(self, images, places, temperature=2.0):
+        """What a smaller read-out learns from this one's answers, logits of classes: the `places` largest of each image and their normaliser."""
+        if not 1 <= places <= min(self.outputs, 1024) or not 0 < temperature < math.inf:
+            raise pink.exception(-1, "a teacher gives between 1 and 1024 of its classes, at a temperature larger than 0")
+        y = self(images)
+        top = y.topk(places, dim=1)
+        return Teacher(top.indices.to(torch.int32), top.values.contiguous(), torch.logsumexp(y / temperature, 1), float(temperature))
+
+    @_on_its_device
+    def learn(self, images, labels=None, teacher=None, teacher_weight=1.0, label_weight=1.0):
+        """One step of AdamW for answers that are logits of classes: on the cross entropy of `labels` (a class each, -1: none), on the distance from what a
+        teacher's teach() gave for these images (the divergence at its temperature, times its square), or on both by their weights.  Returns the mean
+        loss before the step, on the GPU."""
+        if labels is None and teacher is None:
+            raise pink.exception(-1, "classes are learned from labels or a teacher")
+
+        def distilled(y):
+            t, classes = y.shape
+            given = dict(label_weight=0.0, teacher_weight=0.0)
+            if labels is not None:
+                label = torch.as_tensor(labels, device=self.device).to(torch.int32).contiguous()
+                if label.shape != (t,):
+                    raise pink.exception(-1, "labels must be a class for each image")
+                given |= dict(dev_label=label.data_ptr(), label_weight=label_weight)
+            if teacher is not None:
+                at, logits, normaliser = (v.to(self.device, k).contiguous() for v, k in zip(teacher, (torch.int32, torch.float32, torch.float32)))
+                if at.shape != logits.shape or at.shape[0] != t or normaliser.shape != (t,):
+                    raise pink.exception(-1, "a teacher's places must be of these images")
+                given |= dict(dev_teacher_class=at.data_ptr(), dev_teacher_logits=logits.data_ptr(), places=at.shape[1], temperature=teacher.temperature,
+                              dev_teacher_normaliser=normaliser.data_ptr(), teacher_weight=teacher_weight)
+            losses, dy, each = torch.empty(t, device=self.device), torch.empty_like(y), torch.full((t,), 1.0 / t, device=self.device)
+            self.readout.distil(y.data_ptr(), t, classes, losses.data_ptr(), dy.data_ptr(), dev_image_weights=each.data_ptr(), **given)
+            return losses.sum, dy
+        return self._train(images, distilled)
 
 
 def synthetic_sources(count, edge, rng):
@@ -221,12 +328,31 @@ def synthetic_sources(count, edge, rng):
     return images, np.stack([(size - 3.25) / 1.0, (ratio - 0.65) / 0.2], 1).astype(np.float32)
 
 
+def distil_small_sources(som, images, targets, new, truth, steps, batch, rng, options):
+    """Sixteen classes of size and axis ratio: a read-out is trained on labels, and a smaller one on labels and the first one's answers."""
+    def classes(values):
+        edges = np.quantile(targets, (0.25, 0.5, 0.75), axis=0)
+        return sum((values[:, i, None] > edges[:, i]).sum(1) * 4 ** i for i in range(2)).astype(np.int32)
+    label, right = classes(targets), classes(truth)
+    teacher = MapReadout(som, outputs=16, hidden=64, **{**options, "blocks": max(1, options["blocks"])})
+    student = MapReadout(som, outputs=16, hidden=8, **{**options, "blocks": 0})
+    for name, learner, learn in (("teacher", teacher, lambda pick: teacher.learn(images[pick], label[pick])),
+                                 ("student", student, lambda pick: student.learn(images[pick], label[pick], teacher.teach(images[pick], places=4)))):
+        for step in range(steps):
+            loss = learn(rng.integers(0, len(images), batch))
+            if step % 50 == 0 or step + 1 == steps:
+                print("%s, step %4d: loss %.4f" % (name, step + 1, float(loss)), flush=True)
+        print("%s, new sources: %.3f of the classes right" % (name, float((learner(new).argmax(1).cpu().numpy() == right).mean())), flush=True)
+
+
 def main(argv=None):
     parser = argparse.ArgumentParser(prog="pink_amd.readout", description="trains a small map on synthetic sources and a read-out of their size and axis ratio")
     parser.add_argument("--steps", type=int, default=300)
     parser.add_argument("--batch", type=int, default=256)
     parser.add_argument("--chosen", type=int, default=2)
     parser.add_argument("--state-bits", type=int, default=32, choices=(8, 32))
+    parser.add_argument("--blocks", type=int, default=0, help="blocks that the neurons' models share")
+    parser.add_argument("--distil", action="store_true", help="sixteen classes instead: a read-out on labels, and a smaller one from it")
     args = parser.parse_args(argv)
     rng = np.random.default_rng(0)
     edge, region = 32, 22
@@ -236,7 +362,11 @@ def main(argv=None):
     trainer = pink.Trainer(som, pink.GaussianFunctor(1.1, 0.2), number_of_rotations=92, euclidean_distance_dim=region)
     trainer.train(images)
     trainer.update_som()
-    answers = MapReadout(som, outputs=2, chosen=args.chosen, state_bits=args.state_bits, number_of_rotations=92, euclidean_distance_dim=region)
+    options = dict(chosen=args.chosen, state_bits=args.state_bits, number_of_rotations=92, euclidean_distance_dim=region, blocks=args.blocks)
+    if args.distil:
+        new, truth = synthetic_sources(1024, edge, rng)
+        return distil_small_sources(som, images, targets, new, truth, args.steps, args.batch, rng, options)
+    answers = MapReadout(som, outputs=2, **options)
     for step in range(args.steps):
         pick = rng.integers(0, len(images), args.batch)
         loss = answers.step(images[pick], targets[pick])

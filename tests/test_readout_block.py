@@ -189,8 +189,9 @@ def gated_reference(m, element, act, dy):
     out = {"y": (y, off)}
     if dy is not None:
         dh, off_dh = dy @ down, (o + 2) * S * (np.abs(dy) @ np.abs(down))
-        k1, off_k1 = product(slope, b, off_slope, off_b, u + S)          # as it is kept
-        off_k2 = off_v + u * np.abs(v) * 1.01
+        kept = 2.0 ** -15 if element.bf16 else 0                         # (cut off after 16 bits, or all of float32's)
+        k1, off_k1 = product(slope, b, off_slope, off_b, kept + S)
+        off_k2 = off_v + kept * np.abs(v) * 1.01
         da, off_da32 = product(dh, k1, off_dh, off_k1, S)
         db, off_db32 = product(dh, v, off_dh, off_k2, S)
         off_da, off_db = off_da32 + u * np.abs(da) * 1.01 + u * off_da32, off_db32 + u * np.abs(db) * 1.01 + u * off_db32
@@ -240,6 +241,12 @@ GATED = [  # images, features, hidden, outputs, activation, bias, residual, padd
     (1501, 23, 17, 9, "silu", True, True, 0),
     (2100, 520, 1096, 520, "silu", True, True, 0),
     (2099, 519, 1095, 521, "relu", True, False, 1),
+    # few rows and a long summed axis, in whole chunks and not; the same cut into runs
+    (3, 2312, 2120, 40, "silu", True, True, 0),
+    (25, 2313, 2121, 41, "gelu", True, True, 2),
+    (32, 4104, 40, 4104, "silu", False, True, 0),
+    (40, 72, 4104, 136, "silu", True, True, 0),
+    (41, 71, 4101, 135, "silu", True, True, 1),
 ]
 
 
@@ -283,6 +290,19 @@ def test_gated(gpu, t, f, h, o, act, bias, residual, pad, bf16):  # noqa: F811
             ro.gated_backward(shape, p["x"], t, weights, saved, p["dy"], [alone if j == i else None for j in given], x_stride=f + pad, y_gradient_stride=o + pad)
             ro.synchronize()
             assert np.array_equal(gpu.down(alone, names[i], element.dtype), got[i]), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t, f, h, o, act, bias, residual, pad", [
+    # each product in tiles of 256 x 256: with last tiles and stages that are not full
+    (4100, 328, 3080, 264, "silu", True, True, 8),
+    (4097, 64, 3328, 64, "gelu", False, False, 0),
+    (4100, 3080, 192, 3080, "silu", True, True, 0),
+    (72, 1544, 4104, 4104, "relu", True, False, 8),
+    (130, 3080, 4104, 3080, "silu", True, True, 0),
+])
+def test_gated_in_large_tiles(gpu, t, f, h, o, act, bias, residual, pad):  # noqa: F811
+    test_gated(gpu, t, f, h, o, act, bias, residual, pad, True)
 
 
 @pytest.mark.parametrize("act", ["identity", "gelu", "silu"])
