@@ -59,6 +59,16 @@ size_t shares_bytes(uint32_t rows, uint32_t cols, uint32_t depth, uint32_t least
     return s.splits > 1 ? align256((size_t)s.splits * rows * cols * 4) : 0;
 }
 
+// kGate of float32, whose few tiles of 64 x 64 take a compute unit tens of microseconds each: cut so that some 450 are dealt.  Measured (us, whole / cut):
+// 301 rows, 2025 x 1000, 160 tiles 50 / 42 with the launch that joins them.
+Split split_of_gate(uint32_t rows, uint32_t cols, uint32_t depth)
+{
+    const uint64_t tiles = (uint64_t)((rows + 63) / 64) * ((2 * (uint64_t)cols + 63) / 64);
+    if (tiles < 96 || tiles >= 320 || depth < 1536) return {1, depth};
+    const uint32_t splits = (uint32_t)std::min<uint64_t>((448 + tiles - 1) / tiles, depth / 512), each = ((depth + splits - 1) / splits + 127) / 128 * 128;
+    return {(depth + each - 1) / each, each};
+}
+
 template <int OP> constexpr uint32_t kLeastRun = OP == kGradGate || OP == kGradDown ? 512 : 1024;
 
 GatedWork gated_work(const pink_hip_readout *r, const Shape &c, uint64_t images, bool backward)
@@ -73,6 +83,10 @@ GatedWork gated_work(const pink_hip_readout *r, const Shape &c, uint64_t images,
     };
     w.hidden = take(l.row_bytes * (backward ? 2 : 1));
     size_t shares = shares_bytes((uint32_t)images, c.outputs, c.hidden, kLeastRun<kDown>);
+    if (element_bytes(r) == 4) {
+        const Split s = split_of_gate((uint32_t)images, c.hidden, c.features);
+        if (s.splits > 1) shares = std::max(shares, (size_t)s.splits * 2 * images * l.stride * 4);
+    }
     if (backward) {
         const uint64_t runs = (images + 255) / 256 * (256 / kLeastM);
         w.partial = take(runs * 2 * l.stride * 4);
@@ -162,14 +176,20 @@ template <typename E, int OP> int dense(pink_hip_readout *r, DenseArgs &g, uint3
             return launched(r, "k_few");
         }
     }
-    if constexpr (OP != kGate && OP != kBackGate) {
-        const Split s = split_of(g.rows, g.cols, g.depth, kLeastRun<OP>);
+    if constexpr (OP != kBackGate && (OP != kGate || sizeof(E) == 4)) {
+        const Split s = OP == kGate ? split_of_gate(g.rows, g.cols, g.depth) : split_of(g.rows, g.cols, g.depth, kLeastRun<OP>);
         g.splits = s.splits;
         g.depth_each = s.each;
         if (s.splits == 1) g.shares = nullptr;
     }
     TRY((is_direct<E, OP>(g) ? dense_as<E, OP, true>(r, g, runs) : dense_as<E, OP, false>(r, g, runs)));
     if (g.splits == 1) return PINK_HIP_OK;
+    if constexpr (OP == kGate) {
+        const uint64_t blocks = (g.rows * (g.out_stride / 4) + 255) / 256;
+        REFUSE(r, too_many(blocks, 256), "too many images for one call");
+        k_join_gate<E><<<(uint32_t)blocks, 256, 0, r->stream>>>(g);
+        return launched(r, "k_join_gate");
+    }
     const uint64_t blocks = ((uint64_t)g.rows * g.cols + 255) / 256;
     REFUSE(r, too_many(blocks, 256), "too many images for one call");
     k_join<E><<<(uint32_t)blocks, 256, 0, r->stream>>>(g.shares, g.splits, g.rows, g.cols, OP == kDown ? (const E *)g.bias : nullptr,
@@ -219,6 +239,7 @@ int gated(pink_hip_readout *r, const Shape &c, const void *x, uint32_t images, u
     g.out3 = keep ? saved + 2 * l.row_bytes : nullptr;
     g.lower = (uint16_t *)(saved + 3 * l.row_bytes);       // (bfloat16)
     g.out_stride = l.stride;
+    g.shares = sizeof(E) == 4 ? (float *)((char *)r->work + w.shares) : nullptr;
     TRY((dense<E, kGate>(r, g)));
     g.p = saved;
     g.p_stride = l.stride;

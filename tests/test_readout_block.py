@@ -247,6 +247,8 @@ GATED = [  # images, features, hidden, outputs, activation, bias, residual, padd
     (32, 4104, 40, 4104, "silu", False, True, 0),
     (40, 72, 4104, 136, "silu", True, True, 0),
     (41, 71, 4101, 135, "silu", True, True, 1),
+    (200, 1544, 800, 32, "silu", True, False, 0),
+    (200, 1545, 801, 33, "relu", True, True, 0),
 ]
 
 
