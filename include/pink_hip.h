@@ -392,13 +392,13 @@ int pink_hip_readout_adamw(pink_hip_readout *readout, const pink_hip_readout_ten
 int pink_hip_readout_unpack(pink_hip_readout *readout, const pink_hip_readout_tensor *tensors, uint32_t count);
 
 /* Layer norm of rows of `width` elements (at most 2^20): y = weight (x - mean) scale + bias, scale = 1 / sqrt(variance + epsilon), the
- * variance being the mean of (x - mean)^2.  weight and bias (`width` elements) may be NULL, y may be x.  mean and scale (a
+ * variance being the mean of (x - mean)^2.  weight and bias (`width` elements) may be NULL, y may be x, with its stride.  mean and scale (a
  * float32 each row; what the backward call needs) are left where they are not NULL. */
 int pink_hip_readout_norm(pink_hip_readout *readout, const void *dev_x, uint32_t images, uint32_t width, uint64_t x_stride,
                           const void *dev_weight, const void *dev_bias, float epsilon, void *dev_y, uint64_t y_stride,
                           float *dev_mean_out, float *dev_scale_out);
 /* Gradients for those of y, dy: of x, to which residual (NULL: nothing; images x width) is added, and of weight and bias, summed over the images.
- * x, weight, mean and scale as in the forward call.  Gradients that are not wanted are NULL; dx may be dy or residual, not x. */
+ * x, weight, mean and scale as in the forward call.  Gradients that are not wanted are NULL; dx may be dy or residual, with its stride. */
 int pink_hip_readout_norm_backward(pink_hip_readout *readout, const void *dev_x, uint32_t images, uint32_t width, uint64_t x_stride,
                                    const void *dev_weight, const float *dev_mean, const float *dev_scale, const void *dev_dy, uint64_t dy_stride,
                                    const void *dev_residual, uint64_t residual_stride, void *dev_dx_out, uint64_t dx_stride,
@@ -426,12 +426,13 @@ size_t pink_hip_readout_gated_saved_bytes(pink_hip_readout *readout, const pink_
 int pink_hip_readout_gated(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, const void *dev_x, uint32_t images,
                            uint64_t x_stride, const pink_hip_readout_gated_weights *dev_weights, const void *dev_residual,
                            uint64_t residual_stride, void *dev_y, uint64_t y_stride, void *dev_saved);
-/* Gradients for those of y; x and weights as in the forward call that left `saved`.  (The residual's are those of y.) */
+/* Gradients for those of y; x and weights as in the forward call that left `saved`.  (The residual's are those of y.)
+ * Those of the features may lie where x or dy does. */
 int pink_hip_readout_gated_backward(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, const void *dev_x, uint32_t images,
                                     uint64_t x_stride, const pink_hip_readout_gated_weights *dev_weights, const void *dev_saved,
                                     const void *dev_y_gradients, uint64_t y_gradient_stride,
                                     const pink_hip_readout_gated_gradients *dev_gradients_out, uint64_t x_gradient_stride);
-/* Grows the workspace to what forward and backward calls on so many images need. */
+/* Grows the workspace to what forward and backward calls on up to so many images need. */
 int pink_hip_readout_gated_reserve(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, uint32_t images);
 
 /* Losses of answers that are logits of classes, against what was kept of a teacher's logits, its largest, and against labels:
@@ -445,7 +446,7 @@ int pink_hip_readout_gated_reserve(pink_hip_readout *readout, const pink_hip_rea
 typedef struct pink_hip_readout_distil_config {
     uint32_t classes;        /* at least 1 and at most 2^20              */
     uint32_t places;         /* of the teacher, an image; at most 1024   */
-    float temperature;       /* of the teacher's part; larger than 0     */
+    float temperature;       /* of the teacher's part; at least 2^-126   */
     float teacher_weight, label_weight;
 } pink_hip_readout_distil_config;
 /* losses (a float32 each) and gradients of the losses' sum (images x classes) may each be NULL; so may be the teacher's arrays where

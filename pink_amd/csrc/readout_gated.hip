@@ -53,6 +53,9 @@ Split split_of(uint32_t rows, uint32_t cols, uint32_t depth, uint32_t least)
     return {(depth + each - 1) / each, each};
 }
 
+// What any product's runs have at most: of kSplitTiles tiles, with kGate's of float32 of the least multiple of under 320 that is 448 or more.
+constexpr size_t kMostShares = std::max(kSplitTiles, 448u + 320u) * 64 * 64 * 4;
+
 size_t shares_bytes(uint32_t rows, uint32_t cols, uint32_t depth, uint32_t least)
 {
     const Split s = split_of(rows, cols, depth, least);
@@ -291,23 +294,6 @@ int gated_backward(pink_hip_readout *r, const Shape &c, const void *x, uint32_t 
         if (biases)
             TRY((sum_columns<float, E>(r, g.partial, 2 * l.stride, runs, 2 * half, (float *)(work + w.parts), out.gate_bias, out.up_bias, half, c.hidden)));
     }
-    if (out.features) {
-        DenseArgs g = {};
-        g.rows = images;
-        g.p = work + w.hidden;
-        g.p_stride = 2 * l.stride;
-        g.q = weights.gate;
-        g.q2 = weights.up;
-        g.q_stride = c.features;
-        g.cols = c.features;
-        g.depth = 2 * half;
-        g.half = half;
-        g.hidden = c.hidden;
-        g.out = out.features;
-        g.out_stride = dx_stride;
-        g.shares = (float *)(work + w.shares);
-        TRY((dense<E, kBackInput>(r, g)));
-    }
     if (matrices) {
         DenseArgs g = {};
         g.rows = 2 * half;
@@ -341,6 +327,23 @@ int gated_backward(pink_hip_readout *r, const Shape &c, const void *x, uint32_t 
     }
     if (out.down_bias)
         TRY((sum_columns<E, E>(r, (const E *)dy, dy_stride, images, c.outputs, (float *)(work + w.parts), out.down_bias, nullptr, 0, 0)));
+    if (out.features) {                                    // (last: they may lie where x or dy does)
+        DenseArgs g = {};
+        g.rows = images;
+        g.p = work + w.hidden;
+        g.p_stride = 2 * l.stride;
+        g.q = weights.gate;
+        g.q2 = weights.up;
+        g.q_stride = c.features;
+        g.cols = c.features;
+        g.depth = 2 * half;
+        g.half = half;
+        g.hidden = c.hidden;
+        g.out = out.features;
+        g.out_stride = dx_stride;
+        g.shares = (float *)(work + w.shares);
+        TRY((dense<E, kBackInput>(r, g)));
+    }
     return PINK_HIP_OK;
 }
 
@@ -368,7 +371,8 @@ int pink_hip_readout_gated_reserve(pink_hip_readout *r, const pink_hip_readout_g
     if (!r) return PINK_HIP_EINVAL;
     TRY(check_shape(r, c, images));
     HIP_TRY(r, hipSetDevice(r->cfg.device));
-    return grow(r, gated_work(r, *c, images, true).bytes);
+    const GatedWork w = gated_work(r, *c, images, true);   // (fewer images may be cut into runs where more are not)
+    return grow(r, w.shares + kMostShares);
 }
 
 int pink_hip_readout_gated(pink_hip_readout *r, const pink_hip_readout_gated_config *c, const void *x, uint32_t images, uint64_t x_stride,

@@ -2,6 +2,7 @@
 // include/pink_hip.h): layer norm and its gradients, and an image's loss against its teacher and its label.
 #include "readout_handle.h"
 
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -27,7 +28,7 @@ int pink_hip_readout_norm(pink_hip_readout *r, const void *x, uint32_t images, u
     REFUSE(r, !(epsilon >= 0.0f) || std::isinf(epsilon), "pink_hip_readout_norm: epsilon must be 0 or larger, and finite");
     x_stride = x_stride ? x_stride : width;
     y_stride = y_stride ? y_stride : width;
-    REFUSE(r, x_stride < width || y_stride < width, "pink_hip_readout_norm: rows overlap");
+    REFUSE(r, x_stride < width || y_stride < width || (x == y && x_stride != y_stride && images > 1), "pink_hip_readout_norm: rows overlap");
     if (images == 0) return PINK_HIP_OK;
     REFUSE(r, !x || !y, "pink_hip_readout_norm: null argument");
     REFUSE(r, images > kMaxRows, "too many images for one call");
@@ -54,7 +55,7 @@ int pink_hip_readout_norm_reserve(pink_hip_readout *r, uint32_t images, uint32_t
     REFUSE(r, width == 0 || width > kMaxSize, "pink_hip_readout_norm: width must be between 1 and 1048576");
     REFUSE(r, images > kMaxRows, "too many images for one call");
     HIP_TRY(r, hipSetDevice(r->cfg.device));
-    // (no more rows have fewer parts than images or kNormFew, whose rows are a block's)
+    // (rows up to kNormFew may have a block each, and so more parts than more rows)
     return grow(r, (size_t)std::max(norm_parts(images, width), norm_parts(std::min(images, kNormFew), width)) * 2 * width * 4);
 }
 
@@ -69,6 +70,8 @@ int pink_hip_readout_norm_backward(pink_hip_readout *r, const void *x, uint32_t 
     dx_stride = dx_stride ? dx_stride : width;
     residual_stride = residual_stride ? residual_stride : width;
     REFUSE(r, x_stride < width || dy_stride < width || dx_stride < width || residual_stride < width, "pink_hip_readout_norm_backward: rows overlap");
+    REFUSE(r, images > 1 && dx && ((dx == dy && dx_stride != dy_stride) || (dx == residual && dx_stride != residual_stride)),
+           "pink_hip_readout_norm_backward: rows overlap");
     REFUSE(r, images && (!x || !mean || !scale || !dy), "pink_hip_readout_norm_backward: null argument");
     REFUSE(r, images > kMaxRows, "too many images for one call");
     if (!dweight && !dbias && (!dx || images == 0)) return PINK_HIP_OK;
@@ -99,7 +102,8 @@ int pink_hip_readout_distil(pink_hip_readout *r, const pink_hip_readout_distil_c
     REFUSE(r, !c, "pink_hip_readout_distil: null argument");
     REFUSE(r, c->classes == 0 || c->classes > kMaxSize, "pink_hip_readout_distil: classes must be between 1 and 1048576");
     REFUSE(r, c->places > kMaxPlaces, "pink_hip_readout_distil: at most 1024 places");
-    REFUSE(r, !(c->temperature > 0.0f) || std::isinf(c->temperature), "pink_hip_readout_distil: temperature must be larger than 0, and finite");
+    // (of a subnormal one the inverse is past float32)
+    REFUSE(r, !(c->temperature >= FLT_MIN) || std::isinf(c->temperature), "pink_hip_readout_distil: temperature must be 2^-126 or larger, and finite");
     REFUSE(r, !std::isfinite(c->teacher_weight) || !std::isfinite(c->label_weight), "pink_hip_readout_distil: weights must be finite");
     logit_stride = logit_stride ? logit_stride : c->classes;
     gradient_stride = gradient_stride ? gradient_stride : c->classes;

@@ -164,6 +164,27 @@ def test_norm_of_rows_at_the_edges(gpu):  # noqa: F811
         assert_within(got[[2, 7]], value, bound, "y")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 260, 1000])
+def test_norm_gradients_at_a_level_near_the_largest(gpu, n):  # noqa: F811
+    """Threads that have nothing of a row add nothing, also where a level of 2^120 by a scale of 2^10 is past float32."""
+    rng, element, t = np.random.default_rng(n), Element(False), 3
+    x, dy = np.full((t, n), 2.0 ** 120, np.float32), rng.standard_normal((t, n)).astype(np.float32)
+    args = [gpu.up(a) for a in (x, np.full(t, 2.0 ** 120, np.float32), np.full(t, 2.0 ** 10, np.float32), dy)]
+    out = [gpu.new(s, np.float32) for s in ((t, n), n, n)]
+    with capi.Readout(1, element=element.id) as ro:
+        ro.norm_backward(args[0], t, n, None, args[1], args[2], args[3], *out)
+        ro.synchronize()
+    dx, dw, db = (gpu.down(p, s, np.float32).astype(np.float64) for p, s in zip(out, ((t, n), n, n)))
+    d = dy.astype(np.float64)
+    value = 2.0 ** 10 * (d - d.mean(1, keepdims=True))     # x' is 0
+    # (a mean of n terms, at most 74 additions each: norm_reference's path; then a subtraction, a product, a rounding)
+    bound = 2.0 ** 10 * (74 * S * np.abs(d).mean(1, keepdims=True) + 3 * S * (np.abs(d) + np.abs(d).mean(1, keepdims=True)))
+    assert_within(dx, value, bound, "dx")
+    assert (dw == 0).all()
+    assert_within(db, d.sum(0), 5 * S * np.abs(d).sum(0), "db")
+
+
 # -------------------------------------------------------------------------------------------------------- gated block
 
 def gated_reference(m, element, act, dy):
@@ -337,6 +358,27 @@ def test_gated_in_place(gpu):  # noqa: F811
         ro.synchronize()
         got = gpu.down(x, more.shape, np.uint16)
         assert np.array_equal(got[:t], gpu.down(y, (t, f), np.uint16)) and (got[t:] == 0x4242).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("t, f, h", [(200, 136, 72), (70, 33, 2100)])
+def test_gated_gradients_in_place(gpu, t, f, h, bf16):  # noqa: F811
+    """The gradients of the features may lie where the images or those of the answers do: none of the others change."""
+    rng, element = np.random.default_rng(19), Element(bf16)
+    stored, _ = gated_inputs(rng, element, t, f, h, f, True, False)
+    weights, shape = [gpu.up(stored[i]) for i in WEIGHTS], (f, h, f, capi.ACT_SILU)
+    with capi.Readout(1, element=element.id) as ro:
+        saved, got = gpu.new(ro.gated_saved_bytes(shape, t), np.int8), []
+        for place in ("apart", "x", "dy"):
+            at = {"x": gpu.up(stored["x"]), "dy": gpu.up(stored["dy"]), "apart": gpu.new((t, f), element.dtype)}
+            grads = [gpu.new(stored[i].shape, element.dtype) for i in WEIGHTS]
+            ro.gated(shape, at["x"], t, weights, gpu.new((t, f), element.dtype), dev_saved=saved)
+            ro.gated_backward(shape, at["x"], t, weights, saved, at["dy"], [at[place]] + grads)
+            ro.synchronize()
+            got.append([gpu.down(at[place], (t, f), element.dtype)] + [gpu.down(p, stored[i].shape, element.dtype) for p, i in zip(grads, WEIGHTS)])
+        for other in got[1:]:
+            assert all(np.array_equal(a, b) for a, b in zip(other, got[0]))
 
 
 @pytest.mark.gpu
@@ -583,6 +625,8 @@ def test_calls_that_are_refused(gpu):  # noqa: F811
         refused(lambda: ro.norm(None, 1, 8, x, x, 1e-5, x), "null")
         refused(lambda: ro.norm(x, 1, 8, x, x, 1e-5, None), "null")
         refused(lambda: ro.norm(x, 2, 8, x, x, 1e-5, x, x_stride=7), "overlap")
+        refused(lambda: ro.norm(x, 2, 8, x, x, 1e-5, x, x_stride=9), "overlap")
+        refused(lambda: ro.norm_backward(x, 2, 8, x, x, x, x + 1024, x + 1024, dx_stride=9), "overlap")
         refused(lambda: ro.norm(x, 2 ** 31, 8, x, x, 1e-5, x), "too many")
         refused(lambda: ro.norm_backward(x, 1, 8, x, None, x, x, x), "null")
         refused(lambda: ro.norm_backward(x, 1, 8, x, x, x, x, x, dx_stride=4), "overlap")
@@ -598,7 +642,7 @@ def test_calls_that_are_refused(gpu):  # noqa: F811
         refused(lambda: ro.gated_backward(shape, x, 1, w, None, x, [x] * 7), "null")
         refused(lambda: ro.gated_backward(shape, x, 1, w, x, x, [x] * 7, x_stride=7), "overlap")
         for options, text in ((dict(places=1025), "places"), (dict(temperature=0.0), "temperature"), (dict(temperature=float("inf")), "temperature"),
-                              (dict(temperature=float("nan")), "temperature"), (dict(teacher_weight=float("nan")), "finite"), (dict(label_weight=float("inf")), "finite"),
+                              (dict(temperature=float("nan")), "temperature"), (dict(temperature=1e-40), "temperature"), (dict(teacher_weight=float("nan")), "finite"), (dict(label_weight=float("inf")), "finite"),
                               (dict(places=2), "null"), (dict(logit_stride=3), "overlap"), (dict(gradient_stride=3), "overlap")):
             refused(lambda: ro.distil(x, 1, 8, x, None, **options), text)
         refused(lambda: ro.distil(None, 1, 8, x), "null")
@@ -698,3 +742,31 @@ def test_recorded_calls_do_not_grow_the_workspace(gpu):  # noqa: F811
                     call(ro)
                 assert e.value.status == -4 and "larger workspace" in str(e.value)
             recording.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+def test_a_reserved_workspace_is_enough_for_fewer_images(gpu, bf16):  # noqa: F811
+    """Fewer images than were reserved for may be worked on otherwise: a recorded call of theirs does not have to grow the workspace."""
+    element, (f, h, o, v, most) = Element(bf16), (1600, 640, 24, 70000, 3000)
+    shape, zeros = (f, h, o, capi.ACT_SILU), lambda *s: gpu.up(np.zeros(s, element.dtype))
+    x, dy, dx, weights = zeros(most, f), zeros(most, o), zeros(most, f), [zeros(h, f), zeros(h), zeros(h, f), zeros(h), zeros(o, h), zeros(o)]
+    grads, z, dz, m = [zeros(h, f), zeros(h), zeros(h, f), zeros(h), zeros(o, h), zeros(o)], zeros(80, v), zeros(80, v), gpu.up(np.zeros(most, np.float32))
+    for t in (1, 17, 40, 64, 100, 200, 320, 600, 1000, 1100, 2000):
+        with capi.Readout(1, element=element.id) as ro:
+            saved = gpu.new(ro.gated_saved_bytes(shape, t), np.int8)
+            for calls in (1, 2):
+                if calls == 1:
+                    ro.gated_reserve(shape, most)
+                else:
+                    ro.norm_reserve(most, f)
+                    ro.distil_reserve(80, v)
+                recording = Recording(gpu, ro)
+                with recording:
+                    if calls == 1:
+                        ro.gated(shape, x, t, weights, dy, dev_saved=saved)
+                        ro.gated_backward(shape, x, t, weights, saved, dy, [dx] + grads)
+                    else:
+                        ro.norm_backward(x, t, f, None, m, m, dx, dx, grads[0], grads[2])
+                        ro.distil(z, min(t, 80), v, m, dz)
+                recording.close()
