@@ -31,7 +31,7 @@ size_t parts_bytes(uint64_t count, uint32_t cols) { return align256((count + kSu
 // Of a call's workspace.  Backward: gradients of both hidden values, sums of them down runs of rows, shares of those, and of the
 // products' depth.
 struct GatedWork {
-    size_t hidden, partial, parts, shares, bytes;
+    size_t hidden, partial, parts, answer_parts, shares, bytes;
 };
 
 constexpr uint32_t kFewRows = 32;
@@ -93,7 +93,8 @@ GatedWork gated_work(const pink_hip_readout *r, const Shape &c, uint64_t images,
     if (backward) {
         const uint64_t runs = (images + 255) / 256 * (256 / kLeastM);
         w.partial = take(runs * 2 * l.stride * 4);
-        w.parts = take(std::max(parts_bytes(runs, (uint32_t)(2 * l.stride)), parts_bytes(images, c.outputs)));
+        w.parts = take(parts_bytes(runs, (uint32_t)(2 * l.stride)));
+        w.answer_parts = take(parts_bytes(images, c.outputs));
         shares = std::max({shares, shares_bytes((uint32_t)images, c.features, (uint32_t)(2 * l.stride), kLeastRun<kBackInput>),
                            shares_bytes((uint32_t)(2 * l.stride), c.features, (uint32_t)images, kLeastRun<kGradGate>),
                            shares_bytes(c.outputs, c.hidden, (uint32_t)images, kLeastRun<kGradDown>)});
@@ -201,20 +202,32 @@ template <typename E, int OP> int dense(pink_hip_readout *r, DenseArgs &g, uint3
     return launched(r, "k_join");
 }
 
-// Sums by column over `count` rows, by way of shares of 512 rows each where there are more.
-template <typename V, typename E>
-int sum_columns(pink_hip_readout *r, const V *rows, uint64_t stride, uint32_t count, uint32_t cols, float *parts, void *out, void *out2, uint32_t half, uint32_t hidden)
+// Sums by column of two matrices at once, by way of shares of 512 rows each where there are more.  A matrix without rows there is none of.
+template <typename E, typename V1, typename V2> int sum_columns(pink_hip_readout *r, SumJob first, SumJob second)
 {
-    const uint32_t blocks = (cols + 63) / 64, shares = (count + kSumRows - 1) / kSumRows;
-    if (shares <= 1) {
-        k_sum_parts<V, E><<<blocks, 1024, 0, r->stream>>>(rows, stride, count, count, cols, nullptr, (E *)out, (E *)out2, half, hidden);
-        return launched(r, "k_sum_parts");
+    const auto blocks = [](const SumJob &g) { return g.count ? (g.cols + 63) / 64 : 0; };
+    const auto shares = [](const SumJob &g) { return (uint32_t)(((uint64_t)g.count + kSumRows - 1) / kSumRows); };
+    const uint32_t most = std::max(shares(first), shares(second));
+    REFUSE(r, most > 65535, "too many images for one call");
+    SumJob then[2] = {first, second};
+    for (SumJob *const g : {&first, &second}) {
+        g->each = kSumRows;
+        SumJob &after = then[g == &second];
+        if (shares(*g) > 1) {
+            after.rows = g->shares;
+            after.stride = g->cols;
+            after.count = after.each = shares(*g);
+        } else {
+            g->shares = nullptr;
+            after.count = 0;
+        }
+        after.shares = nullptr;
     }
-    REFUSE(r, shares > 65535, "too many images for one call");
-    k_sum_parts<V, E><<<dim3(blocks, shares), 1024, 0, r->stream>>>(rows, stride, count, kSumRows, cols, parts, nullptr, nullptr, 0, 0);
-    TRY(launched(r, "k_sum_parts"));
-    k_sum_parts<float, E><<<blocks, 1024, 0, r->stream>>>(parts, cols, shares, shares, cols, nullptr, (E *)out, (E *)out2, half, hidden);
-    return launched(r, "k_sum_parts");
+    k_sum_rows<E, V1, V2><<<dim3(blocks(first) + blocks(second), most), 1024, 0, r->stream>>>(first, blocks(first), second);
+    TRY(launched(r, "k_sum_rows"));
+    if (most <= 1) return PINK_HIP_OK;
+    k_sum_rows<E, float, float><<<blocks(then[0]) + blocks(then[1]), 1024, 0, r->stream>>>(then[0], blocks(then[0]), then[1]);
+    return launched(r, "k_sum_rows");
 }
 
 template <typename E>
@@ -272,6 +285,7 @@ int gated_backward(pink_hip_readout *r, const Shape &c, const void *x, uint32_t 
     const char *const saved = (const char *)keep;
     const uint32_t half = (uint32_t)l.stride;
     const bool biases = out.gate_bias || out.up_bias, matrices = out.gate || out.up;
+    SumJob hidden_sums = {}, answer_sums = {};
     if (out.features || matrices || biases) {
         DenseArgs g = {};
         g.rows = images;
@@ -291,9 +305,27 @@ int gated_backward(pink_hip_readout *r, const Shape &c, const void *x, uint32_t 
         g.partial = biases ? (float *)(work + w.partial) : nullptr;
         uint32_t runs = 0;
         TRY((dense<E, kBackGate>(r, g, &runs)));
-        if (biases)
-            TRY((sum_columns<float, E>(r, g.partial, 2 * l.stride, runs, 2 * half, (float *)(work + w.parts), out.gate_bias, out.up_bias, half, c.hidden)));
+        if (biases) {
+            hidden_sums.rows = g.partial;
+            hidden_sums.stride = 2 * l.stride;
+            hidden_sums.count = runs;
+            hidden_sums.cols = 2 * half;
+            hidden_sums.shares = (float *)(work + w.parts);
+            hidden_sums.out = out.gate_bias;
+            hidden_sums.out2 = out.up_bias;
+            hidden_sums.half = half;
+            hidden_sums.hidden = c.hidden;
+        }
     }
+    if (out.down_bias) {
+        answer_sums.rows = dy;
+        answer_sums.stride = dy_stride;
+        answer_sums.count = images;
+        answer_sums.cols = c.outputs;
+        answer_sums.shares = (float *)(work + w.answer_parts);
+        answer_sums.out = out.down_bias;
+    }
+    if (biases || out.down_bias) TRY((sum_columns<E, float, E>(r, hidden_sums, answer_sums)));
     if (matrices) {
         DenseArgs g = {};
         g.rows = 2 * half;
@@ -325,8 +357,6 @@ int gated_backward(pink_hip_readout *r, const Shape &c, const void *x, uint32_t 
         g.shares = (float *)(work + w.shares);
         TRY((dense<E, kGradDown>(r, g)));
     }
-    if (out.down_bias)
-        TRY((sum_columns<E, E>(r, (const E *)dy, dy_stride, images, c.outputs, (float *)(work + w.parts), out.down_bias, nullptr, 0, 0)));
     if (out.features) {                                    // (last: they may lie where x or dy does)
         DenseArgs g = {};
         g.rows = images;
