@@ -202,6 +202,82 @@ template <typename E, int OP> int dense(pink_hip_readout *r, DenseArgs &g, uint3
     return launched(r, "k_join");
 }
 
+// Some of the last three products of a backward pass.
+template <typename E, bool DIRECT> int dense_three_as(pink_hip_readout *r, DenseThree &g, const bool (&wanted)[3], int tile)
+{
+    DenseArgs *const of[3] = {&g.input, &g.grad_gate, &g.grad_down};
+    const auto run = [&](uint32_t pr, uint32_t qc, auto kernel) {
+        uint64_t at = 0;
+        for (int n = 0; n < 3; ++n) {
+            DenseArgs &d = *of[n];
+            d.row_tiles = (d.rows + pr - 1) / pr;
+            d.col_tiles = (d.cols + qc - 1) / qc;
+            g.begin[n] = (uint32_t)at;
+            g.blocks[n] = wanted[n] ? d.row_tiles * d.col_tiles : 0;
+            at += (g.blocks[n] + 7) / 8 * 8;
+        }
+        if (!at) return (int)PINK_HIP_OK;
+        kernel<<<(uint32_t)at, 256, 0, r->stream>>>(g);
+        return launched(r, "k_dense_three");
+    };
+    if (tile == 64) return run(64, 64, k_dense_three<E, 64, 64, 2, 2, 1, 16, 2, DIRECT>);
+    if constexpr (sizeof(E) == 4)
+        if (tile == 32) return run(32, 32, k_dense_three<E, 32, 32, 1, 1, 4, 16, 4, DIRECT>);
+    return run(16, 32, k_dense_three<E, 16, 32, 1, 1, 4, 16, 4, DIRECT>);
+}
+
+// One launch where none of them fills the card with larger tiles, nor has so long an axis that its tiles would be under way when all others are done, and
+// which is then cut into runs.  Tiles as large as all three have enough of.  Measured (us, the whole training step, rows x features x hidden x outputs,
+// each alone / together):
+//                              float32        bfloat16
+//    100 x  331 x  256 x  331      37 /  29       35 /  29     tiles of 16 x 32 (of 32 x 32 float32  31, of 64 x 64 41; bfloat16 29, 32)
+//    500 x  784 x  512 x  784      86 /  76       48 /  40     32 x 32 (76 / 80), bfloat16 64 x 64 (50 / 40 of 16 x 32 / 64 x 64)
+//   2000 x  784 x  256 x  784     142 / 130       70 /  60     the same
+//   1000 x 1024 x 1024 x 1024     226 / 216       84 /  71     64 x 64
+//    300 x 2025 x 1000 x  331     172 / 160      106 /  86     64 x 64
+//   1000 x  784 x 3000 x  784     608 / 517      173 / 144     64 x 64
+//  10813 x  784 x  256 x  784     570 / 737      180 / 186     not: 595 tiles of 128 x 128 in the first
+template <typename E> int dense_three(pink_hip_readout *r, DenseThree &g)
+{
+    const bool input = g.input.out, gate = g.grad_gate.out || g.grad_gate.out2, down = g.grad_down.out;
+    const auto tiles_of = [](const DenseArgs &d, uint32_t size) { return (uint64_t)((d.rows + size - 1) / size) * ((d.cols + size - 1) / size); };
+    uint64_t tiles = 0, work = 0;
+    for (const DenseArgs *const d : {&g.input, &g.grad_gate, &g.grad_down}) {
+        tiles += tiles_of(*d, 64);
+        work += tiles_of(*d, 64) * d->depth;
+    }
+    const int tile = sizeof(E) == 2 ? tiles >= 300 ? 64 : 16 : tiles >= 800 ? 64 : tiles >= 200 ? 32 : 16;
+    const auto few = [&](const DenseArgs &d, uint32_t least) {
+        return tiles_of(d, 128) < 512 && (work / 256 >= d.depth || split_of(d.rows, d.cols, d.depth, least).splits == 1);
+    };
+    // (by the sizes alone: a gradient has the same bits whichever others are wanted)
+    if (few(g.input, kLeastRun<kBackInput>) && few(g.grad_gate, kLeastRun<kGradGate>) && few(g.grad_down, kLeastRun<kGradDown>)) {
+        for (DenseArgs *const d : {&g.input, &g.grad_gate, &g.grad_down}) {
+            d->splits = 1;
+            d->depth_each = d->depth;
+            d->shares = nullptr;
+        }
+        const auto run = [&](bool a, bool b, bool c) {
+            const bool direct = (!a || is_direct<E, kBackInput>(g.input)) && (!b || is_direct<E, kGradGate>(g.grad_gate)) &&
+                                (!c || is_direct<E, kGradDown>(g.grad_down));
+            return direct ? dense_three_as<E, true>(r, g, {a, b, c}, tile) : dense_three_as<E, false>(r, g, {a, b, c}, tile);
+        };
+        // The features' gradients may lie where x or dy does, which the others read.
+        const auto apart = [&](const void *from, uint64_t stride, uint64_t rows, uint64_t cols) {
+            const uintptr_t to = (uintptr_t)g.input.out, at = (uintptr_t)from;
+            return at + ((rows - 1) * stride + cols) * sizeof(E) <= to || to + ((g.input.rows - 1) * g.input.out_stride + g.input.cols) * sizeof(E) <= at;
+        };
+        if (apart(g.grad_gate.q, g.grad_gate.q_stride, g.grad_gate.depth, g.grad_gate.cols) &&
+            apart(g.grad_down.p, g.grad_down.p_stride, g.grad_down.depth, g.grad_down.rows))
+            return run(input, gate, down);
+        TRY(run(false, gate, down));
+        return run(input, false, false);
+    }
+    if (gate) TRY((dense<E, kGradGate>(r, g.grad_gate)));
+    if (down) TRY((dense<E, kGradDown>(r, g.grad_down)));
+    return input ? dense<E, kBackInput>(r, g.input) : PINK_HIP_OK;
+}
+
 // Sums by column of two matrices at once, by way of shares of 512 rows each where there are more.  A matrix without rows there is none of.
 template <typename E, typename V1, typename V2> int sum_columns(pink_hip_readout *r, SumJob first, SumJob second)
 {
@@ -326,55 +402,43 @@ int gated_backward(pink_hip_readout *r, const Shape &c, const void *x, uint32_t 
         answer_sums.out = out.down_bias;
     }
     if (biases || out.down_bias) TRY((sum_columns<E, float, E>(r, hidden_sums, answer_sums)));
-    if (matrices) {
-        DenseArgs g = {};
-        g.rows = 2 * half;
-        g.p = work + w.hidden;
-        g.p_stride = 2 * l.stride;
-        g.q = x;
-        g.q_stride = x_stride;
-        g.cols = c.features;
-        g.depth = images;
-        g.half = half;
-        g.hidden = c.hidden;
-        g.out = out.gate;
-        g.out2 = out.up;
-        g.out_stride = c.features;
-        g.shares = (float *)(work + w.shares);
-        TRY((dense<E, kGradGate>(r, g)));
-    }
-    if (out.down) {
-        DenseArgs g = {};
-        g.rows = c.outputs;
-        g.p = dy;
-        g.p_stride = dy_stride;
-        g.q = saved;
-        g.q_stride = l.stride;
-        g.cols = c.hidden;
-        g.depth = images;
-        g.out = out.down;
-        g.out_stride = c.hidden;
-        g.shares = (float *)(work + w.shares);
-        TRY((dense<E, kGradDown>(r, g)));
-    }
-    if (out.features) {                                    // (last: they may lie where x or dy does)
-        DenseArgs g = {};
-        g.rows = images;
-        g.p = work + w.hidden;
-        g.p_stride = 2 * l.stride;
-        g.q = weights.gate;
-        g.q2 = weights.up;
-        g.q_stride = c.features;
-        g.cols = c.features;
-        g.depth = 2 * half;
-        g.half = half;
-        g.hidden = c.hidden;
-        g.out = out.features;
-        g.out_stride = dx_stride;
-        g.shares = (float *)(work + w.shares);
-        TRY((dense<E, kBackInput>(r, g)));
-    }
-    return PINK_HIP_OK;
+    DenseThree three = {};
+    DenseArgs &gate = three.grad_gate, &down = three.grad_down, &input = three.input;
+    gate.rows = 2 * half;
+    gate.p = work + w.hidden;
+    gate.p_stride = 2 * l.stride;
+    gate.q = x;
+    gate.q_stride = x_stride;
+    gate.cols = c.features;
+    gate.depth = images;
+    gate.half = half;
+    gate.hidden = c.hidden;
+    gate.out = out.gate;
+    gate.out2 = out.up;
+    gate.out_stride = c.features;
+    down.rows = c.outputs;
+    down.p = dy;
+    down.p_stride = dy_stride;
+    down.q = saved;
+    down.q_stride = l.stride;
+    down.cols = c.hidden;
+    down.depth = images;
+    down.out = out.down;
+    down.out_stride = c.hidden;
+    input.rows = images;
+    input.p = work + w.hidden;
+    input.p_stride = 2 * l.stride;
+    input.q = weights.gate;
+    input.q2 = weights.up;
+    input.q_stride = c.features;
+    input.cols = c.features;
+    input.depth = 2 * half;
+    input.half = half;
+    input.hidden = c.hidden;
+    input.out = out.features;
+    input.out_stride = dx_stride;
+    gate.shares = down.shares = input.shares = (float *)(work + w.shares);
+    return dense_three<E>(r, three);
 }
 
 int check_shape(pink_hip_readout *r, const Shape *c, uint32_t images)

@@ -268,6 +268,13 @@ GATED = [  # images, features, hidden, outputs, activation, bias, residual, padd
     (32, 4104, 40, 4104, "silu", False, True, 0),
     (40, 72, 4104, 136, "silu", True, True, 0),
     (41, 71, 4101, 135, "silu", True, True, 1),
+    # the last three products in one launch, in tiles of 16 x 32, 32 x 32 and 64 x 64; not, for one's long axis
+    (90, 328, 248, 328, "silu", True, True, 0),
+    (400, 520, 400, 520, "gelu", True, False, 8),
+    (401, 519, 401, 521, "gelu", True, False, 0),
+    (600, 1032, 1000, 520, "silu", True, True, 0),
+    (1600, 520, 136, 264, "silu", True, True, 0),
+    (3000, 72, 64, 40, "silu", True, True, 0),
     (200, 1544, 800, 32, "silu", True, False, 0),
     (200, 1545, 801, 33, "relu", True, True, 0),
 ]
@@ -362,7 +369,7 @@ def test_gated_in_place(gpu):  # noqa: F811
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bf16", [False, True])
-@pytest.mark.parametrize("t, f, h", [(200, 136, 72), (70, 33, 2100)])
+@pytest.mark.parametrize("t, f, h", [(200, 136, 72), (70, 33, 2100), (600, 520, 400), (1400, 72, 40)])
 def test_gated_gradients_in_place(gpu, t, f, h, bf16):  # noqa: F811
     """The gradients of the features may lie where the images or those of the answers do: none of the others change."""
     rng, element = np.random.default_rng(19), Element(bf16)
