@@ -42,39 +42,54 @@ struct Split {
 
 constexpr uint32_t kFullTiles = 160, kSplitTiles = 256;    // tiles of 64 x 64: that nearly fill the card; that a product is split into
 
-// A product of few results over a long axis is cut into runs, whose sums are float32 and joined afterwards by a launch of its own (4 to 5 us).
-// Runs are 512 long at least where they are sums over rows, 1024 where they are not, whose other forms for few tiles are faster.  Measured (us, whole /
-// split): 64 rows, bfloat16, kBackInput of 4096 hidden values, 1024 columns 33 / 14; 2000 rows, kGradDown of 784 x 512 float32 30 / 24.
-Split split_of(uint32_t rows, uint32_t cols, uint32_t depth, uint32_t least)
+// A product of few results over a long axis is cut into runs, whose sums are float32 and joined afterwards by a launch of its own (4 to 5 us).  Runs are 512
+// long at least where they are sums over rows; where they are not, other forms for few tiles are faster up to 1024 for bfloat16, and to 2048 for
+// float32, in runs of 512.  Measured float32 (us, the block's forward pass; whole, in runs of 1024 at least / of 512): kDown of 64 rows, 4096 hidden
+// values, 1024 results 43 / 35, 98 x 3000 x 1000 85 / 70, 200 x 2048 x 1024 50 / 42, 256 x 1024 x 784 25 / 32.
+template <typename E, int OP> Split split_of(uint32_t rows, uint32_t cols, uint32_t depth)
 {
+    constexpr bool over_rows = OP == kGradGate || OP == kGradDown;
+    const uint32_t least = over_rows || (sizeof(E) == 4 && depth >= 2048) ? 512 : 1024;
     const uint64_t tiles = (uint64_t)((rows + 63) / 64) * ((cols + 63) / 64);
     const uint64_t splits = tiles >= kFullTiles ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(kSplitTiles / tiles, depth / least));
     const uint32_t each = (uint32_t)(((depth + splits - 1) / splits + 127) / 128 * 128);
     return {(depth + each - 1) / each, each};
 }
 
-// What any product's runs have at most: of kSplitTiles tiles, with kGate's of float32 of the least multiple of under 320 that is 448 or more.
-constexpr size_t kMostShares = std::max(kSplitTiles, 448u + 320u) * 64 * 64 * 4;
-
-size_t shares_bytes(uint32_t rows, uint32_t cols, uint32_t depth, uint32_t least)
-{
-    const Split s = split_of(rows, cols, depth, least);
-    return s.splits > 1 ? align256((size_t)s.splits * rows * cols * 4) : 0;
-}
-
-// kGate of float32, whose few tiles of 64 x 64 take a compute unit tens of microseconds each: cut so that some 450 are dealt.  Measured (us, whole / cut):
-// 301 rows, 2025 x 1000, 160 tiles 50 / 42 with the launch that joins them.
+// kGate of float32, whose few tiles of 64 x 64 take a compute unit tens of microseconds each: cut so that the card's 512 places, two a compute unit, come out
+// even.  A place on the summed axis takes two tiles that share a unit 0.026 us, one that has it for itself 0.6 of that; runs are joined in 3 us and
+// 0.004 a tile.  Measured (us, the block's forward pass; in 1 / 2 / 3 / 4 / 6 / 8 runs, * the rule's):
+//    160 tiles, depth 2025  55 / 55 / 46* / 49 / 48 / 48        188, 1936  85 / 78 / 85 / 73* / 80 / 81
+//    256 tiles, depth 4096  127 / 125* / 132 / 129 / 140 / 134  376, 1936  109 / 100* / 114 / 103 / 113 / 113
+// Below a depth of 1536 or 96 tiles smaller tiles are no slower (128 tiles, 1024: 43 / 44 / 49 / 45).
+constexpr uint32_t kGateTiles = 1536;                      // of all runs
 Split split_of_gate(uint32_t rows, uint32_t cols, uint32_t depth)
 {
     const uint64_t tiles = (uint64_t)((rows + 63) / 64) * ((2 * (uint64_t)cols + 63) / 64);
-    if (tiles < 96 || tiles >= 320 || depth < 1536) return {1, depth};
-    const uint32_t splits = (uint32_t)std::min<uint64_t>((448 + tiles - 1) / tiles, depth / 512), each = ((depth + splits - 1) / splits + 127) / 128 * 128;
+    if (tiles < 96 || tiles > kGateTiles / 2 || depth < 1536) return {1, depth};
+    double best = 0.0;
+    uint32_t splits = 1;
+    for (uint32_t s = 1; s <= 8 && s * tiles <= kGateTiles && depth / s >= 256; ++s) {
+        const uint64_t blocks = s * tiles, more = blocks % 512;
+        const double rounds = (double)(blocks / 512) + (more > 256 ? 1.0 : more ? 0.6 : 0.0);
+        const double time = rounds / s * depth * 0.026 + (s > 1 ? 3.0 + 0.004 * (double)blocks : 0.0);
+        if (s > 1 && time >= best) continue;
+        best = time;
+        splits = s;
+    }
+    const uint32_t each = ((depth + splits - 1) / splits + 127) / 128 * 128;
     return {(depth + each - 1) / each, each};
 }
 
-template <int OP> constexpr uint32_t kLeastRun = OP == kGradGate || OP == kGradDown ? 512 : 1024;
+constexpr size_t kMostShares = std::max(kSplitTiles, kGateTiles) * 64 * 64 * 4;
 
-GatedWork gated_work(const pink_hip_readout *r, const Shape &c, uint64_t images, bool backward)
+template <typename E, int OP> size_t shares_bytes(uint32_t rows, uint32_t cols, uint32_t depth)
+{
+    const Split s = split_of<E, OP>(rows, cols, depth);
+    return s.splits > 1 ? align256((size_t)s.splits * rows * cols * 4) : 0;
+}
+
+template <typename E> GatedWork gated_work(const pink_hip_readout *r, const Shape &c, uint64_t images, bool backward)
 {
     const GatedLayout l = gated_layout(r, c, images);
     GatedWork w = {};
@@ -85,8 +100,8 @@ GatedWork gated_work(const pink_hip_readout *r, const Shape &c, uint64_t images,
         return here;
     };
     w.hidden = take(l.row_bytes * (backward ? 2 : 1));
-    size_t shares = shares_bytes((uint32_t)images, c.outputs, c.hidden, kLeastRun<kDown>);
-    if (element_bytes(r) == 4) {
+    size_t shares = shares_bytes<E, kDown>((uint32_t)images, c.outputs, c.hidden);
+    if constexpr (sizeof(E) == 4) {
         const Split s = split_of_gate((uint32_t)images, c.hidden, c.features);
         if (s.splits > 1) shares = std::max(shares, (size_t)s.splits * 2 * images * l.stride * 4);
     }
@@ -95,9 +110,9 @@ GatedWork gated_work(const pink_hip_readout *r, const Shape &c, uint64_t images,
         w.partial = take(runs * 2 * l.stride * 4);
         w.parts = take(parts_bytes(runs, (uint32_t)(2 * l.stride)));
         w.answer_parts = take(parts_bytes(images, c.outputs));
-        shares = std::max({shares, shares_bytes((uint32_t)images, c.features, (uint32_t)(2 * l.stride), kLeastRun<kBackInput>),
-                           shares_bytes((uint32_t)(2 * l.stride), c.features, (uint32_t)images, kLeastRun<kGradGate>),
-                           shares_bytes(c.outputs, c.hidden, (uint32_t)images, kLeastRun<kGradDown>)});
+        shares = std::max({shares, shares_bytes<E, kBackInput>((uint32_t)images, c.features, (uint32_t)(2 * l.stride)),
+                           shares_bytes<E, kGradGate>((uint32_t)(2 * l.stride), c.features, (uint32_t)images),
+                           shares_bytes<E, kGradDown>(c.outputs, c.hidden, (uint32_t)images)});
     }
     w.shares = take(shares);
     w.bytes = at;
@@ -181,7 +196,7 @@ template <typename E, int OP> int dense(pink_hip_readout *r, DenseArgs &g, uint3
         }
     }
     if constexpr (OP != kBackGate && (OP != kGate || sizeof(E) == 4)) {
-        const Split s = OP == kGate ? split_of_gate(g.rows, g.cols, g.depth) : split_of(g.rows, g.cols, g.depth, kLeastRun<OP>);
+        const Split s = OP == kGate ? split_of_gate(g.rows, g.cols, g.depth) : split_of<E, OP>(g.rows, g.cols, g.depth);
         g.splits = s.splits;
         g.depth_each = s.each;
         if (s.splits == 1) g.shares = nullptr;
@@ -247,11 +262,12 @@ template <typename E> int dense_three(pink_hip_readout *r, DenseThree &g)
         work += tiles_of(*d, 64) * d->depth;
     }
     const int tile = sizeof(E) == 2 ? tiles >= 300 ? 64 : 16 : tiles >= 800 ? 64 : tiles >= 200 ? 32 : 16;
-    const auto few = [&](const DenseArgs &d, uint32_t least) {
-        return tiles_of(d, 128) < 512 && (work / 256 >= d.depth || split_of(d.rows, d.cols, d.depth, least).splits == 1);
-    };
+    const auto few = [&](const DenseArgs &d, const Split &alone) { return tiles_of(d, 128) < 512 && (work / 256 >= d.depth || alone.splits == 1); };
     // (by the sizes alone: a gradient has the same bits whichever others are wanted)
-    if (few(g.input, kLeastRun<kBackInput>) && few(g.grad_gate, kLeastRun<kGradGate>) && few(g.grad_down, kLeastRun<kGradDown>)) {
+    const bool together = few(g.input, split_of<E, kBackInput>(g.input.rows, g.input.cols, g.input.depth)) &&
+                          few(g.grad_gate, split_of<E, kGradGate>(g.grad_gate.rows, g.grad_gate.cols, g.grad_gate.depth)) &&
+                          few(g.grad_down, split_of<E, kGradDown>(g.grad_down.rows, g.grad_down.cols, g.grad_down.depth));
+    if (together) {
         for (DenseArgs *const d : {&g.input, &g.grad_gate, &g.grad_down}) {
             d->splits = 1;
             d->depth_each = d->depth;
@@ -311,7 +327,7 @@ int gated(pink_hip_readout *r, const Shape &c, const void *x, uint32_t images, u
           const void *residual, uint64_t residual_stride, void *y, uint64_t y_stride, void *keep)
 {
     const GatedLayout l = gated_layout(r, c, images);
-    const GatedWork w = gated_work(r, c, images, false);
+    const GatedWork w = gated_work<E>(r, c, images, false);
     TRY(grow(r, w.bytes));
     char *const saved = keep ? (char *)keep : (char *)r->work;
     DenseArgs g = {};
@@ -355,7 +371,7 @@ int gated_backward(pink_hip_readout *r, const Shape &c, const void *x, uint32_t 
                    const void *keep, const void *dy, uint64_t dy_stride, const pink_hip_readout_gated_gradients &out, uint64_t dx_stride)
 {
     const GatedLayout l = gated_layout(r, c, images);
-    const GatedWork w = gated_work(r, c, images, true);
+    const GatedWork w = gated_work<E>(r, c, images, true);
     TRY(grow(r, w.bytes));
     char *const work = (char *)r->work;
     const char *const saved = (const char *)keep;
@@ -465,8 +481,8 @@ int pink_hip_readout_gated_reserve(pink_hip_readout *r, const pink_hip_readout_g
     if (!r) return PINK_HIP_EINVAL;
     TRY(check_shape(r, c, images));
     HIP_TRY(r, hipSetDevice(r->cfg.device));
-    const GatedWork w = gated_work(r, *c, images, true);   // (fewer images may be cut into runs where more are not)
-    return grow(r, w.shares + kMostShares);
+    const GatedWork w = element_bytes(r) == 2 ? gated_work<Bfloat>(r, *c, images, true) : gated_work<float>(r, *c, images, true);
+    return grow(r, w.shares + kMostShares);                // (fewer images may be cut into runs where more are not)
 }
 
 int pink_hip_readout_gated(pink_hip_readout *r, const pink_hip_readout_gated_config *c, const void *x, uint32_t images, uint64_t x_stride,
