@@ -55,8 +55,9 @@ int pink_hip_readout_norm_reserve(pink_hip_readout *r, uint32_t images, uint32_t
     REFUSE(r, width == 0 || width > kMaxSize, "pink_hip_readout_norm: width must be between 1 and 1048576");
     REFUSE(r, images > kMaxRows, "too many images for one call");
     HIP_TRY(r, hipSetDevice(r->cfg.device));
-    // (rows up to kNormFew may have a block each, and so more parts than more rows)
-    return grow(r, (size_t)std::max(norm_parts(images, width), norm_parts(std::min(images, kNormFew), width)) * 2 * width * 4);
+    uint32_t parts = 0;                                    // (few rows may have a block each, and so more parts than more rows)
+    for (const uint32_t rows : {images, std::min(images, kNormFewLong), std::min(images, kNormFew)}) parts = std::max(parts, norm_parts(rows, width));
+    return grow(r, (size_t)parts * 2 * width * 4);
 }
 
 int pink_hip_readout_norm_backward(pink_hip_readout *r, const void *x, uint32_t images, uint32_t width, uint64_t x_stride,

@@ -67,7 +67,8 @@ NORMS = [  # images, width, weight, bias, residual, padding of rows: every numbe
     (20, 256, True, True, False, 8), (1100, 33, True, True, True, 0), (5, 331, True, True, True, 0), (17, 512, False, False, False, 0),
     (6, 1000, True, True, True, 0), (9, 1024, True, True, False, 8), (301, 2025, True, True, True, 0), (13, 2048, True, True, False, 0), (3, 2049, True, True, True, 1),
     (530, 4096, True, True, True, 0), (5, 4999, True, False, True, 0), (3, 8192, True, True, False, 0), (2, 8200, False, True, True, 8),
-    (2, 16384, True, True, True, 0), (70, 16385, True, True, True, 0), (2, 40003, True, True, False, 5), (1, 2 ** 20, True, True, True, 0),
+    (2, 16384, True, True, True, 0), (1030, 1000, True, True, False, 0), (8195, 1030, True, True, True, 0),
+    (70, 16385, True, True, True, 0), (2, 40003, True, True, False, 5), (1, 2 ** 20, True, True, True, 0),
 ]
 
 
