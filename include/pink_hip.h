@@ -261,14 +261,16 @@ int pink_hip_make_update_factors(uint32_t layout, const uint32_t *dims, uint32_t
 /* ------------------------------------------------------------------------------------------------
  * Read-out of a trained map.  No counterpart in the reference, which ends at the heatmap: here the
  * neurons nearest to an image answer a question about it, each with a two-layer model of its own.
- * Three operators share one handle: images are routed to neurons by their distances (the heatmap of
+ * Operators that share one handle: images are routed to neurons by their distances (the heatmap of
  * pink_hip_map_device, or any), the chosen neurons' models are evaluated on the images' features and
- * added up by their gates, and AdamW trains both.
+ * added up by their gates, and AdamW trains both.  Before the models features may go through blocks that
+ * all neurons share (layer norm, a gated feed-forward block); answers that are logits of classes have
+ * a loss against labels and against what was kept of a teacher's answers.
  *
  * All data pointers are device pointers.  Calls are asynchronous on the handle's stream: its own, or
  * one given with pink_hip_readout_set_stream; inputs made on another stream have to be complete (or
  * ordered by events) before.  The handle holds a workspace that grows to what its calls need; a call
- * that makes it grow waits for the stream and allocates (pink_hip_readout_reserve grows it beforehand),
+ * that makes it grow waits for the stream and allocates (the reserve calls grow it beforehand),
  * and is refused with PINK_HIP_ESTATE while the stream is captured into a graph.  A graph of recorded
  * calls works in the workspace they were recorded with: the handle keeps that one, also past its growing,
  * until it is destroyed, and no such graph may be launched afterwards; launches and other calls of
@@ -315,7 +317,8 @@ const char *pink_hip_readout_last_error(const pink_hip_readout *readout);
 #define PINK_HIP_OWN_STREAM ((void *)-1)
 int pink_hip_readout_set_stream(pink_hip_readout *readout, void *hip_stream);
 int pink_hip_readout_synchronize(pink_hip_readout *readout);
-/* Grows the workspace to what any call on so many images needs. */
+/* Grows the workspace to what any call on so many images needs: of routing and the neurons' models (norm, gated and distil, whose
+ * sizes are their arguments, have a reserve of their own). */
 int pink_hip_readout_reserve(pink_hip_readout *readout, uint32_t images);
 
 /* Logits z[t][n] = sharpness[n] * (radius[n] - distance[t][n]) as 32-bit numbers (a subtraction and a

@@ -427,8 +427,9 @@ class Context:
 
 
 class Readout:
-    """The read-out of a trained map: images routed to neurons by their distances, the chosen neurons' two-layer models, and the
-    optimiser that trains both (the pink_hip_readout_* functions of include/pink_hip.h, which say what each computes).
+    """The read-out of a trained map: images routed to neurons by their distances, the chosen neurons' two-layer models, the
+    optimiser that trains both, layer norm and the gated block of what all neurons share, and the loss of logits of classes against
+    labels and a teacher (the pink_hip_readout_* functions of include/pink_hip.h, which say what each computes).
 
     All data arguments are device pointers (integers, None for NULL).  Calls are asynchronous: on the handle's own stream, or on the
     one given to set_stream, e.g. torch.cuda.current_stream().cuda_stream where PyTorch was imported before this library was
@@ -560,7 +561,7 @@ class Readout:
         return int(self._L.pink_hip_readout_gated_saved_bytes(self._h, C.byref(_GatedConfig(*shape)), images))
 
     def gated_reserve(self, shape, images):
-        """Grows the workspace to what gated() and gated_backward() on so many images need."""
+        """Grows the workspace to what gated() and gated_backward() on up to so many images need."""
         self._check(self._L.pink_hip_readout_gated_reserve(self._h, C.byref(_GatedConfig(*shape)), images))
 
     def gated(self, shape, dev_x, images, weights, dev_y, dev_residual=None, dev_saved=None, x_stride=0, residual_stride=0, y_stride=0):
@@ -572,7 +573,8 @@ class Readout:
 
     def gated_backward(self, shape, dev_x, images, weights, dev_saved, dev_y_gradients, gradients, x_stride=0, y_gradient_stride=0,
                        x_gradient_stride=0):
-        """`gradients`: pointers to where those of the features and of the weights, in their order, go; None where one is not wanted."""
+        """`gradients`: pointers to where those of the features and of the weights, in their order, go; None where one is not wanted.  Those of the
+        features may lie where the features or dev_y_gradients do."""
         c, w, g = _GatedConfig(*shape), _GatedWeights(*weights), _GatedGradients(*gradients)
         self._check(self._L.pink_hip_readout_gated_backward(self._h, C.byref(c), dev_x, images, x_stride, C.byref(w), dev_saved, dev_y_gradients,
                                                             y_gradient_stride, C.byref(g), x_gradient_stride))

@@ -1,5 +1,6 @@
 // readout.hip -- the read-out of a trained map (pink_hip_readout_* of include/pink_hip.h): images routed to neurons by
-// their distances, the neurons' two-layer models, and the optimiser that trains both.
+// their distances, the neurons' two-layer models, and the optimiser that trains both.  readout_rows.hip and readout_gated.hip have the handle's
+// other operators.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
