@@ -480,6 +480,7 @@ int pink_hip_readout_gated_reserve(pink_hip_readout *r, const pink_hip_readout_g
 {
     if (!r) return PINK_HIP_EINVAL;
     TRY(check_shape(r, c, images));
+    if (images == 0) return PINK_HIP_OK;
     HIP_TRY(r, hipSetDevice(r->cfg.device));
     const GatedWork w = element_bytes(r) == 2 ? gated_work<Bfloat>(r, *c, images, true) : gated_work<float>(r, *c, images, true);
     return grow(r, w.shares + kMostShares);                // (fewer images may be cut into runs where more are not)

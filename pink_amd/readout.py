@@ -123,7 +123,8 @@ class MapReadout:
             self.states = {k: dict(first=state(v, torch.float32), second=state(v, torch.float32)) for k, v in self.parameters.items()}
         self._tensors = self.readout.tensors([
             dict(value=v.data_ptr(), gradient=self.gradients[k].data_ptr(), size=v.numel(),
-                 decay=weight_decay if k.split(".")[-1] in ("first", "second", "gate", "up", "down") else 0.0, **{s: x.data_ptr() for s, x in self.states[k].items()}) for k, v in self.parameters.items()])
+                 decay=weight_decay if k.split(".")[-1] in ("first", "second", "gate", "up", "down") else 0.0,
+                 **{s: x.data_ptr() for s, x in self.states[k].items()}) for k, v in self.parameters.items()])
         self.parameters, self.gradients = types.MappingProxyType(self.parameters), types.MappingProxyType(self.gradients)
         self.states = types.MappingProxyType({k: types.MappingProxyType(v) for k, v in self.states.items()})
         self.bias = zeros(n)                               # for an even load; takes part in the choice of neurons only
@@ -147,7 +148,7 @@ class MapReadout:
 
     @_on_its_device
     def load_state_dict(self, saved):
-        """Goes on from what state_dict() gave, of a read-out with as many neurons, hidden values and outputs and the same state_bits."""
+        """Goes on from what state_dict() gave, of a read-out with as many neurons, hidden values, outputs and blocks and the same state_bits."""
         held = self._held()
         if set(saved) != set(held) | {"level", "steps"}:
             raise pink.exception(-1, "not the state of such a read-out: " + ", ".join(sorted(set(saved) ^ (set(held) | {"level", "steps"}))))

@@ -668,6 +668,10 @@ def test_no_images(gpu):  # noqa: F811
         ro.norm(None, 0, 8, None, None, 1e-5, None)
         ro.gated((8, 8, 8, 1), None, 0, [None] * 6, None)
         ro.distil(None, 0, 8, None)
+        ro.norm_reserve(0, 8)
+        ro.gated_reserve((8, 8, 8, 1), 0)
+        ro.distil_reserve(0, 8)
+        assert ro.gated_saved_bytes((8, 8, 8, 1), 0) == 0
         grads = [gpu.new(64, np.float32) for _ in range(8)]
         ro.norm_backward(None, 0, 8, None, None, None, None, None, grads[0], grads[1])
         ro.gated_backward((8, 8, 8, 1), None, 0, [None] * 6, None, None, [None] + grads[2:])
