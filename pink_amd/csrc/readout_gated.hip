@@ -42,6 +42,30 @@ struct Split {
 
 constexpr uint32_t kFullTiles = 160, kSplitTiles = 256;    // tiles of 64 x 64: that nearly fill the card; that a product is split into
 
+// Gradients of the weights in tiles of 128 x 128, some hundreds of them over all images: cut so that 512 places come out even, two a compute unit.  A place of the
+// axis takes two tiles that share a unit 0.11 us (float32; bfloat16 0.012), runs are joined in 5 us and 8 bytes a value.  Measured (us, a training
+// step, rows x features x hidden x outputs, whole / cut): 16000 x 1600 x 3200 x 1600 (650 and 325 tiles) float32 13797 / 12800, bfloat16 2013 / 1934;
+// 16000 x 1600 x 1600 x 1600 (325, 169) 7387 / 6769, 1166 / 1099; 4096 x 1024 x 2048 x 1024 (256) stays whole.
+constexpr uint32_t kMostRuns = 4;
+template <typename E> Split split_of_gradients(uint32_t rows, uint32_t cols, uint32_t depth)
+{
+    const uint64_t tiles = (uint64_t)((rows + 127) / 128) * ((cols + 127) / 128);
+    const bool larger = sizeof(E) == 2 && (uint64_t)((rows + 255) / 256) * ((cols + 255) / 256) >= 192;          // (tiles of 256 x 256)
+    if (larger || tiles >= 2048) return {1, depth};
+    double best = 0.0;
+    uint32_t splits = 1;
+    for (uint32_t s = 1; s <= kMostRuns && depth / s >= 512; ++s) {
+        const uint64_t blocks = s * tiles, more = blocks % 512;
+        const double rounds = (double)(blocks / 512) + (more > 256 ? 1.0 : more ? 0.6 : 0.0);
+        const double time = rounds / s * depth * (sizeof(E) == 4 ? 0.11 : 0.012) + (s > 1 ? 5.0 + 2e-6 * s * rows * cols : 0.0);
+        if (s > 1 && time >= best) continue;
+        best = time;
+        splits = s;
+    }
+    const uint32_t each = ((depth + splits - 1) / splits + 127) / 128 * 128;
+    return {(depth + each - 1) / each, each};
+}
+
 // A product of few results over a long axis is cut into runs, whose sums are float32 and joined afterwards by a launch of its own (4 to 5 us).  Runs are 512
 // long at least where they are sums over rows; where they are not, other forms for few tiles are faster up to 1024 for bfloat16, and to 2048 for
 // float32, in runs of 512.  Measured float32 (us, the block's forward pass; whole, in runs of 1024 at least / of 512): kDown of 64 rows, 4096 hidden
@@ -49,6 +73,8 @@ constexpr uint32_t kFullTiles = 160, kSplitTiles = 256;    // tiles of 64 x 64: 
 template <typename E, int OP> Split split_of(uint32_t rows, uint32_t cols, uint32_t depth)
 {
     constexpr bool over_rows = OP == kGradGate || OP == kGradDown;
+    if constexpr (over_rows)
+        if ((uint64_t)((rows + 127) / 128) * ((cols + 127) / 128) >= 256) return split_of_gradients<E>(rows, cols, depth);
     const uint32_t least = over_rows || (sizeof(E) == 4 && depth >= 2048) ? 512 : 1024;
     const uint64_t tiles = (uint64_t)((rows + 63) / 64) * ((cols + 63) / 64);
     const uint64_t splits = tiles >= kFullTiles ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(kSplitTiles / tiles, depth / least));
@@ -174,9 +200,9 @@ template <int OP> int dense_large(pink_hip_readout *r, DenseArgs &g, uint32_t *r
 template <typename E, int OP, bool DIRECT> int dense_as(pink_hip_readout *r, DenseArgs &g, uint32_t *runs)
 {
     const auto tiles = [&](uint32_t pr, uint32_t qc) { return (uint64_t)((g.rows + pr - 1) / pr) * ((g.cols * (OP == kGate ? 2ull : 1ull) + qc - 1) / qc); };
-    if (g.splits > 1) return dense_of_tile<E, OP, 64, 64, 2, 2, 1, 16, 2, DIRECT>(r, g, runs);
+    if (g.splits > 1 && tiles(128, 128) < 256) return dense_of_tile<E, OP, 64, 64, 2, 2, 1, 16, 2, DIRECT>(r, g, runs);
     if constexpr (sizeof(E) == 2 && DIRECT)
-        if (tiles(256, 256) >= 192 && is_large<OP>(g)) return dense_large<OP>(r, g, runs);
+        if (g.splits == 1 && tiles(256, 256) >= 192 && is_large<OP>(g)) return dense_large<OP>(r, g, runs);
     if (tiles(128, 128) >= 256) return dense_of_tile<E, OP, 128, 128, 2, 2, 1, 32, 1, DIRECT>(r, g, runs);
     if (tiles(64, 64) >= (sizeof(E) == 2 ? kFullTiles : 192)) return dense_of_tile<E, OP, 64, 64, 2, 2, 1, 16, 2, DIRECT>(r, g, runs);
     if (tiles(32, 32) >= 384) return dense_of_tile<E, OP, 32, 32, 1, 1, 4, 16, 4, DIRECT>(r, g, runs);
@@ -483,7 +509,9 @@ int pink_hip_readout_gated_reserve(pink_hip_readout *r, const pink_hip_readout_g
     if (images == 0) return PINK_HIP_OK;
     HIP_TRY(r, hipSetDevice(r->cfg.device));
     const GatedWork w = element_bytes(r) == 2 ? gated_work<Bfloat>(r, *c, images, true) : gated_work<float>(r, *c, images, true);
-    return grow(r, w.shares + kMostShares);                // (fewer images may be cut into runs where more are not)
+    // (fewer images may be cut into runs where more are not)
+    const uint64_t gate = 2ull * gated_layout(r, *c, images).stride * c->features, down = (uint64_t)c->outputs * c->hidden;
+    return grow(r, w.shares + std::max<size_t>(kMostShares, std::min<uint64_t>(std::max(gate, down), 2048 * 128 * 128) * kMostRuns * 4));
 }
 
 int pink_hip_readout_gated(pink_hip_readout *r, const pink_hip_readout_gated_config *c, const void *x, uint32_t images, uint64_t x_stride,

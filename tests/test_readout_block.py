@@ -338,6 +338,12 @@ def test_gated_in_large_tiles(gpu, t, f, h, o, act, bias, residual, pad):  # noq
     test_gated(gpu, t, f, h, o, act, bias, residual, pad, True)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("t, f, h, o, bf16", [(2200, 1930, 1150, 24, False), (2201, 1931, 1151, 23, False), (12000, 1200, 2000, 8, True)])
+def test_gated_with_weights_gradients_in_runs_of_large_tiles(gpu, t, f, h, o, bf16):  # noqa: F811
+    test_gated(gpu, t, f, h, o, "silu", False, False, 0, bf16)
+
+
 @pytest.mark.parametrize("act", ["identity", "gelu", "silu"])
 def test_gated_gradients_of_the_restatement_against_differences(act):
     rng, element, d = np.random.default_rng(8), Element(False), 1e-5
