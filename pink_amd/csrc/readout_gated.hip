@@ -66,18 +66,21 @@ template <typename E> Split split_of_gradients(uint32_t rows, uint32_t cols, uin
     return {(depth + each - 1) / each, each};
 }
 
-// A product of few results over a long axis is cut into runs, whose sums are float32 and joined afterwards by a launch of its own (4 to 5 us).  Runs are 512
-// long at least where they are sums over rows; where they are not, other forms for few tiles are faster up to 1024 for bfloat16, and to 2048 for
-// float32, in runs of 512.  Measured float32 (us, the block's forward pass; whole, in runs of 1024 at least / of 512): kDown of 64 rows, 4096 hidden
-// values, 1024 results 43 / 35, 98 x 3000 x 1000 85 / 70, 200 x 2048 x 1024 50 / 42, 256 x 1024 x 784 25 / 32.
+// A product of few results over a long axis is cut into runs, whose sums are float32 and joined afterwards by a launch of its own (4 to 5 us).  Sums over
+// rows are cut for two tiles a compute unit, in runs of 256 at least; the others, whose other forms for few tiles are faster up to a depth of 1024 for bfloat16
+// and 2048 for float32, for one, in runs of 1024 and 512.  Measured (us, the block's forward pass, float32; whole, in runs of 1024 at least / of
+// 512): kDown of 64 rows, 4096 hidden values, 1024 results 43 / 35, 98 x 3000 x 1000 85 / 70, 200 x 2048 x 1024 50 / 42, 256 x 1024 x 784 25 / 32.
+// (A training step, rows x features x hidden x outputs, float32 and bfloat16; sums over rows for one tile a unit in runs of 512 at least / for two in runs
+// of 256): 6000 x 331 x 331 x 331 355 / 303, 183 / 154; 16000 x 784 x 256 x 784 717 / 673, 217 / 185; 16000 x 100 x 200 x 100 157 / 166, 127 / 116.
 template <typename E, int OP> Split split_of(uint32_t rows, uint32_t cols, uint32_t depth)
 {
     constexpr bool over_rows = OP == kGradGate || OP == kGradDown;
     if constexpr (over_rows)
         if ((uint64_t)((rows + 127) / 128) * ((cols + 127) / 128) >= 256) return split_of_gradients<E>(rows, cols, depth);
-    const uint32_t least = over_rows || (sizeof(E) == 4 && depth >= 2048) ? 512 : 1024;
+    const uint32_t least = over_rows ? 256 : sizeof(E) == 4 && depth >= 2048 ? 512 : 1024;
     const uint64_t tiles = (uint64_t)((rows + 63) / 64) * ((cols + 63) / 64);
-    const uint64_t splits = tiles >= kFullTiles ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(kSplitTiles / tiles, depth / least));
+    const uint64_t full = over_rows ? 300 : kFullTiles, places = over_rows ? 512 : kSplitTiles;
+    const uint64_t splits = tiles >= full ? 1 : std::max<uint64_t>(1, std::min<uint64_t>(places / tiles, depth / least));
     const uint32_t each = (uint32_t)(((depth + splits - 1) / splits + 127) / 128 * 128);
     return {(depth + each - 1) / each, each};
 }
@@ -267,7 +270,7 @@ template <typename E, bool DIRECT> int dense_three_as(pink_hip_readout *r, Dense
     return run(16, 32, k_dense_three<E, 16, 32, 1, 1, 4, 16, 4, DIRECT>);
 }
 
-// One launch where none of them fills the card with larger tiles, nor has so long an axis that its tiles would be under way when all others are done, and
+// One launch where none of them fills the card with larger tiles, nor has so long an axis that its tiles would be under way long after all others are done, and
 // which is then cut into runs.  Tiles as large as all three have enough of.  Measured (us, the whole training step, rows x features x hidden x outputs,
 // each alone / together):
 //                              float32        bfloat16
@@ -277,7 +280,11 @@ template <typename E, bool DIRECT> int dense_three_as(pink_hip_readout *r, Dense
 //   1000 x 1024 x 1024 x 1024     226 / 216       84 /  71     64 x 64
 //    300 x 2025 x 1000 x  331     172 / 160      106 /  86     64 x 64
 //   1000 x  784 x 3000 x  784     608 / 517      173 / 144     64 x 64
+//   1000 x   64 x   64 x   16      52 /  32       43 /  29     16 x 32
+//   2000 x  331 x  256 x  331     117 /  97       77 /  71     16 x 32
+//   3000 x  331 x  256 x  331     144 / 147       84 / 117     not: 3000 rows
 //  10813 x  784 x  256 x  784     570 / 737      180 / 186     not: 595 tiles of 128 x 128 in the first
+constexpr uint32_t kTogether = 2048;                       // rows that sums over them take in one go
 template <typename E> int dense_three(pink_hip_readout *r, DenseThree &g)
 {
     const bool input = g.input.out, gate = g.grad_gate.out || g.grad_gate.out2, down = g.grad_down.out;
@@ -288,11 +295,10 @@ template <typename E> int dense_three(pink_hip_readout *r, DenseThree &g)
         work += tiles_of(*d, 64) * d->depth;
     }
     const int tile = sizeof(E) == 2 ? tiles >= 300 ? 64 : 16 : tiles >= 800 ? 64 : tiles >= 200 ? 32 : 16;
-    const auto few = [&](const DenseArgs &d, const Split &alone) { return tiles_of(d, 128) < 512 && (work / 256 >= d.depth || alone.splits == 1); };
+    const auto few = [&](const DenseArgs &d, bool whole) { return tiles_of(d, 128) < 512 && (work / 256 >= d.depth || whole); };
     // (by the sizes alone: a gradient has the same bits whichever others are wanted)
-    const bool together = few(g.input, split_of<E, kBackInput>(g.input.rows, g.input.cols, g.input.depth)) &&
-                          few(g.grad_gate, split_of<E, kGradGate>(g.grad_gate.rows, g.grad_gate.cols, g.grad_gate.depth)) &&
-                          few(g.grad_down, split_of<E, kGradDown>(g.grad_down.rows, g.grad_down.cols, g.grad_down.depth));
+    const bool together = few(g.input, split_of<E, kBackInput>(g.input.rows, g.input.cols, g.input.depth).splits == 1) &&
+                          few(g.grad_gate, g.grad_gate.depth < kTogether) && few(g.grad_down, g.grad_down.depth < kTogether);
     if (together) {
         for (DenseArgs *const d : {&g.input, &g.grad_gate, &g.grad_down}) {
             d->splits = 1;

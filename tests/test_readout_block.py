@@ -275,6 +275,9 @@ GATED = [  # images, features, hidden, outputs, activation, bias, residual, padd
     (401, 519, 401, 521, "gelu", True, False, 0),
     (600, 1032, 1000, 520, "silu", True, True, 0),
     (1600, 520, 136, 264, "silu", True, True, 0),
+    (2047, 72, 64, 40, "silu", True, True, 0),
+    (2048, 72, 64, 40, "silu", True, True, 0),
+    (2600, 331, 331, 331, "relu", True, True, 0),
     (3000, 72, 64, 40, "silu", True, True, 0),
     (97, 1544, 3001, 32, "silu", True, False, 0),
     (65, 2112, 2200, 72, "gelu", True, True, 8),
