@@ -422,7 +422,7 @@ typedef struct pink_hip_readout_gated_weights {
 typedef struct pink_hip_readout_gated_gradients {
     void *features, *gate, *gate_bias, *up, *up_bias, *down, *down_bias;
 } pink_hip_readout_gated_gradients;
-/* residual may be NULL; y may be x or residual.  What a backward pass needs is left in `saved` (pink_hip_readout_gated_saved_bytes bytes, which
+/* residual may be NULL; y may be x, or residual with its stride.  What a backward pass needs is left in `saved` (pink_hip_readout_gated_saved_bytes bytes, which
  * is 0 for arguments that are refused; 256-byte aligned) unless it is NULL: h, rounded to the handle's element type, and
  * the two factors of its gradient, f(a) and f'(a) times the other, with bfloat16 to 16 bits of their significands. */
 size_t pink_hip_readout_gated_saved_bytes(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, uint32_t images);

@@ -542,6 +542,8 @@ int pink_hip_readout_gated(pink_hip_readout *r, const pink_hip_readout_gated_con
     y_stride = y_stride ? y_stride : c->outputs;
     residual_stride = residual_stride ? residual_stride : c->outputs;
     REFUSE(r, x_stride < c->features || y_stride < c->outputs || residual_stride < c->outputs, "pink_hip_readout_gated: rows overlap");
+    // (blocks of kDown write rows that others have yet to read; x has been read by then)
+    REFUSE(r, images > 1 && y && y == residual && y_stride != residual_stride, "pink_hip_readout_gated: rows overlap");
     REFUSE(r, (uintptr_t)saved & 255, "pink_hip_readout_gated: saved must be aligned to 256 bytes");
     if (images == 0) return PINK_HIP_OK;
     REFUSE(r, !x || !weights || !weights->gate || !weights->up || !weights->down || !y, "pink_hip_readout_gated: null argument");

@@ -793,3 +793,32 @@ def test_a_reserved_workspace_is_enough_for_fewer_images(gpu, bf16):  # noqa: F8
                         ro.norm_backward(x, t, f, None, m, m, dx, dx, grads[0], grads[2])
                         ro.distil(z, min(t, 80), v, m, dz)
                 recording.close()
+
+
+@pytest.mark.gpu
+def test_gated_over_a_residual_of_other_strides(gpu):  # noqa: F811
+    """Answers take the residual's place row by row, or not at all."""
+    rng, element, (t, f, h) = np.random.default_rng(20), Element(False), (40, 24, 16)
+    stored, _ = gated_inputs(rng, element, t, f, h, f, True, True)
+    weights, shape = [gpu.up(stored[i]) for i in WEIGHTS], (f, h, f, capi.ACT_SILU)
+    x, wide = gpu.up(stored["x"]), padded(stored["residual"], 5, np.nan)
+    with capi.Readout(1) as ro:
+        for images in (2, t):
+            for strides in ((0, f + 5), (f + 5, 0), (f + 5, f + 6)):
+                place = gpu.up(wide)
+                refused(lambda: ro.gated(shape, x, images, weights, place, dev_residual=place, residual_stride=strides[0], y_stride=strides[1]), "overlap")
+                assert np.array_equal(gpu.down(place, wide.shape, np.float32), wide, equal_nan=True)
+        for images, strides in ((t, (f + 5, f + 5)), (1, (0, f + 5)), (1, (f + 5, 0))):
+            place, y = gpu.up(wide), gpu.new((images, f), np.float32)
+            ro.gated(shape, x, images, weights, y, dev_residual=place, residual_stride=f + 5)
+            ro.gated(shape, x, images, weights, place, dev_residual=place, residual_stride=strides[0], y_stride=strides[1])
+            ro.synchronize()
+            got = gpu.down(place, wide.shape, np.float32)
+            assert np.array_equal(got[:images, :f], gpu.down(y, (images, f), np.float32))
+            assert np.isnan(got[:, f:]).all() and np.array_equal(got[images:, :f], wide[images:, :f])
+        # x has been read when answers are written, whatever its stride
+        place, y = gpu.up(padded(stored["x"], 5, np.nan)), gpu.new((t, f), np.float32)
+        ro.gated(shape, place, t, weights, y, x_stride=f + 5)
+        ro.gated(shape, place, t, weights, place, x_stride=f + 5)
+        ro.synchronize()
+        assert np.array_equal(gpu.down(place, (t, f), np.float32), gpu.down(y, (t, f), np.float32))
