@@ -822,3 +822,31 @@ def test_gated_over_a_residual_of_other_strides(gpu):  # noqa: F811
         ro.gated(shape, place, t, weights, place, x_stride=f + 5)
         ro.synchronize()
         assert np.array_equal(gpu.down(place, (t, f), np.float32), gpu.down(y, (t, f), np.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("v", [10, 700, 9000, 140000])
+def test_distil_of_rows_that_are_not_finite_and_have_nothing_to_learn(gpu, v, bf16):  # noqa: F811
+    """Without a label, and without a place that takes part: NaN all the same, and rows that are finite 0."""
+    rng, element = np.random.default_rng(21), Element(bf16)
+    z = rng.standard_normal((6, v)).astype(np.float32)
+    z[1, v // 2], z[2, v - 1], z[3, 0], z[4], z[5] = np.nan, np.inf, np.nan, np.nan, -np.inf
+    teachers = {"out of range": (np.full((6, 2), -1, np.int32), np.ones((6, 2), np.float32)), "lowest": (np.tile(np.array([0, v - 1], np.int32), (6, 1)), np.full((6, 2), -np.inf, np.float32)),
+                "none": (None, None)}
+    logits = gpu.up(element.store(z)[0])
+    with capi.Readout(1, element=element.id) as ro:
+        for name, (at, teacher) in teachers.items():
+            p, k = (gpu.up(at), gpu.up(teacher)), 0 if at is None else 2
+            for label in (None, np.full(6, -1, np.int32), np.full(6, v, np.int32)):
+                for weight in (0.0, 1.0):
+                    for grads in (None, gpu.new((6, v), element.dtype)):
+                        losses = gpu.up(np.full(6, 7.0, np.float32))
+                        ro.distil(logits, 6, v, losses, grads, dev_teacher_class=p[0], dev_teacher_logits=p[1], places=k, dev_label=gpu.up(label), temperature=2.0,
+                                  teacher_weight=weight, label_weight=1.0)
+                        ro.synchronize()
+                        got = gpu.down(losses, 6, np.float32)
+                        assert (got[[0, 5]] == 0).all() and np.isnan(got[1:5]).all(), (name, weight, got)
+                        if grads:
+                            g = element.values(gpu.down(grads, (6, v), element.dtype))
+                            assert (g[[0, 5]] == 0).all() and np.isnan(g[1:5]).all(), (name, weight)
