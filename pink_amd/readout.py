@@ -191,6 +191,10 @@ class MapReadout:
         each = part.sum(0)
         return torch.stack((mean, spread)), (1 / spread).repeat(heat.shape[1]), torch.where(each > 0, known.sum(0) / each.clamp(min=1), mean)
 
+    def _scale(self, heat):
+        """Level, sharpness and radius: the read-out's, or before its first step those that the images would set."""
+        return (self.level, self.parameters["sharpness"], self.parameters["radius"]) if self.level is not None else self._levels(heat)
+
     def _weights(self):
         return [self.parameters[k].data_ptr() for k in ("first", "first_bias", "second", "second_bias")]
 
@@ -230,8 +234,8 @@ class MapReadout:
                             dbias, dev_residual=dx.data_ptr())
 
     def _forward(self, heat, keep):
-        r, p, t = self.readout, self.parameters, heat.shape[0]
-        level, sharpness, radius = (self.level, p["sharpness"], p["radius"]) if self.level is not None else self._levels(heat)
+        r, t = self.readout, heat.shape[0]
+        level, sharpness, radius = scale = self._scale(heat)
         x = torch.where(torch.isfinite(heat), (heat - level[0]) / level[1], 0.0)
         neuron = torch.empty((t, self.chosen), dtype=torch.int32, device=self.device)
         gates, y = torch.empty((t, self.chosen), device=self.device), torch.empty((t, self.outputs), device=self.device)
@@ -239,7 +243,7 @@ class MapReadout:
         x, kept = self._through_blocks(x, keep)
         r.route(heat.data_ptr(), t, sharpness.data_ptr(), radius.data_ptr(), self.bias.data_ptr(), neuron.data_ptr(), gates.data_ptr())
         r.experts(x.data_ptr(), t, neuron.data_ptr(), gates.data_ptr(), self._weights(), y.data_ptr(), dev_saved=saved.data_ptr() if keep else None)
-        return types.SimpleNamespace(x=x, neuron=neuron, gates=gates, y=y, saved=saved, kept=kept)
+        return types.SimpleNamespace(x=x, neuron=neuron, gates=gates, y=y, saved=saved, kept=kept, scale=scale)
 
     @_on_its_device
     def __call__(self, images):
@@ -253,23 +257,23 @@ class MapReadout:
         t = heat.shape[0]
         if t == 0:
             raise pink.exception(-1, "a step needs images")
-        if self.level is None:
-            if not torch.isfinite(heat).any():
-                raise pink.exception(-1, "the first step needs an image with a finite distance")
-            self.level, sharpness, radius = self._levels(heat)
-            p["sharpness"].copy_(sharpness)
-            p["radius"].copy_(radius)
+        if self.level is None and not torch.isfinite(heat).any():
+            raise pink.exception(-1, "the first step needs an image with a finite distance")
         f = self._forward(heat, True)
         loss, dy = loss_of(f.y)
+        level, sharpness, radius = f.scale
         dgates, dx = torch.empty_like(f.gates), torch.empty_like(f.x) if self.blocks else None
         r.experts_backward(f.x.data_ptr(), t, f.gates.data_ptr(), self._weights(), f.saved.data_ptr(), dy.data_ptr(),
                            [dx.data_ptr() if self.blocks else None, dgates.data_ptr()] + [g[k].data_ptr() for k in ("first", "first_bias", "second", "second_bias")])
         if self.blocks:
             self._back_through_blocks(f.kept, dx)
-        r.route_backward(heat.data_ptr(), t, p["sharpness"].data_ptr(), p["radius"].data_ptr(), self.bias.data_ptr(), f.neuron.data_ptr(),
+        r.route_backward(heat.data_ptr(), t, sharpness.data_ptr(), radius.data_ptr(), self.bias.data_ptr(), f.neuron.data_ptr(),
                          f.gates.data_ptr(), dgates.data_ptr(), None, g["sharpness"].data_ptr(), g["radius"].data_ptr())
-        self.steps += 1
-        r.adamw(self._tensors, self.steps, learning_rate=self.learning_rate, bits=self.state_bits)
+        if self.level is None:
+            p["sharpness"].copy_(sharpness)
+            p["radius"].copy_(radius)
+        r.adamw(self._tensors, self.steps + 1, learning_rate=self.learning_rate, bits=self.state_bits)
+        self.level, self.steps = level, self.steps + 1     # (a step that is refused sets neither)
         r.balance(f.neuron.data_ptr(), t, self.balance_rate, self.bias.data_ptr())
         return loss()
 

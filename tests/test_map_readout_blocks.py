@@ -31,6 +31,46 @@ def test_read_outs_and_steps_that_are_refused(made):  # noqa: F811
     assert [name for name, *_ in recorder.calls] == ["route", "experts", "distil", "experts_backward", "route_backward", "adamw", "balance"]
 
 
+def test_a_first_step_that_is_refused_sets_nothing(made):  # noqa: F811
+    """Neither level, sharpness and radius nor anything else: the next step's images are the first then."""
+    from pink_amd import capi, pink, readout
+    answers, recorder, torch = made
+    heat = torch.rand(5, 6)
+    good = readout.Teacher(torch.zeros(5, 2, dtype=torch.int32), torch.zeros(5, 2), torch.zeros(5), 2.0)
+    before = {k: v.clone() for k, v in answers._held().items()}
+    def unchanged():
+        return answers.level is None and answers.steps == 0 and all(torch.equal(v, before[k]) for k, v in answers._held().items())
+    for options in (dict(), dict(labels=[0, 1]), dict(teacher=good._replace(normaliser=torch.zeros(4))), dict(labels=[0] * 5, teacher=good._replace(logits=torch.zeros(5, 3)))):
+        with pytest.raises(pink.exception):
+            answers.learn(heat, **options)
+        assert unchanged()
+    for targets in (torch.zeros(4, 2), torch.zeros(5, 3), torch.zeros(3)):
+        with pytest.raises(Exception):
+            answers.step(heat, targets)
+        assert unchanged()
+    with pytest.raises(pink.exception):
+        answers.step(torch.full((5, 6), float("inf")), torch.zeros(5, 2))
+    assert unchanged()
+    def refuse(*args, **options):                          # as the library does what only it looks at: weights, a temperature
+        raise capi.PinkError(-1, "weights must be finite")
+    recorder.distil = refuse
+    with pytest.raises(capi.PinkError):
+        answers.learn(heat, labels=[0] * 5, label_weight=float("nan"))
+    assert unchanged()
+    recorder.adamw = refuse
+    with pytest.raises(capi.PinkError):
+        answers.step(heat, torch.zeros(5, 2))
+    assert answers.level is None and answers.steps == 0
+    del recorder.adamw
+    later = heat * 3 + 1
+    level, sharpness, radius = answers._levels(later)
+    answers.step(later, torch.zeros(5, 2))
+    assert answers.steps == 1 and torch.equal(answers.level, level)
+    assert torch.equal(answers.parameters["sharpness"], sharpness) and torch.equal(answers.parameters["radius"], radius)
+    answers.step(heat, torch.zeros(5, 2))
+    assert answers.steps == 2 and torch.equal(answers.level, level) and torch.equal(answers.parameters["radius"], radius)
+
+
 # What a step's gradients are, in 64 bits; every product of K terms is off by (K + 2) 2^-24 of its magnitudes at most, K <= 256 here, and ten of them follow each other:
 # 2e-4 of a tensor's largest entry, with sums of magnitudes no more than a few times that.
 REFERENCE = """
