@@ -850,3 +850,31 @@ def test_distil_of_rows_that_are_not_finite_and_have_nothing_to_learn(gpu, v, bf
                         if grads:
                             g = element.values(gpu.down(grads, (6, v), element.dtype))
                             assert (g[[0, 5]] == 0).all() and np.isnan(g[1:5]).all(), (name, weight)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 16, 30])
+def test_few_images_by_weights_that_are_not_finite(gpu, t):  # noqa: F811
+    """An infinite weight gives infinite answers, not NaN, also where the second part of a hidden value is 0 or of the other sign; so does an infinite hidden
+    value; what is NaN stays NaN, and other answers are as they would be."""
+    rng, element, (f, h, o) = np.random.default_rng(23), Element(True), (40, 24, 16)
+    stored, value = gated_inputs(rng, element, t, f, h, o, True, False)
+    shape, p = (f, h, o, capi.ACT_SILU), {i: gpu.up(v) for i, v in stored.items()}
+    a, b = value["x"] @ value["gate"].T + value["gate_bias"], value["x"] @ value["up"].T + value["up_bias"]
+    hidden = a / (1 + np.exp(-a)) * b
+    down = stored["down"].copy()
+    down[3, 5], down[7, 2], down[9, 0] = 0x7f80, 0xff80, 0x7fc0          # infinity, minus infinity, NaN
+    with capi.Readout(1, element=element.id) as ro:
+        y, wrong = gpu.new((t, o), np.uint16), gpu.new((t, o), np.uint16)
+        ro.gated(shape, p["x"], t, [p[i] for i in WEIGHTS], y)
+        ro.gated(shape, p["x"], t, [gpu.up(down) if i == "down" else p[i] for i in WEIGHTS], wrong)
+        ro.synchronize()
+        want, got = (element.values(gpu.down(v, (t, o), np.uint16)) for v in (y, wrong))
+        want[:, 3], want[:, 7], want[:, 9] = np.sign(hidden[:, 5]) * np.inf, -np.sign(hidden[:, 2]) * np.inf, np.nan
+        assert np.array_equal(got, want, equal_nan=True)
+        # h past what is finite: a and b of 2^100 in its fourth place
+        gate_bias, up_bias = stored["gate_bias"].copy(), stored["up_bias"].copy()
+        gate_bias[3] = up_bias[3] = element.store(np.array([2.0 ** 100]))[0][0]
+        ro.gated(shape, p["x"], t, [gpu.up(gate_bias) if i == "gate_bias" else gpu.up(up_bias) if i == "up_bias" else p[i] for i in WEIGHTS], wrong)
+        ro.synchronize()
+        assert np.array_equal(element.values(gpu.down(wrong, (t, o), np.uint16)), np.tile(np.sign(value["down"][:, 3]) * np.inf, (t, 1)))
