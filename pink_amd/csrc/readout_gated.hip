@@ -35,9 +35,6 @@ struct GatedWork {
 };
 
 constexpr uint32_t kFewRows = 32;
-// k_few passes h on as two bfloat16 values up to as many weights of the second layer: its blocks all read h, twice as much then.  Measured (us, h as one / two
-// values): one image, 1024 x 2048 x 1024 9.4 / 9.7; 16 images, 4096 x 8192 x 4096 55 / 62, where the many results average the roundings.
-constexpr uint64_t kTwiceWeights = 1 << 22;
 
 struct Split {
     uint32_t splits, each;
@@ -389,8 +386,7 @@ int gated(pink_hip_readout *r, const Shape &c, const void *x, uint32_t images, u
     g.lower = (uint16_t *)(saved + 3 * l.row_bytes);       // (bfloat16)
     g.out_stride = l.stride;
     g.shares = sizeof(E) == 4 ? (float *)((char *)r->work + w.shares) : nullptr;
-    const bool twice = sizeof(E) == 2 && images <= kFewRows && (uint64_t)c.outputs * c.hidden <= kTwiceWeights;
-    if (!keep) g.lower = twice ? (uint16_t *)(saved + l.row_bytes) : nullptr;
+    if (!keep) g.lower = sizeof(E) == 2 && images <= kFewRows ? (uint16_t *)(saved + l.row_bytes) : nullptr;
     TRY((dense<E, kGate>(r, g)));
     if (keep) g.lower = nullptr;                           // (kDown: h is one value)
     g.p = saved;

@@ -7,6 +7,7 @@ of their magnitudes; where a row's terms are added up a few a thread and then by
 term goes through.
 """
 import math
+import types
 
 import numpy as np
 import pytest
@@ -850,6 +851,45 @@ def test_distil_of_rows_that_are_not_finite_and_have_nothing_to_learn(gpu, v, bf
                         if grads:
                             g = element.values(gpu.down(grads, (6, v), element.dtype))
                             assert (g[[0, 5]] == 0).all() and np.isnan(g[1:5]).all(), (name, weight)
+
+
+def few_images(rng, t, f, h, o):
+    """A bfloat16 block's inputs with the residual nearly the rest's opposite, so that what is left shows the sum's own roundings; and answers with a bound for
+    hidden values that go on as two bfloat16 values: what the second leaves of a half step is a half step of that, or of the least number."""
+    element = Element(True)
+    stored, value = gated_inputs(rng, element, t, f, h, o, True, False)
+    stored["residual"], value["residual"] = element.store(-gated_reference(value, element, "silu", None)["y"][0])
+    y, off = gated_reference(value, types.SimpleNamespace(u=element.u ** 2, bf16=True), "silu", None)["y"]
+    off = off + 2.0 ** -126 * np.abs(value["down"]).sum(1)
+    return element, stored, value, y, off + element.u * (np.abs(y) * 1.02 + off)
+
+
+FEW = [(1, 24, 16, 40), (3, 130, 33, 41), (16, 40, 24, 64), (17, 33, 31, 39), (32, 136, 64, 24), (16, 64, 2040, 2048), (16, 64, 2056, 2048), (32, 48, 4104, 1032)]
+
+
+@pytest.mark.parametrize("t, f, h, o", FEW[:5])
+def test_the_bound_of_few_images_tells_one_rounding_of_hidden_values_from_two(t, f, h, o):
+    element, stored, value, y, off = few_images(np.random.default_rng(22), t, f, h, o)
+    a, b = value["x"] @ value["gate"].T + value["gate_bias"], value["x"] @ value["up"].T + value["up_bias"]
+    hidden = a / (1 + np.exp(-a)) * b
+    once = element.store(hidden)[1]
+    twice = once + element.store(hidden - once)[1]
+    more = value["down_bias"] + value["residual"]
+    assert (np.abs(twice @ value["down"].T + more - y) <= off).all() and (np.abs(once @ value["down"].T + more - y) > off).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t, f, h, o", FEW)
+def test_few_images_without_a_backward_pass_have_one_rounding(gpu, t, f, h, o):  # noqa: F811
+    """Whatever the number of weights; with what a backward pass needs, as the block's bound says."""
+    element, stored, value, y, off = few_images(np.random.default_rng(22), t, f, h, o)
+    shape, p = (f, h, o, capi.ACT_SILU), {i: gpu.up(v) for i, v in stored.items()}
+    with capi.Readout(1, element=element.id) as ro:
+        out = gpu.new((t, o), np.uint16)
+        for keep in (None, gpu.new(ro.gated_saved_bytes(shape, t), np.int8)):
+            ro.gated(shape, p["x"], t, [p[i] for i in WEIGHTS], out, dev_residual=p["residual"], dev_saved=keep)
+            ro.synchronize()
+            assert_within(element.values(gpu.down(out, (t, o), np.uint16)), *((y, off) if keep is None else gated_reference(value, element, "silu", None)["y"]), "y")
 
 
 @pytest.mark.gpu
