@@ -46,15 +46,21 @@ constexpr uint32_t kFullTiles = 160, kSplitTiles = 256;    // tiles of 64 x 64: 
 // axis takes two tiles that share a unit 0.11 us (float32; bfloat16 0.012), runs are joined in 5 us and 8 bytes a value.  Measured (us, a training
 // step, rows x features x hidden x outputs, whole / cut): 16000 x 1600 x 3200 x 1600 (650 and 325 tiles) float32 13797 / 12800, bfloat16 2013 / 1934;
 // 16000 x 1600 x 1600 x 1600 (325, 169) 7387 / 6769, 1166 / 1099; 4096 x 1024 x 2048 x 1024 (256) stays whole.
-constexpr uint32_t kMostRuns = 4;
+constexpr uint32_t kMostRuns = 4, kCutTiles = 256;         // (with fewer tiles split_of takes smaller ones)
+constexpr uint32_t kLeastRun = 512;
+uint64_t gradient_tiles(uint32_t rows, uint32_t cols) { return (uint64_t)((rows + 127) / 128) * ((cols + 127) / 128); }
+template <typename E> bool stays_whole(uint32_t rows, uint32_t cols)
+{
+    const bool larger = sizeof(E) == 2 && (uint64_t)((rows + 255) / 256) * ((cols + 255) / 256) >= 192;          // (tiles of 256 x 256)
+    return larger || gradient_tiles(rows, cols) >= 2048;
+}
 template <typename E> Split split_of_gradients(uint32_t rows, uint32_t cols, uint32_t depth)
 {
-    const uint64_t tiles = (uint64_t)((rows + 127) / 128) * ((cols + 127) / 128);
-    const bool larger = sizeof(E) == 2 && (uint64_t)((rows + 255) / 256) * ((cols + 255) / 256) >= 192;          // (tiles of 256 x 256)
-    if (larger || tiles >= 2048) return {1, depth};
+    const uint64_t tiles = gradient_tiles(rows, cols);
+    if (stays_whole<E>(rows, cols)) return {1, depth};
     double best = 0.0;
     uint32_t splits = 1;
-    for (uint32_t s = 1; s <= kMostRuns && depth / s >= 512; ++s) {
+    for (uint32_t s = 1; s <= kMostRuns && depth / s >= kLeastRun; ++s) {
         const uint64_t blocks = s * tiles, more = blocks % 512;
         const double rounds = (double)(blocks / 512) + (more > 256 ? 1.0 : more ? 0.6 : 0.0);
         const double time = rounds / s * depth * (sizeof(E) == 4 ? 0.11 : 0.012) + (s > 1 ? 5.0 + 2e-6 * s * rows * cols : 0.0);
@@ -76,7 +82,7 @@ template <typename E, int OP> Split split_of(uint32_t rows, uint32_t cols, uint3
 {
     constexpr bool over_rows = OP == kGradGate || OP == kGradDown;
     if constexpr (over_rows)
-        if ((uint64_t)((rows + 127) / 128) * ((cols + 127) / 128) >= 256) return split_of_gradients<E>(rows, cols, depth);
+        if (gradient_tiles(rows, cols) >= kCutTiles) return split_of_gradients<E>(rows, cols, depth);
     const uint32_t least = over_rows ? 256 : sizeof(E) == 4 && depth >= 2048 ? 512 : 1024;
     const uint64_t tiles = (uint64_t)((rows + 63) / 64) * ((cols + 63) / 64);
     const uint64_t full = over_rows ? 300 : kFullTiles, places = over_rows ? 512 : kSplitTiles;
@@ -110,7 +116,18 @@ Split split_of_gate(uint32_t rows, uint32_t cols, uint32_t depth)
     return {(depth + each - 1) / each, each};
 }
 
+// What the shares take at most, for any number of images up to this: of split_of and split_of_gate, and of split_of_gradients.
 constexpr size_t kMostShares = std::max(kSplitTiles, kGateTiles) * 64 * 64 * 4;
+template <typename E> size_t most_shares_of_gradients(uint32_t rows, uint32_t cols, uint64_t images)
+{
+    const uint64_t runs = std::min<uint64_t>(kMostRuns, images / kLeastRun);
+    return runs < 2 || gradient_tiles(rows, cols) < kCutTiles || stays_whole<E>(rows, cols) ? 0 : runs * rows * cols * 4;
+}
+template <typename E> size_t most_shares(const pink_hip_readout *r, const Shape &c, uint64_t images)
+{
+    return std::max({kMostShares, most_shares_of_gradients<E>((uint32_t)(2 * gated_layout(r, c, images).stride), c.features, images),
+                     most_shares_of_gradients<E>(c.outputs, c.hidden, images)});
+}
 
 template <typename E, int OP> size_t shares_bytes(uint32_t rows, uint32_t cols, uint32_t depth)
 {
@@ -522,10 +539,10 @@ int pink_hip_readout_gated_reserve(pink_hip_readout *r, const pink_hip_readout_g
     TRY(check_shape(r, c, images));
     if (images == 0) return PINK_HIP_OK;
     HIP_TRY(r, hipSetDevice(r->cfg.device));
-    const GatedWork w = element_bytes(r) == 2 ? gated_work<Bfloat>(r, *c, images, true) : gated_work<float>(r, *c, images, true);
     // (fewer images may be cut into runs where more are not)
-    const uint64_t gate = 2ull * gated_layout(r, *c, images).stride * c->features, down = (uint64_t)c->outputs * c->hidden;
-    return grow(r, w.shares + std::max<size_t>(kMostShares, std::min<uint64_t>(std::max(gate, down), 2048 * 128 * 128) * kMostRuns * 4));
+    const bool bfloat = element_bytes(r) == 2;
+    const size_t before = bfloat ? gated_work<Bfloat>(r, *c, images, true).shares : gated_work<float>(r, *c, images, true).shares;
+    return grow(r, before + align256(bfloat ? most_shares<Bfloat>(r, *c, images) : most_shares<float>(r, *c, images)));
 }
 
 int pink_hip_readout_gated(pink_hip_readout *r, const pink_hip_readout_gated_config *c, const void *x, uint32_t images, uint64_t x_stride,

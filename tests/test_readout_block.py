@@ -6,6 +6,7 @@ is stored (2^-24 float32, 2^-8 bfloat16), s = 2^-24 that of sums.  A sum of K te
 of their magnitudes; where a row's terms are added up a few a thread and then by a tree, K is the number of additions that one
 term goes through.
 """
+import ctypes as C
 import math
 import types
 
@@ -918,3 +919,37 @@ def test_few_images_by_weights_that_are_not_finite(gpu, t):  # noqa: F811
         ro.gated(shape, p["x"], t, [gpu.up(gate_bias) if i == "gate_bias" else gpu.up(up_bias) if i == "up_bias" else p[i] for i in WEIGHTS], wrong)
         ro.synchronize()
         assert np.array_equal(element.values(gpu.down(wrong, (t, o), np.uint16)), np.tile(np.sign(value["down"][:, 3]) * np.inf, (t, 1)))
+
+
+def free_bytes(gpu):
+    free, total = C.c_size_t(), C.c_size_t()
+    gpu.ok(gpu.rt.hipMemGetInfo(C.byref(free), C.byref(total)))
+    return free.value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+def test_a_workspace_reserved_for_few_images_is_small(gpu, bf16):  # noqa: F811
+    """Hidden values and their gradients of 16 images take 4 MB at most, and runs of few tiles 1536 of 64 x 64 float32 numbers; the weights' gradients, of 134 MB
+    each, are cut from 1024 images on."""
+    with capi.Readout(1, element=Element(bf16).id) as ro:
+        before = free_bytes(gpu)
+        ro.gated_reserve((4096, 8192, 4096, capi.ACT_SILU), 16)
+        assert before - free_bytes(gpu) <= 4 * 2 ** 20 + 1536 * 64 * 64 * 4 + 2 * 2 ** 20        # (an allocation is of whole 2 MiB)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f, h, o, most, bf16", [(1930, 1150, 24, 2300, False), (24, 1930, 2300, 2300, False), (1200, 2000, 8, 12000, True)])
+def test_a_reserved_workspace_is_enough_for_gradients_in_runs(gpu, f, h, o, most, bf16):  # noqa: F811
+    """Weights' gradients of some hundred tiles of 128 x 128, which go by the number of images into runs: none of these calls has to grow what was reserved."""
+    element, shape = Element(bf16), (f, h, o, capi.ACT_SILU)
+    x, dy, dx, weights, grads = (gpu.new(s, element.dtype) for s in ((most, f), (most, o), (most, f), (3, h, max(f, o)), (3, h, max(f, o))))
+    for t in (1, 33, 500, 1023, 1024, 1536, 2200, most):
+        with capi.Readout(1, element=element.id) as ro:
+            saved = gpu.new(ro.gated_saved_bytes(shape, t), np.int8)
+            ro.gated_reserve(shape, most)
+            recording = Recording(gpu, ro)
+            with recording:
+                ro.gated(shape, x, t, [weights] * 6, dy, dev_saved=saved)
+                ro.gated_backward(shape, x, t, [weights] * 6, saved, dy, [dx] + [grads] * 6)
+            recording.close()
