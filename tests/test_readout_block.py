@@ -953,3 +953,13 @@ def test_a_reserved_workspace_is_enough_for_gradients_in_runs(gpu, f, h, o, most
                 ro.gated(shape, x, t, [weights] * 6, dy, dev_saved=saved)
                 ro.gated_backward(shape, x, t, [weights] * 6, saved, dy, [dx] + [grads] * 6)
             recording.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("t, v, k, temperature, rest, a, b, weighted, pad", [
+    # rows that a block of 1024 threads holds in 4, 8 and 16 chunks each, of either type, odd and exactly full
+    (66, 20001, 33, 2.0, True, 1.0, 0.3, True, 3), (66, 32768, 20, 0.7, True, 1.0, 0.4, False, 0), (65, 65536, 8, 4.0, True, 1.0, 0.3, True, 0), (67, 16384, 300, 1.0, False, 0.5, 1.0, False, 8),
+])
+def test_distil_of_many_long_rows(gpu, t, v, k, temperature, rest, a, b, weighted, pad, bf16):  # noqa: F811
+    test_distil(gpu, t, v, k, temperature, rest, a, b, weighted, pad, bf16)
