@@ -294,6 +294,11 @@ class MapReadout:
         top = y.topk(places, dim=1)
         return Teacher(top.indices.to(torch.int32), top.values.contiguous(), torch.logsumexp(y / temperature, 1), float(temperature))
 
+    def _class_numbers(self, of):
+        """As 32-bit numbers; what these cannot hold is past all classes, or before them, as it was."""
+        of = torch.as_tensor(of, device=self.device)
+        return (of if of.dtype == torch.int32 else of.to(torch.int64).clamp(-1, 2 ** 31 - 1).to(torch.int32)).contiguous()
+
     @_on_its_device
     def learn(self, images, labels=None, teacher=None, teacher_weight=1.0, label_weight=1.0):
         """One step of AdamW for answers that are logits of classes: on the cross entropy of `labels` (a class each, -1: none), on the distance from what a
@@ -306,12 +311,12 @@ class MapReadout:
             t, classes = y.shape
             given = dict(label_weight=0.0, teacher_weight=0.0)
             if labels is not None:
-                label = torch.as_tensor(labels, device=self.device).to(torch.int32).contiguous()
+                label = self._class_numbers(labels)
                 if label.shape != (t,):
                     raise pink.exception(-1, "labels must be a class for each image")
                 given |= dict(dev_label=label.data_ptr(), label_weight=label_weight)
             if teacher is not None:
-                at, logits, normaliser = (v.to(self.device, k).contiguous() for v, k in zip(teacher, (torch.int32, torch.float32, torch.float32)))
+                at, (logits, normaliser) = self._class_numbers(teacher.classes), (v.to(self.device, torch.float32).contiguous() for v in teacher[1:3])
                 if at.shape != logits.shape or at.shape[0] != t or normaliser.shape != (t,):
                     raise pink.exception(-1, "a teacher's places must be of these images")
                 given |= dict(dev_teacher_class=at.data_ptr(), dev_teacher_logits=logits.data_ptr(), places=at.shape[1], temperature=teacher.temperature,

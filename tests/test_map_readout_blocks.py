@@ -71,6 +71,26 @@ def test_a_first_step_that_is_refused_sets_nothing(made):  # noqa: F811
     assert answers.steps == 2 and torch.equal(answers.level, level) and torch.equal(answers.parameters["radius"], radius)
 
 
+def test_class_numbers_that_32_bits_do_not_hold_are_no_classes(made):  # noqa: F811
+    from pink_amd import readout
+    import ctypes
+    answers, recorder, torch = made
+    taken = {}
+
+    def distil(*args, dev_label, dev_teacher_class, places, **options):      # (on the CPU here: addresses that can be read)
+        taken["label"] = list((ctypes.c_int32 * 5).from_address(dev_label))
+        taken["teacher"] = list((ctypes.c_int32 * (5 * places)).from_address(dev_teacher_class))
+    recorder.distil = distil
+    far = [1, -1, 2 ** 32 + 1, -2 ** 32 + 1, 2 ** 31]
+    teacher = readout.Teacher(torch.tensor([far, [0, 1, 2 ** 40, 1, 0]]).T, torch.zeros(5, 2), torch.zeros(5), 2.0)
+    answers.learn(torch.rand(5, 6), labels=far, teacher=teacher)
+    assert taken["label"] == [1, -1, 2 ** 31 - 1, -1, 2 ** 31 - 1]
+    assert taken["teacher"] == [1, 0, -1, 1, 2 ** 31 - 1, 2 ** 31 - 1, -1, 1, 2 ** 31 - 1, 0]
+    for labels in (torch.tensor([0, 1, 1, 0, 1], dtype=torch.uint8), torch.tensor([False, True, True, False, True]), torch.tensor([0, 1, 1, 0, 1], dtype=torch.int32)):
+        answers.learn(torch.rand(5, 6), labels=labels, teacher=teacher)
+        assert taken["label"] == [0, 1, 1, 0, 1]
+
+
 # What a step's gradients are, in 64 bits; every product of K terms is off by (K + 2) 2^-24 of its magnitudes at most, K <= 256 here, and ten of them follow each other:
 # 2e-4 of a tensor's largest entry, with sums of magnitudes no more than a few times that.
 REFERENCE = """
