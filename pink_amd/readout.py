@@ -288,8 +288,8 @@ class MapReadout:
     @_on_its_device
     def teach(self, images, places, temperature=2.0):
         """What a smaller read-out learns from this one's answers, logits of classes: the `places` largest of each image and their normaliser."""
-        if not 1 <= places <= min(self.outputs, 1024) or not 0 < temperature < math.inf:
-            raise pink.exception(-1, "a teacher gives between 1 and 1024 of its classes, at a temperature larger than 0")
+        if not 1 <= places <= min(self.outputs, 1024) or not torch.finfo(torch.float32).tiny <= temperature <= torch.finfo(torch.float32).max:
+            raise pink.exception(-1, "a teacher gives between 1 and 1024 of its classes, at a temperature of 2^-126 or larger that float32 holds")
         y = self(images)
         top = y.topk(places, dim=1)
         return Teacher(top.indices.to(torch.int32), top.values.contiguous(), torch.logsumexp(y / temperature, 1), float(temperature))

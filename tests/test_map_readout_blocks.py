@@ -71,6 +71,17 @@ def test_a_first_step_that_is_refused_sets_nothing(made):  # noqa: F811
     assert answers.steps == 2 and torch.equal(answers.level, level) and torch.equal(answers.parameters["radius"], radius)
 
 
+def test_teachers_are_of_temperatures_that_are_learned_at(made):  # noqa: F811
+    """learn() hands the temperature on as a float32 that is not subnormal: teach() gives no answers at any other."""
+    from pink_amd import pink
+    answers, _, torch = made
+    for temperature in (1e-40, 2.0 ** -127, 2.0 ** 128 * (1 - 2.0 ** -30), 2.0 ** 128, 1e39, -1.0):
+        with pytest.raises(pink.exception):
+            answers.teach(torch.rand(5, 6), 1, temperature)
+    for temperature in (2.0 ** -126, 1, 2.0 ** 127):
+        assert answers.teach(torch.rand(5, 6), 1, temperature).temperature == temperature
+
+
 def test_class_numbers_that_32_bits_do_not_hold_are_no_classes(made):  # noqa: F811
     from pink_amd import readout
     import ctypes
