@@ -2625,6 +2625,7 @@ int fail(pink_hip_ctx *ctx, int code, const std::string &msg)
 {
     if (ctx) ctx->err = msg;
     else g_create_error = msg;
+    if (code == PINK_HIP_ENOMEM || code == PINK_HIP_EDEVICE) (void)hipGetLastError();   // (returned here, it is no later launch's)
     return code;
 }
 

@@ -74,6 +74,7 @@ int fail(pink_hip_readout *r, int code, const char *what, const char *why = null
 {
     char *const to = r ? r->err : g_readout_error;
     std::snprintf(to, 320, why ? "%s: %s" : "%s", what, why);
+    if (code == PINK_HIP_ENOMEM || code == PINK_HIP_EDEVICE) (void)hipGetLastError();          // (returned here, it is no later launch's)
     return code;
 }
 

@@ -963,3 +963,26 @@ def test_a_reserved_workspace_is_enough_for_gradients_in_runs(gpu, f, h, o, most
 ])
 def test_distil_of_many_long_rows(gpu, t, v, k, temperature, rest, a, b, weighted, pad, bf16):  # noqa: F811
     test_distil(gpu, t, v, k, temperature, rest, a, b, weighted, pad, bf16)
+
+
+@pytest.mark.gpu
+def test_calls_after_one_that_found_no_memory(gpu):  # noqa: F811
+    """A workspace that there is no memory for is refused, and the calls after that are as they were."""
+    rng, (t, n) = np.random.default_rng(24), (40, 100)
+    x = rng.standard_normal((t, n)).astype(np.float32)
+    with capi.Readout(1) as ro:
+        at, y, again, dw = gpu.up(x), gpu.new((t, n), np.float32), gpu.new((t, n), np.float32), gpu.new(n, np.float32)
+        mean, scale = gpu.new(t, np.float32), gpu.new(t, np.float32)
+        ro.norm(at, t, n, None, None, EPSILON, y, mean, scale)
+        for _ in range(2):
+            with pytest.raises(capi.PinkError) as e:
+                ro.gated_reserve((2 ** 20, 2 ** 20, 2 ** 20, capi.ACT_SILU), 2 ** 30)            # (2^53 bytes)
+            assert e.value.status == -2 and "memory" in str(e.value), (e.value.status, str(e.value))
+            ro.norm(at, t, n, None, None, EPSILON, again)
+            with pytest.raises(capi.PinkError) as e:
+                capi.Context(4000, 1, 64, 10000, 1, False, 32)                                   # (1.6 TB of neurons)
+            assert e.value.status == -2, (e.value.status, str(e.value))
+            ro.norm(at, t, n, None, None, EPSILON, again)
+            ro.norm_backward(at, t, n, None, mean, scale, at, None, dw)                          # (with a workspace)
+        ro.synchronize()
+        assert np.array_equal(gpu.down(again, (t, n), np.float32), gpu.down(y, (t, n), np.float32))
