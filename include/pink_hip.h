@@ -424,14 +424,15 @@ typedef struct pink_hip_readout_gated_gradients {
 } pink_hip_readout_gated_gradients;
 /* residual may be NULL; y may be x, or residual with its stride.  What a backward pass needs is left in `saved` (pink_hip_readout_gated_saved_bytes bytes, which
  * is 0 for arguments that are refused; 256-byte aligned) unless it is NULL: h, rounded to the handle's element type, and
- * the two factors of its gradient, f(a) and f'(a) times the other, with bfloat16 to 16 bits of their significands.  Sums are float32.  With
+ * the two factors of its gradient, f(a) and f'(a) times the other, with bfloat16 cut off after 16 bits of their significands.  Sums are float32.  With
  * bfloat16 the second layer takes h rounded to it, but of up to 32 images without `saved` as two such values, so that y has one rounding: y of
  * the same images may differ in its last bits with and without `saved`, and among more images. */
 size_t pink_hip_readout_gated_saved_bytes(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, uint32_t images);
 int pink_hip_readout_gated(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, const void *dev_x, uint32_t images,
                            uint64_t x_stride, const pink_hip_readout_gated_weights *dev_weights, const void *dev_residual,
                            uint64_t residual_stride, void *dev_y, uint64_t y_stride, void *dev_saved);
-/* Gradients for those of y; x and weights as in the forward call that left `saved`.  (The residual's are those of y.)
+/* Gradients for those of y; x and weights as in the forward call that left `saved`.  (The residual's are those of y.)  Those of gate x +
+ * gate_bias and of up x + up_bias, which the biases' add up as float32, are rounded to the element type for the products that follow.
  * Those of the features may lie where x or dy does. */
 int pink_hip_readout_gated_backward(pink_hip_readout *readout, const pink_hip_readout_gated_config *config, const void *dev_x, uint32_t images,
                                     uint64_t x_stride, const pink_hip_readout_gated_weights *dev_weights, const void *dev_saved,
